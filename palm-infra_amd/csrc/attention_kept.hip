@@ -1,0 +1,271 @@
+// Causal grouped-query attention over the paged cache in which a query at position p sees the last `window` positions
+// (p - window < j <= p) and its sequence's first `kept` ones (j < kept): all arithmetic in 32-bit, any head size up to 512.  This is the
+// float32 mode, and what serves head sizes that the bfloat16 matrix-core kernels do not take.
+//
+//   s_j = scale q . k_j for the keys seen,  o = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),  m their maximum
+//
+// K is [pages, nkv, 64, hd], V is kept transposed, [pages, nkv, hd, 64].  What a run of queries sees is the pages of the first positions
+// that lie before the window's first page, then the pages from there on: they are walked as one row.  The pages between are not
+// looked at (they may have been given back).
+//
+// Both products run on the matrix cores in float32 (v_mfma_f32_16x16x4_f32: every product and sum an FMA), transposed as in the
+// bfloat16 kernels:  S^T[key, column] = K Q^T,  O^T[d, column] = V^T P^T.  A lane (r, g) holds row r of the first operand and column r of the
+// second at the places g of the four summed ones, and rows 4 g .. 4 g + 3 of column r of the result.  So a lane's four scores of a tile of 16 keys are
+// of keys 4 g .. 4 g + 3, and the products that follow take them as they are if their first operand is V^T at the same keys: one read of 16 bytes.
+// The 16 columns are (position, head): up to 16 heads of the kv head, of as many positions as fit.
+//
+// A block has four waves that take every fourth page, and a long row is cut into slices of several blocks, joined by a second kernel:
+// single tokens and short runs behind a long history have few columns and many pages.
+//
+// A key that a column does not see has weight zero there, but the products multiply its value all the same, and zero times an infinity or a
+// NaN (a page's uncleared end, a token whose activations overflowed and that has left the window) is NaN.  On a page where some column sees
+// less than all keys such values are taken as zero, and added again, as they are, to the columns that do see them.
+#include "mfma.h"
+
+PALM_DEFINE_LAST_ERROR()
+
+constexpr int KA_WAVES = 4;
+constexpr int KA_COLUMNS = 16;
+constexpr int KA_MAX_HD = 512;
+
+__device__ inline f32x4 mfma_16x16x4(float a, float b, f32x4 acc) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, acc, 0, 0, 0); }
+
+// Four consecutive elements from d on, widened; beyond hd zeros.  FOURS: hd is a multiple of four and rows start on their sizes.
+template <bool FOURS, typename T> __device__ inline f32x4 four_at(const T* row, int d, int hd) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (FOURS) {
+        if (d < hd) {
+            if constexpr (sizeof(T) == 4) {
+                const float4 four = *reinterpret_cast<const float4*>(row + d);
+                v = f32x4{four.x, four.y, four.z, four.w};
+            } else {
+                const uint2 u = *reinterpret_cast<const uint2*>(row + d);
+                v = f32x4{__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u)};
+            }
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (d + e < hd) v[e] = to_float(row[d + e]);
+    }
+    return v;
+}
+
+__device__ inline bool finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
+
+// The pages that queries at positions lo .. hi see, as one row of n.
+struct SeenRow {
+    int n, front, page_lo;       // of the row, the first `front` are the sequence's own first pages, the others the pages from page_lo on
+    __device__ SeenRow(int lo, int hi, int window, int kept) {
+        page_lo = max(0, lo - window + 1) / PAGE_TOKENS;
+        front = min((kept + PAGE_TOKENS - 1) / PAGE_TOKENS, page_lo);
+        n = front + hi / PAGE_TOKENS - page_lo + 1;
+    }
+    __device__ int page(int i) const { return i < front ? i : i - front + page_lo; }
+};
+
+// grid (kv heads * groups of heads, tiles of positions, sequences * slices).  A record of the workspace, for each (row, head, slice): maximum, sum, two
+// floats unused, then the unnormalised output.
+template <typename T, int DT, bool FOURS>
+__global__ __launch_bounds__(KA_WAVES * WAVE) void attention_kept_kernel(
+    const T* __restrict__ q, const T* __restrict__ k_cache, const T* __restrict__ v_cache, const int* __restrict__ block_table, int max_pages,
+    const int* __restrict__ seq_slot, const int* __restrict__ seq_start, const int* __restrict__ seq_new, const int* __restrict__ cu_new, int nh,
+    int nkv, int hd, float scale, int window, int kept, int heads, int slices, float* __restrict__ work, T* __restrict__ out) {
+    __shared__ f32x4 o_lds[KA_WAVES - 1][DT][WAVE];
+    __shared__ float m_lds[KA_WAVES - 1][WAVE], l_lds[KA_WAVES - 1][WAVE];
+    const int b = blockIdx.z / slices, slice = blockIdx.z % slices;
+    const int G = nh / nkv, n_groups = (G + heads - 1) / heads;
+    const int kvh = blockIdx.x / n_groups, group = blockIdx.x % n_groups;
+    const int here = min(heads, G - group * heads), rows = KA_COLUMNS / heads;      // heads and positions of the tile
+    const int n_new = seq_new[b], tile = blockIdx.y * rows;
+    if (tile >= n_new) return;
+    const int lane = threadIdx.x % WAVE, r = lane % 16, g = lane / 16;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+    const int start = seq_start[b], last = min(tile + rows, n_new) - 1;
+    const int qi = min(tile + r / heads, last);                                     // this lane's column
+    const bool valid = r / heads < rows && tile + r / heads <= last && r % heads < here;
+    const int head = kvh * G + group * heads + min(r % heads, here - 1);
+    const size_t row = (size_t)cu_new[b] + qi;
+    const int pos = start + qi, first = max(0, pos - window + 1);
+    const SeenRow seen(start + tile, start + last, window, kept);
+    const int per = (seen.n + slices - 1) / slices, begin = slice * per, end = min(seen.n, begin + per);
+    const int all_first = max(0, start + last - window + 1), all_last = start + tile;   // keys from all_first to all_last: seen by every column
+    const int* pages = block_table + (size_t)seq_slot[b] * max_pages;
+
+    f32x4 qv[DT], o[DT];
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+        qv[dt] = four_at<FOURS>(q + (row * nh + head) * hd, dt * 16 + 4 * g, hd);
+        o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    for (int i = begin + wave; i < end; i += KA_WAVES) {
+        const int page = seen.page(i), key0 = page * PAGE_TOKENS;
+        const size_t at = ((size_t)pages[page] * nkv + kvh) * PAGE_TOKENS * hd;
+        const T *kp = k_cache + at, *vp = v_cache + at;
+        const bool masked = all_last < key0 + PAGE_TOKENS - 1 || (all_first > key0 && kept < key0 + PAGE_TOKENS);   // the same in every lane
+        auto sees = [&](int in_page) { const int key = key0 + in_page; return key <= pos && (key >= first || key < kept); };
+        f32x4 s[4];
+        float mx = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                const f32x4 kd = four_at<FOURS>(kp + (size_t)(16 * t + r) * hd, dt * 16 + 4 * g, hd);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc = mfma_16x16x4(kd[e], qv[dt][e], acc);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                s[t][e] = !masked || sees(16 * t + 4 * g + e) ? acc[e] * scale : -INFINITY;
+                mx = fmaxf(mx, s[t][e]);
+            }
+        }
+        mx = fmaxf(mx, __shfl_xor(mx, 16, WAVE));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, WAVE));
+        const float m_new = fmaxf(m, mx), from = m_new == -INFINITY ? 0.f : m_new;      // (a column may see no key of its tile's first pages)
+        const float alpha = m == -INFINITY ? 0.f : expf(m - from);
+        m = m_new;
+        l *= alpha;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                s[t][e] = expf(s[t][e] - from);
+                l += s[t][e];
+            }
+        bool wild = false;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+            f32x4 acc = o[dt] * alpha;
+            const int d = dt * 16 + r;
+            const T* vrow = vp + (size_t)min(d, hd - 1) * PAGE_TOKENS;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                f32x4 vd = four_at<true>(vrow, 16 * t + 4 * g, PAGE_TOKENS);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (masked && !finite(vd[e])) { wild = true; vd[e] = 0.f; }
+                    if (d >= hd) vd[e] = 0.f;
+                    acc = mfma_16x16x4(vd[e], s[t][e], acc);
+                }
+            }
+            o[dt] = acc;
+        }
+        if (__any(wild)) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int d = dt * 16 + 4 * g + e;
+                    for (int j = 0; j < PAGE_TOKENS && d < hd; ++j) {
+                        const float v = to_float(vp[(size_t)d * PAGE_TOKENS + j]);
+                        if (!finite(v) && sees(j)) o[dt][e] += v;
+                    }
+                }
+        }
+    }
+    l += __shfl_xor(l, 16, WAVE);
+    l += __shfl_xor(l, 32, WAVE);
+    if (wave > 0) {
+        m_lds[wave - 1][lane] = m;
+        l_lds[wave - 1][lane] = l;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o_lds[wave - 1][dt][lane] = o[dt];
+    }
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int w = 0; w < KA_WAVES - 1; ++w) {
+        const float mw = m_lds[w][lane], top = fmaxf(m, mw);
+        if (mw == -INFINITY) continue;                          // it saw none of the column's keys
+        const float mine = m == -INFINITY ? 0.f : expf(m - top), its = expf(mw - top);
+        l = l * mine + l_lds[w][lane] * its;
+        m = top;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt] = o[dt] * mine + o_lds[w][dt][lane] * its;
+    }
+    if (!valid) return;
+    if (slices > 1) {
+        float* record = work + ((row * nh + head) * slices + slice) * (hd + 4);
+        if (g == 0) { record[0] = m; record[1] = l; }
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (dt * 16 + 4 * g + e < hd) record[4 + dt * 16 + 4 * g + e] = o[dt][e];
+        return;
+    }
+    T* to = out + (row * nh + head) * hd;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (dt * 16 + 4 * g + e < hd) to[dt * 16 + 4 * g + e] = from_float<T>(o[dt][e] / l);
+}
+
+// A wave for each (row, head): the slices' records in their order.
+template <typename T>
+__global__ __launch_bounds__(WAVE) void attention_kept_join_kernel(const float* __restrict__ work, int slices, int hd, T* __restrict__ out) {
+    const float* w = work + (size_t)blockIdx.x * slices * (hd + 4);
+    const int lane = threadIdx.x;
+    float m = -INFINITY, l = 0.f;
+    for (int s = lane; s < slices; s += WAVE) m = fmaxf(m, w[(size_t)s * (hd + 4)]);
+    m = wave_max(m);
+    for (int s = lane; s < slices; s += WAVE) l += w[(size_t)s * (hd + 4) + 1] * expf(w[(size_t)s * (hd + 4)] - m);
+    l = wave_sum(l);
+    for (int d = lane; d < hd; d += WAVE) {
+        float o = 0.f;
+        for (int s = 0; s < slices; ++s) {
+            const float ms = w[(size_t)s * (hd + 4)];
+            if (ms != -INFINITY) o += w[(size_t)s * (hd + 4) + 4 + d] * expf(ms - m);       // (an empty slice has no output)
+        }
+        out[(size_t)blockIdx.x * hd + d] = from_float<T>(o / l);
+    }
+}
+
+// heads of a kv head that a tile's columns are
+static int heads_of_tile(int nh, int nkv) { return nh / nkv < KA_COLUMNS ? nh / nkv : KA_COLUMNS; }
+
+// Into how many slices a row of pages is cut: until the launch has two blocks a compute unit, and not into less than a page for each wave.
+PALM_API int palm_attention_kept_slices(int n_seqs, int max_new, int max_total, int nh, int nkv, int window, int kept) {
+    PALM_CHECK(n_seqs > 0 && max_new > 0 && max_total >= max_new && nh > 0 && nkv > 0 && nh % nkv == 0 && window > 0 && kept >= 0,
+               "attention_kept: seqs=%d max_new=%d max_total=%d heads=%d kv=%d window=%d kept=%d", n_seqs, max_new, max_total, nh, nkv, window, kept);
+    const int heads = heads_of_tile(nh, nkv), rows = KA_COLUMNS / heads;
+    const long long blocks = (long long)nkv * ((nh / nkv + heads - 1) / heads) * ((max_new + rows - 1) / rows) * n_seqs;
+    const long long keys = (long long)window + rows + kept < max_total ? (long long)window + rows + kept : max_total;
+    const long long most = ((keys + PAGE_TOKENS - 1) / PAGE_TOKENS + KA_WAVES - 1) / KA_WAVES, wanted = (512 + blocks - 1) / blocks;
+    return (int)(wanted < most ? wanted : most);
+}
+
+// dtype of q, the cache and out: 0 float32, 1 bfloat16.  work: rows * nh * slices * (hd + 4) floats where there is more than one slice.
+PALM_API int palm_attention_kept(hipStream_t stream, const void* q, int dtype, const void* k_cache, const void* v_cache, const int* block_table,
+                                 int max_pages, const int* seq_slot, const int* seq_start, const int* seq_new, const int* cu_new, int n_seqs, int rows,
+                                 int max_new, int nh, int nkv, int hd, float scale, int window, int kept, int slices, float* work, void* out) {
+    PALM_CHECK(n_seqs >= 0 && max_new >= 0 && rows >= 0 && nh > 0 && nkv > 0 && nh % nkv == 0, "attention_kept: seqs=%d max_new=%d heads=%d kv=%d", n_seqs,
+               max_new, nh, nkv);
+    PALM_CHECK(hd > 0 && hd <= KA_MAX_HD, "attention_kept: head size %d is not within 1 to %d", hd, KA_MAX_HD);
+    PALM_CHECK(window > 0 && kept >= 0 && max_pages > 0, "attention_kept: window=%d kept=%d max_pages=%d", window, kept, max_pages);
+    PALM_CHECK(slices >= 1 && (slices == 1 || work), "attention_kept: %d slices need a workspace", slices);
+    if (n_seqs == 0 || max_new == 0 || rows == 0) return 0;
+    const int heads = heads_of_tile(nh, nkv), per = KA_COLUMNS / heads;
+    const long long x = (long long)nkv * ((nh / nkv + heads - 1) / heads), y = (max_new + per - 1) / per, z = (long long)n_seqs * slices;
+    PALM_CHECK(y <= 65535 && z <= 65535, "attention_kept: %d new tokens of %d sequences in %d slices are more than one launch takes", max_new, n_seqs, slices);
+    const dim3 grid((unsigned)x, (unsigned)y, (unsigned)z);
+    const bool fours = hd % 4 == 0 && ((uintptr_t)q | (uintptr_t)k_cache) % 16 == 0;
+    PALM_CHECK((uintptr_t)v_cache % 16 == 0, "attention_kept: values do not start on 16 bytes");
+#define PALM_KEPT(DT, FOURS) attention_kept_kernel<T, DT, FOURS><<<grid, KA_WAVES * WAVE, 0, stream>>>((const T*)q, (const T*)k_cache, (const T*)v_cache, \
+        block_table, max_pages, seq_slot, seq_start, seq_new, cu_new, nh, nkv, hd, scale, window, kept, heads, slices, work, (T*)out)
+    PALM_DTYPE_SWITCH(dtype, T,
+        if (!fours) { if (hd <= 128) PALM_KEPT(8, false); else PALM_KEPT(32, false); }
+        else if (hd <= 32) PALM_KEPT(2, true);
+        else if (hd <= 64) PALM_KEPT(4, true);
+        else if (hd <= 128) PALM_KEPT(8, true);
+        else if (hd <= 256) PALM_KEPT(16, true);
+        else PALM_KEPT(32, true);
+        PALM_LAUNCHED();
+        if (slices > 1) { attention_kept_join_kernel<T><<<rows * nh, WAVE, 0, stream>>>(work, slices, hd, (T*)out); PALM_LAUNCHED(); });
+#undef PALM_KEPT
+    return 0;
+}

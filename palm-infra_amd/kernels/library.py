@@ -24,6 +24,9 @@ Libraries:
   ``gla_d<N>``          gated linear attention (a decay for every key channel and token), compiled for key sizes up to N
   ``delta_head_d<N>``   the delta rule with one decay a head behind short convolutions, compiled for key sizes up to N
   ``streams``           a residual stream in several copies with learned weights between them, and its norms
+  ``attention_kept``    attention with a window and first positions that stay visible, in 32-bit, any head size
+  ``pages``             pages of the cache copied to other pages, in all layers at once
+  ``logprobs``          log probabilities of given tokens, entropies and the likeliest tokens
   ``mlstm``             a matrix memory with input and forget gates per head and token
   ``latent_attention_k<K>_v<V>``  attention over compressed rows on the matrix cores, compiled for rows up to 32 K and
                         latents up to 16 V
@@ -82,6 +85,9 @@ LATENT_SOURCES = ["latent_attention.hip"]
 FEEDFORWARD_SOURCES = ["moe.hip", "moe_few.hip", "moe_ring.hip", "moe_grouped.hip", "activation.hip"]
 STREAMS_SOURCES = ["streams.hip"]
 MLSTM_SOURCES = ["mlstm.hip"]
+ATTENTION_KEPT_SOURCES = ["attention_kept.hip"]
+PAGES_SOURCES = ["pages.hip"]
+LOGPROBS_SOURCES = ["logprobs.hip"]
 RECURRENT_SOURCES = ["retention.hip"]
 GLA_SOURCES = ["gla.hip"]
 DELTA_HEAD_SOURCES = ["delta_head.hip"]
@@ -238,6 +244,12 @@ def _spec(name: str):
         return FEEDFORWARD_SOURCES, ()
     if name == "streams":
         return STREAMS_SOURCES, ()
+    if name == "attention_kept":
+        return ATTENTION_KEPT_SOURCES, ()
+    if name == "pages":
+        return PAGES_SOURCES, ()
+    if name == "logprobs":
+        return LOGPROBS_SOURCES, ()
     if name == "mlstm":
         return MLSTM_SOURCES, ()
     if name.startswith("gla_d"):

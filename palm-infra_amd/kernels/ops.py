@@ -1225,6 +1225,19 @@ _STREAMS_SIGNATURES = {
     "palm_streams_mix_norm": [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
                               c_void_p, c_float, c_float, c_void_p, c_int, c_int, c_void_p, c_int],
 }
+_ATTENTION_KEPT_SIGNATURES = {
+    "palm_attention_kept": [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                            c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_void_p],
+    "palm_attention_kept_slices": [c_int, c_int, c_int, c_int, c_int, c_int, c_int],
+}
+_PAGES_SIGNATURES = {
+    "palm_copy_pages": [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p,
+                        c_int],
+}
+_LOGPROBS_SIGNATURES = {
+    "palm_token_logprobs": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p],
+    "palm_token_logprobs_work": [c_int, c_int, c_int],
+}
 _MLSTM_SIGNATURES = {
     "palm_mlstm_pad": [c_int],
     "palm_mlstm": [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_float, c_float, c_void_p, c_float,
@@ -1289,6 +1302,20 @@ def streams_lib():
 
 def mlstm_lib():
     return _small("mlstm", _MLSTM_SIGNATURES)
+
+
+def attention_kept_lib():
+    return _small("attention_kept", _ATTENTION_KEPT_SIGNATURES)
+
+
+def pages_lib():
+    return _small("pages", _PAGES_SIGNATURES)
+
+
+def logprobs_lib():
+    lib = _small("logprobs", _LOGPROBS_SIGNATURES)
+    lib.palm_token_logprobs_work.restype = c_longlong
+    return lib
 
 
 def padded_key_size(dim: int) -> int:
@@ -2815,3 +2842,172 @@ def mlstm(rows: torch.Tensor, gates: torch.Tensor, gate_bias: torch.Tensor | Non
                  _p(m_state), _p(ctx.seq_slot), _p(ctx.seq_new), _p(ctx.cu_new), ctx.n_seqs, heads, dim, vdim, _p(out), int(ctx.max_new),
                  chunk, _p(starts), _p(keeps), n, _p(qk), _p(coef))
     return out
+
+
+# ---- attention with a window and first positions that stay visible ------------------------------------------------------
+
+@functools.lru_cache(maxsize=1024)
+def _kept_slices(n_seqs: int, max_new: int, max_total: int, nh: int, nkv: int, window: int, kept: int) -> int:
+    n = attention_kept_lib().palm_attention_kept_slices(n_seqs, max_new, max_total, nh, nkv, window, kept)
+    _need(n >= 1, "attention_kept: sizes that no launch has")
+    return n
+
+
+def attention_kept_exact(q: torch.Tensor, k_cache, v_cache, block_table, seq_slot, seq_start, seq_new, cu_new, max_new: int, max_total: int, nh: int,
+                         nkv: int, hd: int, scale: float, window: int, kept: int) -> torch.Tensor:
+    """``attention_kept`` in 32-bit arithmetic, for float32 and bfloat16 and any head size up to 512."""
+    n, B = q.shape[0], seq_slot.shape[0]
+    out = torch.empty_like(q)
+    if n == 0 or B == 0 or max_new == 0:
+        return out
+    slices = _kept_slices(B, max_new, max_total, nh, nkv, window, kept)
+    work = torch.empty((n * nh * slices * (hd + 4),), dtype=F32, device=q.device) if slices > 1 else None
+    _call_on(q.device, attention_kept_lib(), "palm_attention_kept", _p(q), _code(q, "attention_kept q"), _p(k_cache), _p(v_cache), _p(block_table),
+             block_table.shape[1], _p(seq_slot), _p(seq_start), _p(seq_new), _p(cu_new), B, n, int(max_new), nh, nkv, hd, float(scale), window, kept,
+             slices, _p(work), _p(out))
+    return out
+
+
+def attention_kept(q: torch.Tensor, k_cache, v_cache, block_table, seq_slot, seq_start, seq_new, cu_new, max_new: int, max_total: int, nh: int,
+                   nkv: int, hd: int, scale: float, window: int, kept: int) -> torch.Tensor:
+    """Causal attention of the step's queries over the cache of which a query at position p sees the last ``window`` positions (p - window < j <= p) and the
+    sequence's first ``kept`` ones (j < kept): what keeps a stream without an end within a bounded number of pages.
+
+    q [n, nh hd]; sequence b has seq_new[b] queries (none, if it is zero) from row cu_new[b] on, at positions seq_start[b] and up, whose keys and values are
+    in the cache; ``max_new`` and ``max_total``: the most new tokens of a sequence and the longest sequence with them, or more.  Pages that no query of
+    the step sees are not read, whatever the page table says of them; what masked places hold (an infinity, a NaN) does not show."""
+    what = "attention_kept"
+    _dev(what, q, k_cache, v_cache, block_table, seq_slot, seq_start, seq_new, cu_new)
+    _i32(what, block_table, seq_slot, seq_start, seq_new, cu_new)
+    window, kept, max_new, max_total = int(window), int(kept), int(max_new), int(max_total)
+    if not (nh > 0 and nkv > 0 and nh % nkv == 0):
+        raise KernelError(f"{what}: {nh} heads are not a multiple of {nkv} kv heads")
+    if not (q.dim() == 2 and q.shape[1] == nh * hd):
+        raise KernelError(f"{what}: q {tuple(q.shape)} is not [n, {nh}*{hd}]")
+    _check_cache(what, k_cache, v_cache, block_table, nkv, hd)
+    if not (k_cache.dtype == q.dtype):
+        raise KernelError(f"{what}: cache is {k_cache.dtype}, queries are {q.dtype}")
+    _code(q, f"{what} q")
+    B = seq_slot.shape[0]
+    _need(seq_slot.dim() == 1 and seq_start.shape == (B,) and seq_new.shape == (B,) and cu_new.shape == (B + 1,),
+          "attention_kept: per-sequence arrays differ in length")
+    if not (window >= 1 and kept >= 0 and window < 1 << 30 and kept < 1 << 30):
+        raise KernelError(f"{what}: a window of {window} positions and {kept} first ones: at least one, and none or more")
+    if not (0 <= max_new <= max_total <= block_table.shape[1] * PAGE_TOKENS):
+        raise KernelError(f"{what}: {max_new} new tokens in sequences of up to {max_total}; the page table has room for {block_table.shape[1] * PAGE_TOKENS}")
+    return attention_kept_exact(q, k_cache, v_cache, block_table, seq_slot, seq_start, seq_new, cu_new, max_new, max_total, nh, nkv, hd, scale, window, kept)
+
+
+# ---- pages of the cache copied to other pages (library ``pages``) ----------------------------------------------------
+
+def _call_on(device: torch.device, lib, fn_name: str, *args) -> None:
+    """``library.call`` with ``device`` current, on torch's current stream there."""
+    if device.index == torch._C._cuda_getDevice():
+        library.call(lib, fn_name, _stream(), *args)
+        return
+    with torch.cuda.device(device):
+        library.call(lib, fn_name, _stream(), *args)
+
+
+def _host_ints(what: str, name: str, values) -> array:
+    try:
+        return array("i", values)
+    except (TypeError, OverflowError) as e:
+        raise KernelError(f"{what}: {name} is no list of whole numbers ({e})") from None
+
+
+def _copy(what: str, storages, layers: int, pages: int, page_tokens: int, src, dst, tokens) -> None:
+    """``storages``: (tensor, runs of a page, elements of a run, elements a position) each."""
+    s, d = _host_ints(what, "src", src), _host_ints(what, "dst", dst)
+    t = None if tokens is None else _host_ints(what, "tokens", tokens)
+    if len(s) != len(d) or (t is not None and len(t) != len(s)):
+        raise KernelError(f"{what}: {len(s)} sources, {len(d)} destinations" + ("" if t is None else f", {len(t)} counts of positions"))
+    if len(s) == 0 or layers == 0:
+        return
+    args = []
+    for tensor, runs, run, position in storages:
+        if tensor.element_size() not in (2, 4):
+            raise KernelError(f"{what}: elements of {tensor.element_size()} bytes")
+        args += [_p(tensor), runs, run * tensor.element_size(), position * tensor.element_size()]
+    args += [None, 0, 0, 0] * (2 - len(storages))
+    _call_on(storages[0][0].device, pages_lib(), "palm_copy_pages", *args, layers, pages, page_tokens, s.buffer_info()[0], d.buffer_info()[0],
+             None if t is None else t.buffer_info()[0], len(s))
+
+
+def copy_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, src, dst, tokens=None) -> None:
+    """Keys and values of page ``src[i]`` to page ``dst[i]``, in all layers: k_cache [layers, pages, kv heads, 64, head size], v_cache [layers,
+    pages, kv heads, head size, 64] (head counts and sizes of its own, if it has).  ``tokens[i]``: of the page's first so many positions (None: of all);
+    the destination's positions behind them stay as they are.  ``src``, ``dst``, ``tokens`` are lists on the host, as a page table has them.
+    A page may go to several others; one that is written twice, or both read and written, is refused."""
+    what = "copy_pages"
+    _dev(what, k_cache, v_cache)
+    for t in (k_cache, v_cache):
+        _code(t, what)
+    if not (k_cache.dim() == 5 and k_cache.shape[3] == PAGE_TOKENS and k_cache.numel() > 0):
+        raise KernelError(f"{what}: keys {tuple(k_cache.shape)} are not [layers, pages, kv heads, {PAGE_TOKENS}, head size]")
+    if not (v_cache.dim() == 5 and v_cache.shape[4] == PAGE_TOKENS and v_cache.shape[:2] == k_cache.shape[:2] and v_cache.dtype == k_cache.dtype
+            and v_cache.numel() > 0):
+        raise KernelError(f"{what}: values {tuple(v_cache.shape)} {v_cache.dtype} are not [layers, pages, heads, size, {PAGE_TOKENS}] of the keys' "
+                          f"{tuple(k_cache.shape)} {k_cache.dtype} (values are kept transposed)")
+    layers, pages, heads, _, hd = k_cache.shape
+    _copy(what, [(k_cache, heads, PAGE_TOKENS * hd, hd), (v_cache, v_cache.shape[2] * v_cache.shape[3], PAGE_TOKENS, 1)], layers, pages, PAGE_TOKENS,
+          src, dst, tokens)
+
+
+def copy_rows(data: torch.Tensor, src, dst, tokens=None) -> None:
+    """``copy_pages`` for pages of one row a position: data [layers, pages, 64, *row]."""
+    what = "copy_rows"
+    _dev(what, data)
+    if not (data.dim() >= 3 and data.shape[2] == PAGE_TOKENS and data.numel() > 0):
+        raise KernelError(f"{what}: rows {tuple(data.shape)} are not [layers, pages, {PAGE_TOKENS}, ..]")
+    row = data[0, 0, 0].numel()
+    _copy(what, [(data, 1, PAGE_TOKENS * row, row)], data.shape[0], data.shape[1], PAGE_TOKENS, src, dst, tokens)
+
+
+def copy_states(data: torch.Tensor, src, dst) -> None:
+    """The state of slot ``src[i]`` to slot ``dst[i]``, in all layers: data [layers, slots, *shape]."""
+    what = "copy_states"
+    _dev(what, data)
+    if not (data.dim() >= 2 and data.numel() > 0):
+        raise KernelError(f"{what}: states {tuple(data.shape)} are not [layers, slots, ..]")
+    size = data[0, 0].numel()
+    _copy(what, [(data, 1, size, size)], data.shape[0], data.shape[1], 1, src, dst, None)
+
+
+# ---- how likely tokens are (library ``logprobs``) ----------------------------------------------------------------------
+
+LOGPROBS_MOST = 64
+
+
+@functools.lru_cache(maxsize=256)
+def _logprobs_work(rows: int, V: int, top: int) -> int:
+    return logprobs_lib().palm_token_logprobs_work(rows, V, top)
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top: int = 0):
+    """Of rows of logits [rows, vocab] float32: the log probability of each row's token (``tokens`` [rows] int32; None: none is asked for),
+    the entropy of each row's distribution, and its ``top`` likeliest tokens (64 at most), the likeliest first and equal ones by their number, with their
+    log probabilities: (given [rows] or None, entropy [rows], ids [rows, top] int32, best [rows, top]), float32 but the ids.
+
+    A token outside the vocabulary has NaN.  Minus infinity is a token that cannot come; a row that leaves no token, or holds a NaN or plus infinity,
+    has NaN for all its results (its ids are then some tokens of the vocabulary)."""
+    what = "token_logprobs"
+    _dev(what, logits, tokens)
+    _i32(what, tokens)
+    if not (logits.dim() == 2 and logits.dtype == F32):
+        raise KernelError(f"{what}: logits {tuple(logits.shape)} {logits.dtype} are not float32 [rows, vocab]")
+    n, V = logits.shape
+    if not (tokens is None or tokens.shape == (n,)):
+        raise KernelError(f"{what}: tokens {tuple(tokens.shape)} for {n} rows")
+    top = int(top)
+    if not (0 <= top <= min(LOGPROBS_MOST, V)):
+        raise KernelError(f"{what}: the {top} likeliest of {V} tokens ({LOGPROBS_MOST} at most)")
+    dev = logits.device
+    out = torch.empty((n * (2 + top),), dtype=F32, device=dev)
+    given, entropy, best = out[:n], out[n:2 * n], out[2 * n:].view(n, top)
+    ids = torch.empty((n, top), dtype=torch.int32, device=dev)
+    if n:
+        needed = _logprobs_work(n, V, top)
+        work = torch.empty((needed,), dtype=torch.uint8, device=dev) if needed else None
+        _call_on(dev, logprobs_lib(), "palm_token_logprobs", _p(logits), n, V, _p(tokens), top, _p(work), needed, _p(given), _p(entropy), _p(ids), _p(best))
+    return (given if tokens is not None else None), entropy, ids, best

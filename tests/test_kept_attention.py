@@ -1,0 +1,218 @@
+"""Attention with a window and first positions that stay visible, against its definition in 64 bits.
+
+The pages that no query sees are one page full of NaN, and so is what lies behind each sequence's end: what is read of them shows.
+
+Tolerances, for an output o = sum w v of weights that sum to one.  A score is a sum of hd products, off by at most hd 2^-24 sum |q k| scale (each
+of hd roundings relative to a partial sum), which scales its weight by e^(2 of those) at most, with the maximum's own; exponentials are off by
+a few 2^-24 and a sum of N of them by N 2^-24.  bfloat16 on the matrix cores: a weight is rounded by 2^-8 relative to it, in the sum of weights too, and the
+result once more by 2^-8 of itself."""
+import math
+
+import pytest
+import torch
+
+DEV = "cuda:0"
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from palm_infra_amd.kernels import ops
+    return ops
+
+
+class Case:
+    """A step over a cache: ``seqs`` are (tokens before, new tokens)."""
+
+    def __init__(self, seqs, nh, nkv, hd, window, kept, dtype, seed=0, q_scale=2.0):
+        g = torch.Generator().manual_seed(seed)
+        self.seqs, self.nh, self.nkv, self.hd, self.window, self.kept, self.dtype = seqs, nh, nkv, hd, window, kept, dtype
+        lists = []
+        for start, new in seqs:
+            pages, first = (start + new + 63) // 64, max(0, start - window + 1) // 64
+            lists.append([p for p in range(pages) if new and (p < (kept + 63) // 64 or p >= first)])
+        n_pages = sum(map(len, lists))
+        width = max(max((s + n + 63) // 64 for s, n in seqs), 1)
+        order = torch.randperm(n_pages, generator=g).tolist()
+        slots = torch.randperm(len(seqs) + 2, generator=g).tolist()[:len(seqs)]
+        self.table = torch.full((len(seqs) + 2, width), n_pages, dtype=torch.int32)
+        self.k = torch.randn(n_pages + 1, nkv, 64, hd, generator=g).to(dtype)
+        self.v = torch.randn(n_pages + 1, nkv, hd, 64, generator=g).to(dtype)
+        self.k[n_pages], self.v[n_pages] = math.nan, math.nan
+        for slot, pages, (start, new) in zip(slots, lists, seqs):
+            for p in pages:
+                self.table[slot, p] = order.pop()
+            if pages and (start + new) % 64:
+                last = self.table[slot, pages[-1]]
+                self.k[last, :, (start + new) % 64:] = math.nan
+                self.v[last, :, :, (start + new) % 64:] = math.nan
+        self.cu = [0]
+        for _, new in seqs:
+            self.cu.append(self.cu[-1] + new)
+        self.q = (torch.randn(self.cu[-1], nh * hd, generator=g) * q_scale).to(dtype)
+        self.slots = slots
+
+    def place(self, b, j):
+        return int(self.table[self.slots[b], j // 64]), j % 64
+
+    def run(self, ops, fn=None, **more):
+        i = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+        fn = fn or ops.attention_kept
+        return fn(self.q.to(DEV), self.k.to(DEV), self.v.to(DEV), self.table.to(DEV), i(self.slots), i([s for s, _ in self.seqs]),
+                  i([n for _, n in self.seqs]), i(self.cu), max(n for _, n in self.seqs), max(s + n for s, n in self.seqs), self.nh, self.nkv,
+                  self.hd, self.hd ** -0.5, self.window, self.kept, **more).cpu()
+
+    def plain(self):
+        """The results and how far a kernel's may be from them."""
+        out = torch.zeros(self.q.shape, dtype=torch.float64)
+        off = torch.zeros_like(out)
+        G, hd, scale = self.nh // self.nkv, self.hd, self.hd ** -0.5
+        rounding = 2.0 ** -8 if self.dtype == BF16 else 2.0 ** -24
+        for b, (start, new) in enumerate(self.seqs):
+            for i in range(new):
+                p = start + i
+                keys = torch.arange(p + 1)
+                keys = keys[(keys > p - self.window) | (keys < self.kept)]
+                page, at = self.table[self.slots[b]].long()[keys // 64], keys % 64
+                row = self.cu[b] + i
+                q = self.q[row].double().view(self.nh, hd)
+                k, v = self.k[page, :, at].double(), self.v[page, :, :, at].double()     # [keys, nkv, hd]
+                k, v = k.repeat_interleave(G, 1), v.repeat_interleave(G, 1)
+                s = (q * k).sum(-1) * scale                                           # [keys, nh]
+                w = torch.softmax(s, 0)[..., None]
+                o = (w * v).sum(0)
+                ds = hd * 2.0 ** -24 * ((q * k).abs().sum(-1) * scale).amax(0)[:, None]
+                weigh = (w * v.abs()).sum(0)
+                e = weigh * (4 * ds + (len(keys) + 16) * 2.0 ** -24 + (2 * rounding if self.dtype == BF16 else 0)) + rounding * (o.abs() + weigh * 2 * rounding)
+                out[row], off[row] = o.reshape(-1), e.reshape(-1)
+        return out, off
+
+    def check(self, got):
+        want, off = self.plain()
+        assert got.dtype == self.dtype and got.shape == self.q.shape
+        same = torch.where(torch.isfinite(want), (got.double() - want).abs() <= off, (got.double() == want) | (got.isnan() & want.isnan()))
+        assert bool(same.all()), (int((~same).sum()), float((got.double() - want).abs().nan_to_num(9e9).max()))
+
+
+SHAPES = [(4, 2, 16), (5, 1, 64), (8, 8, 128), (6, 2, 20), (3, 1, 6), (40, 2, 32), (2, 1, 80), (4, 4, 192), (10, 2, 128), (4, 1, 512)]
+LONG = [(4, 2, 64), (8, 2, 128)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("nh,nkv,hd", SHAPES)
+@pytest.mark.parametrize("window,kept", [(1, 0), (1, 1), (5, 4), (64, 64), (100, 3), (70, 130), (4096, 4)])
+def test_prompts_pieces_and_single_tokens(ops, nh, nkv, hd, window, kept, dtype):
+    case = Case([(0, 1), (0, 70), (250, 17), (130, 0), (400, 1), (64, 64), (63, 2)], nh, nkv, hd, window, kept, dtype, seed=hd + window)
+    case.check(case.run(ops))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("nh,nkv,hd", SHAPES)
+@pytest.mark.parametrize("window,kept", [(1, 0), (1, 1), (5, 4), (64, 64), (100, 3), (70, 130), (4096, 4)])
+def test_a_step_of_single_tokens(ops, nh, nkv, hd, window, kept, dtype):
+    case = Case([(n, 1) for n in (0, 1, 63, 64, 65, 127, 500, 301, 200)], nh, nkv, hd, window, kept, dtype, seed=hd + window)
+    case.check(case.run(ops))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("nh,nkv,hd", LONG)
+@pytest.mark.parametrize("seqs", [[(5000, 1)], [(3000, 1), (70, 1), (2047, 1)], [(3000, 5)], [(0, 700)], [(900, 300), (0, 65)]])
+@pytest.mark.parametrize("window,kept", [(1000, 4), (2048, 129), (333, 64)])
+def test_long_rows_of_pages(ops, nh, nkv, hd, seqs, window, kept, dtype):
+    case = Case(seqs, nh, nkv, hd, window, kept, dtype, seed=len(seqs))
+    case.check(case.run(ops))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("nh,nkv,hd", [(4, 2, 16), (8, 2, 64), (8, 2, 128), (6, 2, 20)])
+@pytest.mark.parametrize("seqs", [[(0, 200)], [(300, 30), (290, 1)], [(310, 1), (200, 1)]])
+def test_what_masked_places_hold_does_not_show(ops, nh, nkv, hd, seqs, dtype):
+    """Infinities and NaN in keys and values: a query that sees such a value has it in its result, the others do not."""
+    case = Case(seqs, nh, nkv, hd, 90, 3, dtype, seed=5)
+    for b, (start, new) in enumerate(seqs):
+        for j, what in ((20, math.inf), (100, math.nan), (150, -math.inf), (215, math.inf), (start + new - 2, math.nan)):
+            page, at = case.place(b, j) if j < start + new else (len(case.k) - 1, 0)
+            if page == len(case.k) - 1:
+                continue
+            case.v[page, 0, :3, at] = what
+        for j in (40, 120):                                     # keys too, where no query's window reaches them
+            if j < start - 90 and case.place(b, j)[0] != len(case.k) - 1:
+                case.k[case.place(b, j)[0], :, j % 64] = math.nan
+                case.v[case.place(b, j)[0], :, :, j % 64] = math.inf
+    case.check(case.run(ops))
+
+
+@pytest.mark.gpu
+def test_without_first_positions_it_is_the_window_alone(ops):
+    """The framework's other window, on the same step."""
+    case = Case([(0, 90), (200, 33), (77, 1)], 8, 2, 64, 50, 0, F32, seed=3)
+    i = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    case.k[-1], case.v[-1] = 0, 0
+    other = ops.attention_exact(case.q.to(DEV), case.k.to(DEV), case.v.to(DEV), case.table.to(DEV), i(case.slots), i([0, 200, 77]), i([90, 33, 1]),
+                                i(case.cu), 90, 8, 2, 64, 64 ** -0.5, 50).cpu()
+    assert torch.allclose(case.run(ops), other, rtol=1e-4, atol=1e-5)
+
+
+@pytest.mark.gpu
+def test_a_captured_step_replays_with_new_contents(ops):
+    case = Case([(500, 1), (70, 1), (1500, 1)], 8, 2, 128, 300, 4, BF16, seed=8)
+    other = Case([(500, 1), (70, 1), (1500, 1)], 8, 2, 128, 300, 4, BF16, seed=9)
+    i = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    held = [t.to(DEV) for t in (case.q, case.k, case.v, case.table)] + [i(case.slots), i([500, 70, 1500]), i([1, 1, 1]), i(case.cu)]
+    args = (1, 1501, 8, 2, 128, 128 ** -0.5, 300, 4)
+    ops.attention_kept(*held, *args)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.attention_kept(*held, *args)
+    for turn in range(4):
+        now = (case, other)[turn % 2]
+        for t, new in zip(held, (now.q, now.k, now.v, now.table, torch.tensor(now.slots, dtype=torch.int32))):
+            t.copy_(new.to(DEV))
+        graph.replay()
+        torch.cuda.synchronize()
+        now.check(out.cpu())
+        now.check(ops.attention_kept(*held, *args).cpu())
+
+
+def _refused(ops, match, **change):
+    z = lambda *shape, dtype=torch.int32: torch.zeros(shape, dtype=dtype)
+    a = dict(q=z(3, 8 * 16, dtype=F32), k_cache=z(5, 2, 64, 16, dtype=F32), v_cache=z(5, 2, 16, 64, dtype=F32), block_table=z(3, 4), seq_slot=z(2), seq_start=z(2),
+             seq_new=z(2), cu_new=z(3), max_new=2, max_total=200, nh=8, nkv=2, hd=16, scale=0.25, window=64, kept=4)
+    a.update(change)
+    with pytest.raises(ops.KernelError, match=match):
+        ops.attention_kept(**a)
+
+
+def test_refusals(ops, monkeypatch):
+    _refused(ops, "GPU only")
+    monkeypatch.setattr(ops, "_dev", lambda what, *tensors: None)       # the checks behind that one need no GPU
+    z = lambda *shape, dtype=torch.int32: torch.zeros(shape, dtype=dtype)
+    _refused(ops, "not a multiple", nh=7)
+    _refused(ops, "is not \\[n, 8\\*16\\]", q=z(3, 100, dtype=F32))
+    _refused(ops, "key cache", k_cache=z(5, 2, 32, 16, dtype=F32))
+    _refused(ops, "value cache", v_cache=z(5, 2, 64, 16, dtype=F32))
+    _refused(ops, "page table", block_table=z(12))
+    _refused(ops, "queries are torch.bfloat16", q=z(3, 8 * 16, dtype=BF16))
+    _refused(ops, "neither float32 nor bfloat16", q=z(3, 128, dtype=torch.float16), k_cache=z(5, 2, 64, 16, dtype=torch.float16),
+             v_cache=z(5, 2, 16, 64, dtype=torch.float16))
+    _refused(ops, "differ in length", seq_new=z(3))
+    _refused(ops, "differ in length", cu_new=z(2))
+    _refused(ops, "window of 0", window=0)
+    _refused(ops, "-1 first ones", kept=-1)
+    _refused(ops, "room for 256", max_total=257)
+    _refused(ops, "3 new tokens", max_new=3, max_total=2)
+    _refused(ops, "int32", seq_slot=z(2, dtype=torch.int64))
+
+
+def test_slices_fill_the_chip_and_leave_no_wave_without_a_page(ops):
+    n = ops.attention_kept_lib().palm_attention_kept_slices
+    assert n(1, 1, 64, 32, 8, 2048, 4) == 1                     # one page
+    assert n(1, 1, 5001, 32, 8, 2048, 4) == 9                   # 33 pages for four waves
+    assert n(1, 1, 1 << 24, 32, 8, 1 << 24, 0) == 64            # 8 blocks, 512 wanted
+    assert n(64, 1, 5001, 32, 8, 2048, 4) == 1
+    assert n(1, 2000, 2000, 32, 8, 2048, 4) == 1
