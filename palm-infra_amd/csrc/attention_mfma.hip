@@ -2,7 +2,8 @@
 // head size (PALM_HEAD_DIM, a multiple of 16).  Same semantics as the exact kernel
 // (models/qwen3.py:336-341; kernels/attention.cpp:84-217, 937-962): head h reads kv head h / (nh / nkv),
 // keys j <= p of the query's own sequence (j > p - window with a window), softmax in 32-bit with the
-// running maximum, o = sum_j p_j v_j.
+// running maximum, o = sum_j p_j v_j.  With KEPT a query also sees its sequence's first `kept` keys, however far back they lie: the pages
+// that hold them and lie before the window's first page stand in front of it in the row of pages that is walked over.
 //
 // Cache layouts: K [pages, nkv, 64 keys, hd] (a key's row is contiguous); V is kept transposed,
 // [pages, nkv, hd, 64 keys], so that for both products the summed index is contiguous in memory.
@@ -87,11 +88,23 @@ __device__ inline void load_values(const bf16_t* __restrict__ vp, int r, int g, 
     }
 }
 
+// Pages of the first `kept` positions that lie before the window's first page.
+template <bool KEPT> __device__ inline int pages_in_front(int kept, int page_lo) {
+    return KEPT ? min((kept + PAGE_TOKENS - 1) / PAGE_TOKENS, page_lo) : 0;
+}
+// The row of pages is numbered so that the window's pages have their own numbers; those in front of page_lo are the sequence's first.
+template <bool KEPT> __device__ inline int page_of_row(int p, int page_lo, int front) { return KEPT && p < page_lo ? p - (page_lo - front) : p; }
+// Whether key `key` is seen: in-page indices of the first and the last key of the window, and of the first key that is not one of the first `kept`.
+template <bool KEPT> __device__ inline bool key_is_seen(int key, int lo, int hi, int kept) {
+    return KEPT ? key <= hi && (key >= lo || key < kept) : key >= lo && key <= hi;
+}
+
 // Scores of a page's 64 keys against the columns' queries and the online softmax; leaves the page's
 // weights as the B operands of the second product.  Keys outside [lo, hi] (in-page indices) are masked.
 // qv: the B operand of the first product (this lane's query, chunks g, g+4, ..).
+template <bool KEPT = false>
 __device__ inline float score_page(const PageOperands& ops, const bf16x8 (&qv)[KSTEPS], int lo, int hi,
-                                   float scale_log2, Columns& c, int g, bf16x8 (&pv)[2]) {
+                                   float scale_log2, Columns& c, int g, bf16x8 (&pv)[2], int kept = 0) {
     f32x4 s[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -107,7 +120,7 @@ __device__ inline float score_page(const PageOperands& ops, const bf16x8 (&qv)[K
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int key = tile_key(t, 4 * g + i);
-            const float v = (key >= lo && key <= hi) ? s[t][i] * scale_log2 : -INFINITY;
+            const float v = key_is_seen<KEPT>(key, lo, hi, kept) ? s[t][i] * scale_log2 : -INFINITY;
             s[t][i] = v;
             mx = fmaxf(mx, v);
         }
@@ -148,6 +161,18 @@ __device__ inline void blank_values_after(PageOperands& ops, int hi, int g) {
         }
 }
 
+// With first keys that stay visible a page has keys that are not seen in its middle too.
+__device__ inline void blank_values_unseen(PageOperands& ops, int lo, int hi, int kept, int g) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const bool seen = key_is_seen<true>(h * 32 + g * 8 + e, lo, hi, kept);
+#pragma unroll
+            for (int dt = 0; dt < DTILES; ++dt) ops.v[dt][h][e] = seen ? ops.v[dt][h][e] : (__bf16)0.0f;
+        }
+}
+
 __device__ inline void weigh_values(const PageOperands& ops, const bf16x8 (&pv)[2], float alpha, Columns& c) {
 #pragma unroll
     for (int dt = 0; dt < DTILES; ++dt) {
@@ -158,7 +183,7 @@ __device__ inline void weigh_values(const PageOperands& ops, const bf16x8 (&pv)[
     }
 }
 
-// All pages p0 <= p < p1 of one sequence and kv head.  The reads of the next page are issued as soon as the
+// All pages p0 <= p < p1 of the row of one sequence and kv head.  The reads of the next page are issued as soon as the
 // registers of the current one are free: K after the scores, V after the weighted sum, so that a page's
 // latency hides behind the previous page's arithmetic.  first/last: the column's own key range.
 // start.prepare(qv, c) is called once, after the first page's keys have been asked for: a caller whose query is
@@ -166,24 +191,30 @@ __device__ inline void weigh_values(const PageOperands& ops, const bf16x8 (&pv)[
 struct Ready {
     __device__ void prepare(bf16x8 (&)[KSTEPS], Columns&) {}
 };
-template <typename Start>
+template <bool KEPT, typename Start>
 __device__ inline void attend_pages(const bf16_t* __restrict__ k_cache, const bf16_t* __restrict__ v_cache,
                                     const int* __restrict__ pages, int nkv, int kvh, int p0, int p1,
                                     bf16x8 (&qv)[KSTEPS], int first, int last, float scale_log2, Columns& c,
-                                    int r, int g, Start& start) {
+                                    int r, int g, Start& start, int kept, int page_lo, int front) {
     if (p0 >= p1) return;
     PageOperands ops;
-    size_t base = ((size_t)pages[p0] * nkv + kvh) * PAGE_TOKENS * HD;
+    size_t base = ((size_t)pages[page_of_row<KEPT>(p0, page_lo, front)] * nkv + kvh) * PAGE_TOKENS * HD;
     load_keys(k_cache + base, r, g, ops);
     start.prepare(qv, c);
     load_values(v_cache + base, r, g, ops);
     for (int p = p0; p < p1; ++p) {
         const bool more = p + 1 < p1;
-        const size_t next = more ? ((size_t)pages[p + 1] * nkv + kvh) * PAGE_TOKENS * HD : base;
+        const size_t next = more ? ((size_t)pages[page_of_row<KEPT>(p + 1, page_lo, front)] * nkv + kvh) * PAGE_TOKENS * HD : base;
         bf16x8 pv[2];
-        const float alpha = score_page(ops, qv, first - p * PAGE_TOKENS, last - p * PAGE_TOKENS, scale_log2, c, g, pv);
+        const int key0 = page_of_row<KEPT>(p, page_lo, front) * PAGE_TOKENS;
+        const float alpha = score_page<KEPT>(ops, qv, first - key0, last - key0, scale_log2, c, g, pv, kept - key0);
         if (more) load_keys(k_cache + next, r, g, ops);
-        if (last - p * PAGE_TOKENS < PAGE_TOKENS - 1) blank_values_after(ops, last - p * PAGE_TOKENS, g);   // the same in every lane
+        // (the same in every lane)
+        if constexpr (KEPT) {
+            if (last - key0 < PAGE_TOKENS - 1 || (first > key0 && kept - key0 < PAGE_TOKENS)) blank_values_unseen(ops, first - key0, last - key0, kept - key0, g);
+        } else {
+            if (last - key0 < PAGE_TOKENS - 1) blank_values_after(ops, last - key0, g);
+        }
         weigh_values(ops, pv, alpha, c);
         if (more) load_values(v_cache + next, r, g, ops);
         base = next;
@@ -203,21 +234,24 @@ __device__ inline void load_query(const bf16_t* qrow, bool valid, int g, bf16x8 
 // ---- decode ---------------------------------------------------------------------------------------
 // How a query at position `pos` cuts its key range into slices of whole pages.  The decode kernels and the merge
 // must agree on it (the merge reads only the records of slices that hold pages), so it is written once.
+template <bool KEPT = false>
 struct SliceCut {
-    int first;            // the first key the query sees
+    int first;            // the first key of the query's window
     int page_lo;          // the page that holds it
-    int n_pages;          // pages from there to the query's own
+    int front;            // pages of first keys in front of it
+    int n_pages;          // pages of the row: those, and from there to the query's own
     int per;              // pages a slice
     int live;             // slices that hold pages: 1 <= live <= n_slices
-    __device__ SliceCut(int pos, int window, int n_slices) {
+    __device__ SliceCut(int pos, int window, int n_slices, int kept = 0) {
         first = window > 0 ? max(0, pos - window + 1) : 0;
         page_lo = first / PAGE_TOKENS;
-        n_pages = pos / PAGE_TOKENS - page_lo + 1;
+        front = pages_in_front<KEPT>(kept, page_lo);
+        n_pages = pos / PAGE_TOKENS - page_lo + 1 + front;
         per = (n_pages + n_slices - 1) / n_slices;
         live = (n_pages + per - 1) / per;
     }
-    __device__ int begin(int slice) const { return page_lo + slice * per; }
-    __device__ int end(int slice) const { return min(begin(slice) + per, page_lo + n_pages); }
+    __device__ int begin(int slice) const { return page_lo - front + slice * per; }
+    __device__ int end(int slice) const { return min(begin(slice) + per, page_lo - front + n_pages); }
 };
 
 // grid (slices, nkv * query groups, sequences), one wave each.  Workspace per (sequence, head, slice):
@@ -257,17 +291,18 @@ __device__ inline void finish_slice(Columns& c, bool valid, int b, int head, int
 #else
 #define DECODE_WAVES_PER_SIMD
 #endif
+template <bool KEPT>
 __global__ __launch_bounds__(WAVE) DECODE_WAVES_PER_SIMD void attention_decode_kernel(
     const bf16_t* __restrict__ q, const bf16_t* __restrict__ k_cache, const bf16_t* __restrict__ v_cache,
     const int* __restrict__ block_table, int max_pages, const int* __restrict__ seq_slot,
     const int* __restrict__ seq_start, int nh, int nkv, float scale_log2, int window, int n_slices,
-    float* __restrict__ work, bf16_t* __restrict__ out) {
+    float* __restrict__ work, bf16_t* __restrict__ out, int kept) {
     const int slice = blockIdx.x, b = blockIdx.z;
     const int G = nh / nkv, groups = (G + 15) / 16;
     const int kvh = blockIdx.y / groups, qg = blockIdx.y % groups;
     const int lane = threadIdx.x, r = lane % 16, g = lane / 16;
     const int pos = seq_start[b];                       // the query's position; keys 0..pos are in the cache
-    const SliceCut cut(pos, window, n_slices);
+    const SliceCut<KEPT> cut(pos, window, n_slices, kept);
     const int first = cut.first, p0 = cut.begin(slice), p1 = cut.end(slice);
     const int head = kvh * G + qg * 16 + r;             // this lane's query head (column r)
     const bool valid = qg * 16 + r < G;
@@ -282,7 +317,7 @@ __global__ __launch_bounds__(WAVE) DECODE_WAVES_PER_SIMD void attention_decode_k
 
     const int* pages = block_table + (size_t)seq_slot[b] * max_pages;
     Ready ready;
-    attend_pages(k_cache, v_cache, pages, nkv, kvh, p0, p1, qv, first, pos, scale_log2, c, r, g, ready);
+    attend_pages<KEPT>(k_cache, v_cache, pages, nkv, kvh, p0, p1, qv, first, pos, scale_log2, c, r, g, ready, kept, cut.page_lo, cut.front);
     finish_slice(c, valid, b, head, nh, slice, n_slices, p0 >= p1, g, work, out);
 }
 
@@ -295,10 +330,10 @@ __global__ __launch_bounds__(WAVE) DECODE_WAVES_PER_SIMD void attention_decode_k
 // shorter one's last records exist but hold what an earlier step left: one sequence of 2,048 tokens in a step
 // recorded for 4,096 fills 33 of 64) and counts as nothing by a select.  (8 sequences, 12 slices: a step of 36 layers
 // 4.04 ms against 4.12 with the reads where they are used.)
-template <int AT_ONCE>
+template <int AT_ONCE, bool KEPT>
 __global__ __launch_bounds__(WAVE) void attention_merge_kernel(const float* __restrict__ work, int n_slices, int nh,
                                                                const int* __restrict__ seq_start, int window,
-                                                               bf16_t* __restrict__ out) {
+                                                               bf16_t* __restrict__ out, int kept) {
     constexpr int PER = (HD + WAVE - 1) / WAVE;
     const float* w = work + (size_t)blockIdx.x * n_slices * WORK_STRIDE;
     const int lane = threadIdx.x;
@@ -314,7 +349,7 @@ __global__ __launch_bounds__(WAVE) void attention_merge_kernel(const float* __re
         }
     };
     ask(0);
-    const int live = SliceCut(seq_start[blockIdx.x / nh], window, n_slices).live;       // as the decode kernels cut the range
+    const int live = SliceCut<KEPT>(seq_start[blockIdx.x / nh], window, n_slices, kept).live;       // as the decode kernels cut the range
     float m = lane < live ? mine.x : -INFINITY, l = 0.f;
     for (int s = lane + WAVE; s < live; s += WAVE) m = fmaxf(m, w[(size_t)s * WORK_STRIDE]);
     m = wave_max(m);
@@ -344,17 +379,19 @@ __global__ __launch_bounds__(WAVE) void attention_merge_kernel(const float* __re
 }
 
 // slices read together by the merge: all of a step's where they are few, never more than fit in registers
+template <bool KEPT = false>
 static void launch_merge(hipStream_t stream, const float* work, int n_slices, int n_seqs, int nh, const int* seq_start,
-                         int window, bf16_t* out) {
-    if (n_slices <= 4) attention_merge_kernel<4><<<n_seqs * nh, WAVE, 0, stream>>>(work, n_slices, nh, seq_start, window, out);
-    else if (n_slices <= 8) attention_merge_kernel<8><<<n_seqs * nh, WAVE, 0, stream>>>(work, n_slices, nh, seq_start, window, out);
-    else attention_merge_kernel<16><<<n_seqs * nh, WAVE, 0, stream>>>(work, n_slices, nh, seq_start, window, out);
+                         int window, bf16_t* out, int kept = 0) {
+    if (n_slices <= 4) attention_merge_kernel<4, KEPT><<<n_seqs * nh, WAVE, 0, stream>>>(work, n_slices, nh, seq_start, window, out, kept);
+    else if (n_slices <= 8) attention_merge_kernel<8, KEPT><<<n_seqs * nh, WAVE, 0, stream>>>(work, n_slices, nh, seq_start, window, out, kept);
+    else attention_merge_kernel<16, KEPT><<<n_seqs * nh, WAVE, 0, stream>>>(work, n_slices, nh, seq_start, window, out, kept);
 }
 
+template <bool KEPT = false>
 static int launch_attention_decode(hipStream_t stream, const void* q, const void* k_cache, const void* v_cache,
                                    const int* block_table, int max_pages, const int* seq_slot, const int* seq_start,
                                    int n_seqs, int nh, int nkv, int hd, float scale, int window, int n_slices,
-                                   float* work, void* out) {
+                                   float* work, void* out, int kept = 0) {
     PALM_CHECK(hd == HD, "attention_decode: this library was built for head size %d, not %d", HD, hd);
     PALM_CHECK(n_seqs >= 0 && nh > 0 && nkv > 0 && nh % nkv == 0, "attention_decode: seqs=%d heads=%d kv=%d", n_seqs, nh, nkv);
     PALM_CHECK(n_slices >= 1 && n_slices <= 65535, "attention_decode: %d slices", n_slices);
@@ -364,12 +401,12 @@ static int launch_attention_decode(hipStream_t stream, const void* q, const void
     const int groups = (nh / nkv + 15) / 16;
     PALM_CHECK(nkv * groups <= 65535 && n_seqs <= 65535, "attention_decode: grid too large");
     dim3 grid(n_slices, nkv * groups, n_seqs);
-    attention_decode_kernel<<<grid, WAVE, 0, stream>>>((const bf16_t*)q, (const bf16_t*)k_cache, (const bf16_t*)v_cache,
-                                                      block_table, max_pages, seq_slot, seq_start, nh, nkv, scale * LOG2E,
-                                                      window, n_slices, work, (bf16_t*)out);
+    attention_decode_kernel<KEPT><<<grid, WAVE, 0, stream>>>((const bf16_t*)q, (const bf16_t*)k_cache, (const bf16_t*)v_cache,
+                                                            block_table, max_pages, seq_slot, seq_start, nh, nkv, scale * LOG2E,
+                                                            window, n_slices, work, (bf16_t*)out, kept);
     PALM_LAUNCHED();
     if (n_slices > 1) {
-        launch_merge(stream, work, n_slices, n_seqs, nh, seq_start, window, (bf16_t*)out);
+        launch_merge<KEPT>(stream, work, n_slices, n_seqs, nh, seq_start, window, (bf16_t*)out, kept);
         PALM_LAUNCHED();
     }
     return 0;
@@ -381,6 +418,16 @@ PALM_API int palm_attention_decode(hipStream_t stream, const void* q, const void
                                    float* work, void* out) {
     return launch_attention_decode(stream, q, k_cache, v_cache, block_table, max_pages, seq_slot, seq_start, n_seqs, nh, nkv,
                                    hd, scale, window, n_slices, work, out);
+}
+
+// The same with the sequence's first `kept` keys visible behind the window (> 0).
+PALM_API int palm_attention_decode_kept(hipStream_t stream, const void* q, const void* k_cache, const void* v_cache,
+                                        const int* block_table, int max_pages, const int* seq_slot, const int* seq_start,
+                                        int n_seqs, int nh, int nkv, int hd, float scale, int window, int n_slices,
+                                        float* work, void* out, int kept) {
+    PALM_CHECK(window > 0 && kept >= 0 && kept < 1 << 30, "attention_decode_kept: window=%d kept=%d", window, kept);
+    return launch_attention_decode<true>(stream, q, k_cache, v_cache, block_table, max_pages, seq_slot, seq_start, n_seqs, nh, nkv,
+                                         hd, scale, window, n_slices, work, out, kept);
 }
 
 // ---- decode with the q/k/v pass folded in -----------------------------------------------------------
@@ -613,14 +660,14 @@ struct FromProjection {
     }
 };
 
-template <typename TIN, int PLANES>
+template <typename TIN, int PLANES, bool KEPT>
 __global__ __launch_bounds__(WAVE) DECODE_WAVES_PER_SIMD void attention_decode_fused_kernel(
     const TIN* __restrict__ qkv, int planes, size_t plane_stride, const float* __restrict__ q_norm_w,
     const float* __restrict__ k_norm_w, float eps, const float* __restrict__ cos_t, const float* __restrict__ sin_t,
     int write_cache, bf16_t* __restrict__ k_cache, bf16_t* __restrict__ v_cache,
     const int* __restrict__ block_table, int max_pages, const int* __restrict__ seq_slot,
     const int* __restrict__ seq_start, int nh, int nkv, float scale_log2, int window, int n_slices,
-    float* __restrict__ work, bf16_t* __restrict__ out) {
+    float* __restrict__ work, bf16_t* __restrict__ out, int kept) {
     if constexpr (FUSED_SERVES_HEAD) {
         __shared__ float new_key[HD], new_value[HD];
         const int slice = blockIdx.x, b = blockIdx.z;
@@ -652,7 +699,7 @@ __global__ __launch_bounds__(WAVE) DECODE_WAVES_PER_SIMD void attention_decode_f
         start.ask();
 
         const int pos = seq_start[b];
-        const SliceCut cut(pos, window, n_slices);
+        const SliceCut<KEPT> cut(pos, window, n_slices, kept);
         const int first = cut.first, p0 = cut.begin(slice), p1 = cut.end(slice);
         const int* pages = block_table + (size_t)seq_slot[b] * max_pages;
         const int page = pos / PAGE_TOKENS;
@@ -671,7 +718,8 @@ __global__ __launch_bounds__(WAVE) DECODE_WAVES_PER_SIMD void attention_decode_f
 #pragma unroll
         for (int dt = 0; dt < DTILES; ++dt) c.o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
         // with a key and value of its own making the step sees the cache up to the position before
-        attend_pages(k_cache, v_cache, pages, nkv, kvh, p0, p1, qv, first, write_cache ? pos - 1 : pos, scale_log2, c, r, g, start);
+        attend_pages<KEPT>(k_cache, v_cache, pages, nkv, kvh, p0, p1, qv, first, write_cache ? pos - 1 : pos, scale_log2, c, r, g, start, kept, cut.page_lo,
+                           cut.front);
         finish_slice(c, valid, b, head, nh, slice, n_slices, p0 >= p1, g, work, out);
     }
 }
@@ -683,12 +731,13 @@ PALM_API int palm_attention_decode_fused_serves(int rotary_dim, int pairing) {
 // qkv: [n_seqs, (nh + 2 nkv) hd] bfloat16 (qkv_is_planes = 0), or [planes, n_seqs, (nh + 2 nkv) hd] float32.
 // cos_t, sin_t: [n_seqs, hd / 2] float32 rows of the sequences' positions, or both null for no rotation.
 // Without write_cache the cache already holds the new position's key and value (a layer that reads another's).
-PALM_API int palm_attention_decode_fused(hipStream_t stream, const void* qkv, int qkv_is_planes, int planes,
+template <bool KEPT>
+static int launch_decode_fused(hipStream_t stream, const void* qkv, int qkv_is_planes, int planes,
                                          const float* q_norm_w, const float* k_norm_w, float eps, const float* cos_t,
                                          const float* sin_t, int rotary_dim, int pairing, int write_cache, void* k_cache,
                                          void* v_cache, const int* block_table, int max_pages, const int* seq_slot,
                                          const int* seq_start, int n_seqs, int nh, int nkv, int hd, float scale,
-                                         int window, int n_slices, float* work, void* out) {
+                                         int window, int n_slices, float* work, void* out, int kept) {
     PALM_CHECK(hd == HD, "attention_decode_fused: this library was built for head size %d, not %d", HD, hd);
     PALM_CHECK((cos_t == nullptr) == (sin_t == nullptr), "attention_decode_fused: cos and sin tables come together");
     PALM_CHECK(palm_attention_decode_fused_serves(cos_t ? rotary_dim : 0, pairing),
@@ -705,9 +754,9 @@ PALM_API int palm_attention_decode_fused(hipStream_t stream, const void* qkv, in
     PALM_CHECK(nkv * groups <= 65535 && n_seqs <= 65535, "attention_decode_fused: grid too large");
     dim3 grid(n_slices, nkv * groups, n_seqs);
     const size_t plane_stride = (size_t)n_seqs * (nh + 2 * nkv) * HD;
-#define PALM_FUSED(TIN, P) attention_decode_fused_kernel<TIN, P><<<grid, WAVE, 0, stream>>>( \
+#define PALM_FUSED(TIN, P) attention_decode_fused_kernel<TIN, P, KEPT><<<grid, WAVE, 0, stream>>>( \
         (const TIN*)qkv, planes, plane_stride, q_norm_w, k_norm_w, eps, cos_t, sin_t, write_cache, (bf16_t*)k_cache, \
-        (bf16_t*)v_cache, block_table, max_pages, seq_slot, seq_start, nh, nkv, scale * LOG2E, window, n_slices, work, (bf16_t*)out)
+        (bf16_t*)v_cache, block_table, max_pages, seq_slot, seq_start, nh, nkv, scale * LOG2E, window, n_slices, work, (bf16_t*)out, kept)
     if (!qkv_is_planes) PALM_FUSED(bf16_t, 1);
     else if (planes == 1) PALM_FUSED(float, 1);
     else if (planes == 2) PALM_FUSED(float, 2);
@@ -715,10 +764,31 @@ PALM_API int palm_attention_decode_fused(hipStream_t stream, const void* qkv, in
 #undef PALM_FUSED
     PALM_LAUNCHED();
     if (n_slices > 1) {
-        launch_merge(stream, work, n_slices, n_seqs, nh, seq_start, window, (bf16_t*)out);
+        launch_merge<KEPT>(stream, work, n_slices, n_seqs, nh, seq_start, window, (bf16_t*)out, kept);
         PALM_LAUNCHED();
     }
     return 0;
+}
+
+PALM_API int palm_attention_decode_fused(hipStream_t stream, const void* qkv, int qkv_is_planes, int planes,
+                                         const float* q_norm_w, const float* k_norm_w, float eps, const float* cos_t,
+                                         const float* sin_t, int rotary_dim, int pairing, int write_cache, void* k_cache,
+                                         void* v_cache, const int* block_table, int max_pages, const int* seq_slot,
+                                         const int* seq_start, int n_seqs, int nh, int nkv, int hd, float scale,
+                                         int window, int n_slices, float* work, void* out) {
+    return launch_decode_fused<false>(stream, qkv, qkv_is_planes, planes, q_norm_w, k_norm_w, eps, cos_t, sin_t, rotary_dim, pairing, write_cache, k_cache, v_cache,
+                                      block_table, max_pages, seq_slot, seq_start, n_seqs, nh, nkv, hd, scale, window, n_slices, work, out, 0);
+}
+// The same with the sequence's first `kept` keys visible behind the window (> 0).
+PALM_API int palm_attention_decode_fused_kept(hipStream_t stream, const void* qkv, int qkv_is_planes, int planes,
+                                         const float* q_norm_w, const float* k_norm_w, float eps, const float* cos_t,
+                                         const float* sin_t, int rotary_dim, int pairing, int write_cache, void* k_cache,
+                                         void* v_cache, const int* block_table, int max_pages, const int* seq_slot,
+                                         const int* seq_start, int n_seqs, int nh, int nkv, int hd, float scale,
+                                         int window, int n_slices, float* work, void* out, int kept) {
+    PALM_CHECK(window > 0 && kept >= 0 && kept < 1 << 30, "attention_decode_fused: window=%d kept=%d", window, kept);
+    return launch_decode_fused<true>(stream, qkv, qkv_is_planes, planes, q_norm_w, k_norm_w, eps, cos_t, sin_t, rotary_dim, pairing, write_cache, k_cache, v_cache,
+                                      block_table, max_pages, seq_slot, seq_start, n_seqs, nh, nkv, hd, scale, window, n_slices, work, out, kept);
 }
 
 // ---- decode cut by pages ------------------------------------------------------------------------------
@@ -948,6 +1018,42 @@ __device__ inline void blank_values_after(bf16_t* v_lds, int tail) {
     }
 }
 
+// With first keys that stay visible (KEPT) a stream runs on past what it once held, so a token whose activations overflowed may lie in a place that
+// most queries do not see: its weight is zero there, but its value is multiplied all the same, and zero times an infinity or a NaN is NaN.  On a page
+// of which some query of the tile sees less than all keys, such values are made zero in LDS, and added at the end, as they are, to the results of the
+// queries that do see them (add_wild_values; inside the walk it would cost its registers).  This also blanks the values behind the sequence's last key (`tail`, an in-page index).  True: there were some among those seen.
+__device__ inline bool tame_values(bf16_t* v_lds, int tail) {
+    bool found = false;
+    for (int idx = threadIdx.x % PF_THREADS; idx < HD * (PAGE_TOKENS / 8); idx += PF_THREADS) {
+        const int d = idx / (PAGE_TOKENS / 8), chunk = idx % (PAGE_TOKENS / 8);
+        uint4* at = reinterpret_cast<uint4*>(v_lds + d * V_STRIDE + (chunk ^ v_swizzle(d)) * 8);
+        uint4 v = *at;
+        uint32_t* two = reinterpret_cast<uint32_t*>(&v);
+        bool change = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t mask = e % 2 ? 0xffff0000u : 0xffffu, exponent = e % 2 ? 0x7f800000u : 0x7f80u;
+            const bool wild = (two[e / 2] & exponent) == exponent, behind = chunk * 8 + e > tail;
+            found = found || (wild && !behind);
+            change = change || wild || behind;
+            if (wild || behind) two[e / 2] &= ~mask;
+        }
+        if (change) *at = v;
+    }
+    return found;
+}
+// What tame_values left out, for the column whose sums `o` are: rows 16 dt + 4 g .. + 3 of the page's V^T in memory.
+template <typename Sees> __device__ inline void add_wild_values(const bf16_t* __restrict__ v_page, f32x4 (&o)[DTILES], int g, Sees sees) {
+#pragma unroll
+    for (int dt = 0; dt < DTILES; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            for (int key = 0; key < PAGE_TOKENS; ++key) {
+                const bf16_t v = v_page[(size_t)(dt * 16 + 4 * g + i) * PAGE_TOKENS + key];
+                if ((v.bits & 0x7f80u) == 0x7f80u && sees(key)) o[dt][i] += to_float(v);
+            }
+}
+
 struct Unit {                 // one (head, 16 query positions): the wave's share of it
     bool live;                // false: the wave has no such unit (fewer units than slots)
     bool active;              // the page at hand holds keys that some column of the unit sees
@@ -976,8 +1082,9 @@ __device__ inline void read_key_fragments(const bf16_t* k_lds, int t, int r, int
 // Scores and softmax of one page for the wave's units.  The fragments of key tile t+1 are read from LDS
 // before the products of tile t run, so a read's latency hides behind arithmetic.  `interior`: every key of
 // the page is visible to every column of the wave (the usual case away from the diagonal), no masking then.
+template <bool KEPT>
 __device__ inline void unit_scores(const bf16_t* k_lds, Unit (&u)[PF_UNITS], int page_first_key, float scale_log2,
-                                   int r, int g, bool interior, bf16x8 (&pv)[PF_UNITS][2], float (&alpha)[PF_UNITS]) {
+                                   int r, int g, bool interior, bf16x8 (&pv)[PF_UNITS][2], float (&alpha)[PF_UNITS], int kept) {
     f32x4 s[PF_UNITS][4];
     bf16x8 kf[2][KSTEPS];
     read_key_fragments(k_lds, 0, r, g, kf[0]);
@@ -1011,7 +1118,7 @@ __device__ inline void unit_scores(const bf16_t* k_lds, Unit (&u)[PF_UNITS], int
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int key = tile_key(t, 4 * g + i);
-                    const float v = (key >= lo && key <= hi) ? s[x][t][i] : -INFINITY;
+                    const float v = key_is_seen<KEPT>(key, lo, hi, kept - page_first_key) ? s[x][t][i] : -INFINITY;
                     s[x][t][i] = v;
                     mx = fmaxf(mx, v);
                 }
@@ -1088,11 +1195,12 @@ __device__ inline void unit_values(const bf16_t* v_lds, Unit (&u)[PF_UNITS], int
 #else
 #define PF_WAVES_PER_SIMD
 #endif
+template <bool KEPT>
 __global__ __launch_bounds__(PF_THREADS) PF_WAVES_PER_SIMD void attention_prefill_kernel(
     const bf16_t* __restrict__ q, const bf16_t* __restrict__ k_cache, const bf16_t* __restrict__ v_cache,
     const int* __restrict__ block_table, int max_pages, const int* __restrict__ seq_slot,
     const int* __restrict__ seq_start, const int* __restrict__ seq_new, const int* __restrict__ cu_new, int nh,
-    int nkv, float scale_log2, int window, int qb, int hg, bf16_t* __restrict__ out) {
+    int nkv, float scale_log2, int window, int qb, int hg, bf16_t* __restrict__ out, int kept) {
     constexpr int K_TILE = PAGE_TOKENS * K_STRIDE, V_TILE = HD * V_STRIDE;
     // Head sizes whose pages fit twice keep two pages of K and of V^T in LDS: while one is used the next is laid
     // down beside it, and one barrier a page is enough.  Larger heads share one buffer between K and V^T.
@@ -1150,17 +1258,24 @@ __global__ __launch_bounds__(PF_THREADS) PF_WAVES_PER_SIMD void attention_prefil
     }
 
     // the pages any of the block's sub-tiles sees (the same for all waves)
-    int p_lo = 0x7fffffff, p_hi = -1;
+    int page_lo = 0x7fffffff, p_hi = -1, pos_least = 0x7fffffff, first_most = 0;
     for (int sub = 0; sub < subs; ++sub) {
         const int tile16 = sub_tile(sub);
         if (tile16 < 0) continue;
         p_hi = max(p_hi, (start + min(tile16 * 16 + 15, n_new - 1)) / PAGE_TOKENS);
-        p_lo = min(p_lo, window > 0 ? max(0, start + tile16 * 16 - window + 1) / PAGE_TOKENS : 0);
+        page_lo = min(page_lo, window > 0 ? max(0, start + tile16 * 16 - window + 1) / PAGE_TOKENS : 0);
+        pos_least = min(pos_least, start + tile16 * 16);
+        first_most = max(first_most, start + min(tile16 * 16 + 15, n_new - 1) - window + 1);
     }
+    const int front = pages_in_front<KEPT>(kept, page_lo), p_lo = page_lo - front;     // the row of pages, see page_of_row
+    auto offset_of = [&](int p) { return ((size_t)pages[page_of_row<KEPT>(p, page_lo, front)] * nkv + kvh) * PAGE_TOKENS * HD; };
+    // with KEPT: whether some query of the block sees less than all keys of a page (the same for all waves)
+    auto at_an_edge = [&](int key0) { return pos_least < key0 + PAGE_TOKENS - 1 || (first_most > key0 && kept < key0 + PAGE_TOKENS); };
+    int wild = 0;                                               // some such page held values that were taken out
     PagePrefetch pf;
     PageSources sources;
     {
-        const size_t base = ((size_t)pages[p_lo] * nkv + kvh) * PAGE_TOKENS * HD;
+        const size_t base = offset_of(p_lo);
         if constexpr (PF_DMA) {
             sources = page_sources();
             page_into_lds(k_cache + base, v_cache + base, sources, k_lds, v_lds);
@@ -1172,10 +1287,11 @@ __global__ __launch_bounds__(PF_THREADS) PF_WAVES_PER_SIMD void attention_prefil
     // is every key of page p visible to every column of this wave that takes part?  (also marks who does)
     auto page_is_interior = [&](int p) -> bool {
         bool inside = true;
+        const int page = page_of_row<KEPT>(p, page_lo, front), key0 = page * PAGE_TOKENS;
 #pragma unroll
         for (int x = 0; x < PF_UNITS; ++x) {
-            u[x].active = u[x].live && p >= u[x].page_lo && p <= u[x].page_hi;
-            inside = inside && (!u[x].active || (u[x].first <= p * PAGE_TOKENS && u[x].pos >= p * PAGE_TOKENS + PAGE_TOKENS - 1));
+            u[x].active = u[x].live && (page >= u[x].page_lo || (KEPT && key0 < kept)) && page <= u[x].page_hi;
+            inside = inside && (!u[x].active || ((u[x].first <= key0 || (KEPT && kept >= key0 + PAGE_TOKENS)) && u[x].pos >= key0 + PAGE_TOKENS - 1));
         }
         return __all(inside);
     };
@@ -1190,12 +1306,15 @@ __global__ __launch_bounds__(PF_THREADS) PF_WAVES_PER_SIMD void attention_prefil
         for (int p = p_lo; p <= p_hi; ++p) {
             const int buf = (p - p_lo) & 1;
             const bool more = p < p_hi;
-            if (seq_tail - p * PAGE_TOKENS < PAGE_TOKENS - 1) {     // the sequence's last page (no page follows it)
-                blank_values_after(v_lds + buf * V_TILE, seq_tail - p * PAGE_TOKENS);
+            const int key0 = page_of_row<KEPT>(p, page_lo, front) * PAGE_TOKENS;
+            if constexpr (KEPT) {
+                if (at_an_edge(key0)) wild |= __syncthreads_or(tame_values(v_lds + buf * V_TILE, seq_tail - key0));
+            } else if (seq_tail - key0 < PAGE_TOKENS - 1) {         // the sequence's last page (no page follows it)
+                blank_values_after(v_lds + buf * V_TILE, seq_tail - key0);
                 __syncthreads();
             }
             if (more) {                                         // in flight while this page is used
-                const size_t next = ((size_t)pages[p + 1] * nkv + kvh) * PAGE_TOKENS * HD;
+                const size_t next = offset_of(p + 1);
                 if constexpr (PF_DMA) {     // straight into the other buffer, whose last readers passed the barrier a page ago
                     page_into_lds(k_cache + next, v_cache + next, sources, k_lds + (buf ^ 1) * K_TILE, v_lds + (buf ^ 1) * V_TILE);
                 } else {
@@ -1206,7 +1325,7 @@ __global__ __launch_bounds__(PF_THREADS) PF_WAVES_PER_SIMD void attention_prefil
             bf16x8 pv[PF_UNITS][2];
             float alpha[PF_UNITS];
             const bool interior = page_is_interior(p);
-            unit_scores(k_lds + buf * K_TILE, u, p * PAGE_TOKENS, scale_log2, r, g, interior, pv, alpha);
+            unit_scores<KEPT>(k_lds + buf * K_TILE, u, key0, scale_log2, r, g, interior, pv, alpha, kept);
             bool moved = false;
 #pragma unroll
             for (int x = 0; x < PF_UNITS; ++x) moved = moved || alpha[x] != 1.0f;
@@ -1223,7 +1342,8 @@ __global__ __launch_bounds__(PF_THREADS) PF_WAVES_PER_SIMD void attention_prefil
     } else {
         for (int p = p_lo; p <= p_hi; ++p) {
             const bool more = p < p_hi;
-            const size_t next = more ? ((size_t)pages[p + 1] * nkv + kvh) * PAGE_TOKENS * HD : 0;
+            const size_t next = more ? offset_of(p + 1) : 0;
+            const int key0 = page_of_row<KEPT>(p, page_lo, front) * PAGE_TOKENS;
             bf16x8 pv[PF_UNITS][2];
             float alpha[PF_UNITS];
             __syncthreads();                                    // everyone is done with the previous page
@@ -1231,7 +1351,7 @@ __global__ __launch_bounds__(PF_THREADS) PF_WAVES_PER_SIMD void attention_prefil
             __syncthreads();
             if (more) prefetch_keys(k_cache + next, pf);        // in flight while this page is used
             const bool interior = page_is_interior(p);
-            unit_scores(k_lds, u, p * PAGE_TOKENS, scale_log2, r, g, interior, pv, alpha);
+            unit_scores<KEPT>(k_lds, u, key0, scale_log2, r, g, interior, pv, alpha, kept);
             bool moved = false;
 #pragma unroll
             for (int x = 0; x < PF_UNITS; ++x) moved = moved || alpha[x] != 1.0f;
@@ -1239,8 +1359,10 @@ __global__ __launch_bounds__(PF_THREADS) PF_WAVES_PER_SIMD void attention_prefil
             __syncthreads();
             stage_values(pf, v_lds);
             __syncthreads();
-            if (seq_tail - p * PAGE_TOKENS < PAGE_TOKENS - 1) {
-                blank_values_after(v_lds, seq_tail - p * PAGE_TOKENS);
+            if constexpr (KEPT) {
+                if (at_an_edge(key0)) wild |= __syncthreads_or(tame_values(v_lds, seq_tail - key0));
+            } else if (seq_tail - key0 < PAGE_TOKENS - 1) {
+                blank_values_after(v_lds, seq_tail - key0);
                 __syncthreads();
             }
             unit_values(v_lds, u, r, g, pv, alpha, rescale);
@@ -1248,6 +1370,15 @@ __global__ __launch_bounds__(PF_THREADS) PF_WAVES_PER_SIMD void attention_prefil
         }
     }
 
+    if (KEPT && wild) {
+        for (int p = p_lo; p <= p_hi; ++p) {
+            const int key0 = page_of_row<KEPT>(p, page_lo, front) * PAGE_TOKENS;
+            if (!at_an_edge(key0)) continue;
+#pragma unroll
+            for (int x = 0; x < PF_UNITS; ++x)
+                add_wild_values(v_cache + offset_of(p), u[x].c.o, g, [&](int key) { return key_is_seen<true>(key, u[x].first - key0, u[x].pos - key0, kept - key0); });
+        }
+    }
 #pragma unroll
     for (int x = 0; x < PF_UNITS; ++x) {
         const float l = u[x].weights[0];
@@ -1310,9 +1441,9 @@ struct PairedUnit {           // one (head, 16 query positions): the wave's shar
 
 // masked (the same in every lane): some column of the wave does not see every key of the page
 constexpr int VALUES_AHEAD = DTILES / 2;       // value tiles whose fragments are asked for before the weights are made
-template <bool PRESCALED>
+template <bool PRESCALED, bool KEPT>
 __device__ __forceinline__ void paired_page(const bf16_t* k_lds, const bf16_t* v_lds, PairedUnit (&u)[PF_UNITS], int page_first_key,
-                                            float scale_log2, int r, int g, bool masked) {
+                                            float scale_log2, int r, int g, bool masked, int kept) {
     f32x4 s[PF_UNITS][4];
     float sub[PF_UNITS];
 #pragma unroll
@@ -1361,7 +1492,7 @@ __device__ __forceinline__ void paired_page(const bf16_t* k_lds, const bf16_t* v
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int key = tile_key(t, 4 * g + i);
-                    s[x][t][i] = (key >= lo && key <= hi) ? s[x][t][i] : -INFINITY;
+                    s[x][t][i] = key_is_seen<KEPT>(key, lo, hi, kept - page_first_key) ? s[x][t][i] : -INFINITY;
                 }
         }
         float top = s[x][0][0];
@@ -1425,12 +1556,12 @@ __device__ __forceinline__ void paired_page(const bf16_t* k_lds, const bf16_t* v
             for (int x = 0; x < PF_UNITS; ++x) u[x].o[dt] = mfma_16x16x32(vf[dt][h], pv[x][h], u[x].o[dt]);
 }
 
-template <int HALVES, bool PRESCALED>
+template <int HALVES, bool PRESCALED, bool KEPT>
 __global__ __launch_bounds__(HALVES * PF_THREADS) PF_WAVES_PER_SIMD void attention_prefill_paired_kernel(
     const bf16_t* __restrict__ q, const bf16_t* __restrict__ k_cache, const bf16_t* __restrict__ v_cache,
     const int* __restrict__ block_table, int max_pages, const int* __restrict__ seq_slot,
     const int* __restrict__ seq_start, const int* __restrict__ seq_new, const int* __restrict__ cu_new, int nh,
-    int nkv, float scale_log2, int window, int qb, int hg, int partners_follow, bf16_t* __restrict__ out) {
+    int nkv, float scale_log2, int window, int qb, int hg, int partners_follow, bf16_t* __restrict__ out, int kept) {
     if constexpr (PF_DMA) {
         constexpr int K_TILE = PAGE_TOKENS * K_STRIDE, V_TILE = HD * V_STRIDE;
         __shared__ __attribute__((aligned(16))) bf16_t k_lds[HALVES * 2 * K_TILE];
@@ -1481,21 +1612,28 @@ __global__ __launch_bounds__(HALVES * PF_THREADS) PF_WAVES_PER_SIMD void attenti
             // the pages any query of the tile sees (the same for all waves)
             const int tile_last = min(tile_first + qb - 1, n_new - 1);
             const int p_hi = (start + tile_last) / PAGE_TOKENS;
-            const int p_lo = window > 0 ? max(0, start + tile_first - window + 1) / PAGE_TOKENS : 0;
+            const int page_lo = window > 0 ? max(0, start + tile_first - window + 1) / PAGE_TOKENS : 0;
+            const int front = pages_in_front<KEPT>(kept, page_lo), p_lo = page_lo - front;          // the row of pages, see page_of_row
             // of every HALVES pages in turn each half takes one, into two places of its own
             bf16_t *k_half = k_lds + half * 2 * K_TILE, *v_half = v_lds + half * 2 * V_TILE;
             auto load_page = [&](int p, int step) {
-                const size_t at = ((size_t)pages[p] * nkv + kvh) * PAGE_TOKENS * HD;
+                const size_t at = ((size_t)pages[page_of_row<KEPT>(p, page_lo, front)] * nkv + kvh) * PAGE_TOKENS * HD;
                 page_into_lds(k_cache + at, v_cache + at, sources, k_half + step % 2 * K_TILE, v_half + step % 2 * V_TILE);
             };
             // is every key of page p visible to every column of this wave?
-            auto interior = [&](int p) -> bool {
+            auto interior = [&](int key0) -> bool {
                 bool inside = true;
 #pragma unroll
                 for (int x = 0; x < PF_UNITS; ++x)
-                    inside = inside && (!u[x].live || (u[x].first <= p * PAGE_TOKENS && u[x].pos >= p * PAGE_TOKENS + PAGE_TOKENS - 1));
+                    inside = inside && (!u[x].live || ((u[x].first <= key0 || (KEPT && kept >= key0 + PAGE_TOKENS)) && u[x].pos >= key0 + PAGE_TOKENS - 1));
                 return __all(inside);
             };
+            // with KEPT: does some query of the tile see less than all keys of a page? (the same for all waves)
+            auto at_an_edge = [&](int p) -> bool {
+                const int key0 = page_of_row<KEPT>(p, page_lo, front) * PAGE_TOKENS;
+                return p <= p_hi && (start + tile_first < key0 + PAGE_TOKENS - 1 || (start + tile_last - window + 1 > key0 && kept < key0 + PAGE_TOKENS));
+            };
+            int wild = 0;                                             // some such page held values that were taken out
             wait_for_all_but_the_youngest_loads<0>();                 // the queries
             if (p_lo + half <= p_hi) load_page(p_lo + half, 0);
             wait_for_all_but_the_youngest_loads<0>();
@@ -1504,12 +1642,15 @@ __global__ __launch_bounds__(HALVES * PF_THREADS) PF_WAVES_PER_SIMD void attenti
                 const int p_step = p_lo + step * HALVES, p = p_step + half;
                 if (p + HALVES <= p_hi) load_page(p + HALVES, step + 1);    // into the place whose readers passed the barrier a step ago
                 bf16_t* v_page = v_half + step % 2 * V_TILE;
-                const int tail_page = seq_tail / PAGE_TOKENS, tail = seq_tail % PAGE_TOKENS;
-                if (tail < PAGE_TOKENS - 1 && p_step <= tail_page && tail_page < p_step + HALVES) {   // the sequence's last page: none follows it
+                const int tail_page = seq_tail / PAGE_TOKENS, tail = seq_tail % PAGE_TOKENS, key0 = page_of_row<KEPT>(p, page_lo, front) * PAGE_TOKENS;
+                if constexpr (KEPT) {
+                    if (at_an_edge(p_step) || (HALVES > 1 && at_an_edge(p_step + 1)))
+                        wild |= __syncthreads_or(at_an_edge(p) && tame_values(v_page, seq_tail - key0));
+                } else if (tail < PAGE_TOKENS - 1 && p_step <= tail_page && tail_page < p_step + HALVES) {   // the sequence's last page: none follows it
                     if (p == tail_page) blank_values_after(v_page, tail);
                     __syncthreads();
                 }
-                if (p <= p_hi) paired_page<PRESCALED>(k_half + step % 2 * K_TILE, v_page, u, p * PAGE_TOKENS, scale_log2, r, g, !interior(p));
+                if (p <= p_hi) paired_page<PRESCALED, KEPT>(k_half + step % 2 * K_TILE, v_page, u, key0, scale_log2, r, g, !interior(key0), kept);
                 wait_for_all_but_the_youngest_loads<0>();             // the half's next page has landed
                 page_barrier();
             }
@@ -1543,6 +1684,16 @@ __global__ __launch_bounds__(HALVES * PF_THREADS) PF_WAVES_PER_SIMD void attenti
                         const float4 o = o_lds[((wave * PF_UNITS + x) * DTILES + dt) * WAVE + lane];
                         u[x].o[dt] = u[x].o[dt] * mine + f32x4{o.x, o.y, o.z, o.w} * its;
                     }
+                }
+            }
+            if (KEPT && wild) {
+                for (int p = p_lo; p <= p_hi; ++p) {
+                    const int page = page_of_row<KEPT>(p, page_lo, front), key0 = page * PAGE_TOKENS;
+                    if (!at_an_edge(p)) continue;
+#pragma unroll
+                    for (int x = 0; x < PF_UNITS; ++x)
+                        add_wild_values(v_cache + ((size_t)pages[page] * nkv + kvh) * PAGE_TOKENS * HD, u[x].o, g,
+                                        [&](int key) { return key_is_seen<true>(key, u[x].first - key0, u[x].pos - key0, kept - key0); });
                 }
             }
 #pragma unroll
@@ -1960,10 +2111,11 @@ PALM_API int palm_attention_prefill_halves(int n_seqs, int max_new, int max_keys
 
 // q_prescaled: the queries come multiplied by scale * log2(e) already (by the pass that rounds them), so a score is
 // the exponent of its weight as it leaves the matrix cores; `scale` is then not applied again.  halves: 1 or 2, 0: by the rule above
-PALM_API int palm_attention_prefill_in(hipStream_t stream, const void* q, const void* k_cache, const void* v_cache,
+template <bool KEPT>
+static int launch_attention_prefill(hipStream_t stream, const void* q, const void* k_cache, const void* v_cache,
                                        const int* block_table, int max_pages, const int* seq_slot, const int* seq_start,
                                        const int* seq_new, const int* cu_new, int n_seqs, int max_new, int nh, int nkv,
-                                       int hd, float scale, int window, int q_prescaled, int max_keys, int halves, void* out) {
+                                       int hd, float scale, int window, int q_prescaled, int max_keys, int halves, void* out, int kept) {
     PALM_CHECK(hd == HD, "attention_prefill: this library was built for head size %d, not %d", HD, hd);
     PALM_CHECK(n_seqs >= 0 && max_new >= 0 && nh > 0 && nkv > 0 && nh % nkv == 0,
                "attention_prefill: seqs=%d max_new=%d heads=%d kv=%d", n_seqs, max_new, nh, nkv);
@@ -1985,11 +2137,11 @@ PALM_API int palm_attention_prefill_in(hipStream_t stream, const void* q, const 
         PALM_CHECK(n_q <= 65535, "attention_prefill: %d new tokens are more than one launch takes", max_new);
         dim3 grid(nkv * n_hg, n_q, n_seqs);
         const long long blocks = (long long)grid.x * grid.y * grid.z;
-        const bool few = halves ? halves == 2 : prefill_takes_halves(n_seqs, max_new, max_keys, nh, nkv, window);
+        const bool few = halves ? halves == 2 : prefill_takes_halves(n_seqs, max_new, max_keys, nh, nkv, KEPT ? window + kept : window);
         const int partners_follow = !few && blocks <= 512 && n_seqs == 1;     // all blocks run at once, two a unit
-#define PALM_PAIRED(HALVES, PRE) attention_prefill_paired_kernel<HALVES, PRE><<<grid, HALVES * PF_THREADS, 0, stream>>>( \
+#define PALM_PAIRED(HALVES, PRE) attention_prefill_paired_kernel<HALVES, PRE, KEPT><<<grid, HALVES * PF_THREADS, 0, stream>>>( \
         (const bf16_t*)q, (const bf16_t*)k_cache, (const bf16_t*)v_cache, block_table, max_pages, seq_slot, seq_start, seq_new, \
-        cu_new, nh, nkv, scale_log2, window, qb, hg, partners_follow, (bf16_t*)out)
+        cu_new, nh, nkv, scale_log2, window, qb, hg, partners_follow, (bf16_t*)out, kept)
         if (few) { if (q_prescaled) PALM_PAIRED(2, true); else PALM_PAIRED(2, false); }
         else { if (q_prescaled) PALM_PAIRED(1, true); else PALM_PAIRED(1, false); }
 #undef PALM_PAIRED
@@ -2001,11 +2153,28 @@ PALM_API int palm_attention_prefill_in(hipStream_t stream, const void* q, const 
     const int n_tiles = subs > 1 ? ((n16 + 1) / 2 + subs / 2 - 1) / (subs / 2) : n16;
     PALM_CHECK(n_tiles <= 65535, "attention_prefill: %d new tokens are more than one launch takes", max_new);
     dim3 grid(nkv * n_hg, n_tiles, n_seqs);
-    attention_prefill_kernel<<<grid, PF_THREADS, 0, stream>>>((const bf16_t*)q, (const bf16_t*)k_cache, (const bf16_t*)v_cache,
+    attention_prefill_kernel<KEPT><<<grid, PF_THREADS, 0, stream>>>((const bf16_t*)q, (const bf16_t*)k_cache, (const bf16_t*)v_cache,
                                                              block_table, max_pages, seq_slot, seq_start, seq_new, cu_new, nh,
-                                                             nkv, scale_log2, window, qb, hg, (bf16_t*)out);
+                                                             nkv, scale_log2, window, qb, hg, (bf16_t*)out, kept);
     PALM_LAUNCHED();
     return 0;
+}
+
+PALM_API int palm_attention_prefill_in(hipStream_t stream, const void* q, const void* k_cache, const void* v_cache,
+                                       const int* block_table, int max_pages, const int* seq_slot, const int* seq_start,
+                                       const int* seq_new, const int* cu_new, int n_seqs, int max_new, int nh, int nkv,
+                                       int hd, float scale, int window, int q_prescaled, int max_keys, int halves, void* out) {
+    return launch_attention_prefill<false>(stream, q, k_cache, v_cache, block_table, max_pages, seq_slot, seq_start, seq_new, cu_new, n_seqs, max_new, nh, nkv, hd, scale,
+                                           window, q_prescaled, max_keys, halves, out, 0);
+}
+// The same with the sequences' first `kept` keys visible behind the window (> 0).
+PALM_API int palm_attention_prefill_kept(hipStream_t stream, const void* q, const void* k_cache, const void* v_cache,
+                                       const int* block_table, int max_pages, const int* seq_slot, const int* seq_start,
+                                       const int* seq_new, const int* cu_new, int n_seqs, int max_new, int nh, int nkv,
+                                       int hd, float scale, int window, int q_prescaled, int max_keys, int halves, void* out, int kept) {
+    PALM_CHECK(window > 0 && kept >= 0 && window < 1 << 30 && kept < 1 << 30, "attention_prefill: window=%d kept=%d", window, kept);
+    return launch_attention_prefill<true>(stream, q, k_cache, v_cache, block_table, max_pages, seq_slot, seq_start, seq_new, cu_new, n_seqs, max_new, nh, nkv, hd, scale,
+                                           window, q_prescaled, max_keys, halves, out, kept);
 }
 
 PALM_API int palm_attention_prefill(hipStream_t stream, const void* q, const void* k_cache, const void* v_cache,

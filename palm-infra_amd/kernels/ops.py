@@ -826,6 +826,13 @@ _ATTENTION_SIGNATURES = {
     "palm_attention_decode_pages": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_int,
                                     c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int,
                                     c_int, c_float, c_int, c_void_p, c_void_p, c_void_p],
+    "palm_attention_decode_kept": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int,
+                                   c_int, c_int, c_float, c_int, c_int, c_void_p, c_void_p, c_int],
+    "palm_attention_prefill_kept": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
+                                    c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_int, c_void_p, c_int],
+    "palm_attention_decode_fused_kept": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_int,
+                                         c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int,
+                                         c_int, c_int, c_float, c_int, c_int, c_void_p, c_void_p, c_int],
     "palm_attention_decode_pages_serves": [c_int, c_int, c_int, c_int],
     "palm_attention_decode_pages_work": [c_int, c_int],
     "palm_attention_decode_fused_serves": [c_int, c_int],
@@ -2869,13 +2876,14 @@ def attention_kept_exact(q: torch.Tensor, k_cache, v_cache, block_table, seq_slo
 
 
 def attention_kept(q: torch.Tensor, k_cache, v_cache, block_table, seq_slot, seq_start, seq_new, cu_new, max_new: int, max_total: int, nh: int,
-                   nkv: int, hd: int, scale: float, window: int, kept: int) -> torch.Tensor:
+                   nkv: int, hd: int, scale: float, window: int, kept: int, q_prescaled: bool = False) -> torch.Tensor:
     """Causal attention of the step's queries over the cache of which a query at position p sees the last ``window`` positions (p - window < j <= p) and the
     sequence's first ``kept`` ones (j < kept): what keeps a stream without an end within a bounded number of pages.
 
     q [n, nh hd]; sequence b has seq_new[b] queries (none, if it is zero) from row cu_new[b] on, at positions seq_start[b] and up, whose keys and values are
     in the cache; ``max_new`` and ``max_total``: the most new tokens of a sequence and the longest sequence with them, or more.  Pages that no query of
-    the step sees are not read, whatever the page table says of them; what masked places hold (an infinity, a NaN) does not show."""
+    the step sees are not read, whatever the page table says of them; what masked places hold (an infinity, a NaN) does not show.
+    ``q_prescaled``: see ``attention_prefill``."""
     what = "attention_kept"
     _dev(what, q, k_cache, v_cache, block_table, seq_slot, seq_start, seq_new, cu_new)
     _i32(what, block_table, seq_slot, seq_start, seq_new, cu_new)
@@ -2895,7 +2903,28 @@ def attention_kept(q: torch.Tensor, k_cache, v_cache, block_table, seq_slot, seq
         raise KernelError(f"{what}: a window of {window} positions and {kept} first ones: at least one, and none or more")
     if not (0 <= max_new <= max_total <= block_table.shape[1] * PAGE_TOKENS):
         raise KernelError(f"{what}: {max_new} new tokens in sequences of up to {max_total}; the page table has room for {block_table.shape[1] * PAGE_TOKENS}")
-    return attention_kept_exact(q, k_cache, v_cache, block_table, seq_slot, seq_start, seq_new, cu_new, max_new, max_total, nh, nkv, hd, scale, window, kept)
+    if not mfma_attention_serves(q, hd):
+        _need(not q_prescaled, "attention_kept: only the prompt kernel takes scaled queries")
+        return attention_kept_exact(q, k_cache, v_cache, block_table, seq_slot, seq_start, seq_new, cu_new, max_new, max_total, nh, nkv, hd, scale, window, kept)
+    out = torch.empty_like(q)
+    n = q.shape[0]
+    if n == 0 or B == 0 or max_new == 0:
+        return out
+    lib = attention_lib(hd)
+    if max_new == 1 and n == B and not q_prescaled:              # (one token each: as many as there are sequences)
+        n_slices = decode_slices(B, nh, nkv, _kept_keys(max_total, window, kept))
+        work = torch.empty((B * nh * n_slices * (hd + 4),), dtype=F32, device=q.device) if n_slices > 1 else None
+        _call_on(q.device, lib, "palm_attention_decode_kept", _p(q), _p(k_cache), _p(v_cache), _p(block_table), block_table.shape[1], _p(seq_slot),
+                 _p(seq_start), B, nh, nkv, hd, float(scale), window, n_slices, _p(work), _p(out), kept)
+        return out
+    _call_on(q.device, lib, "palm_attention_prefill_kept", _p(q), _p(k_cache), _p(v_cache), _p(block_table), block_table.shape[1], _p(seq_slot),
+             _p(seq_start), _p(seq_new), _p(cu_new), B, max_new, nh, nkv, hd, float(scale), window, int(bool(q_prescaled)), max_total, 0, _p(out), kept)
+    return out
+
+
+def _kept_keys(max_total: int, window: int, kept: int) -> int:
+    """How many keys a single token's query walks over at most, its own page and those that the window and the first ones begin and end in whole."""
+    return min(max_total, window + PAGE_TOKENS + (kept + PAGE_TOKENS - 1) // PAGE_TOKENS * PAGE_TOKENS)
 
 
 # ---- pages of the cache copied to other pages (library ``pages``) ----------------------------------------------------
