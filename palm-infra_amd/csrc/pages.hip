@@ -37,6 +37,18 @@ template <> struct Chunk<16> { using type = uint4; };
 template <> struct Chunk<4> { using type = uint32_t; };
 template <> struct Chunk<2> { using type = uint16_t; };
 
+// The first `bytes` (even, fewer than all) of a chunk.
+__device__ inline void store_first(char* to, uint4 v, int bytes) {
+    if (bytes & 8) *reinterpret_cast<uint2*>(to) = make_uint2(v.x, v.y);
+    const uint32_t word = bytes & 8 ? v.z : v.x, after = bytes & 8 ? v.w : v.y;
+    if (bytes & 4) *reinterpret_cast<uint32_t*>(to + (bytes & 8)) = word;
+    if (bytes & 2) *reinterpret_cast<uint16_t*>(to + (bytes & 12)) = (uint16_t)(bytes & 4 ? after : word);
+}
+__device__ inline void store_first(char* to, uint32_t v, int bytes) {
+    if (bytes & 2) *reinterpret_cast<uint16_t*>(to) = (uint16_t)v;
+}
+__device__ inline void store_first(char*, uint16_t, int) {}
+
 // grid (blocks of a page's chunks, source pages, layers * storages)
 template <int BYTES>
 __global__ __launch_bounds__(CP_THREADS) void copy_pages_kernel(Storage first, Storage second, int layers, CopyPlan plan) {
@@ -70,11 +82,8 @@ __global__ __launch_bounds__(CP_THREADS) void copy_pages_kernel(Storage first, S
         for (int i = 0; i < CP_EACH; ++i) {
             if (rest[i] >= BYTES) {
                 *reinterpret_cast<T*>(to + place[i]) = held[i];
-            } else if (rest[i] > 0) {                                  // the last positions' chunk: two bytes at a time
-                const uint16_t* half = reinterpret_cast<const uint16_t*>(&held[i]);
-#pragma unroll
-                for (int h = 0; h < BYTES / 2; ++h)
-                    if (2 * h < rest[i]) reinterpret_cast<uint16_t*>(to + place[i])[h] = half[h];
+            } else if (rest[i] > 0) {                                  // the last positions' chunk: its halves, quarters and eighths as they are used
+                store_first(to + place[i], held[i], rest[i]);
             }
         }
     }
