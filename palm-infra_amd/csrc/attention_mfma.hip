@@ -1271,7 +1271,8 @@ __global__ __launch_bounds__(PF_THREADS) PF_WAVES_PER_SIMD void attention_prefil
     auto offset_of = [&](int p) { return ((size_t)pages[page_of_row<KEPT>(p, page_lo, front)] * nkv + kvh) * PAGE_TOKENS * HD; };
     // with KEPT: whether some query of the block sees less than all keys of a page (the same for all waves)
     auto at_an_edge = [&](int key0) { return pos_least < key0 + PAGE_TOKENS - 1 || (first_most > key0 && kept < key0 + PAGE_TOKENS); };
-    int wild = 0;                                               // some such page held values that were taken out
+    __shared__ int wild;                                        // some such page held values that were taken out
+    if (KEPT && threadIdx.x == 0) wild = 0;
     PagePrefetch pf;
     PageSources sources;
     {
@@ -1308,7 +1309,10 @@ __global__ __launch_bounds__(PF_THREADS) PF_WAVES_PER_SIMD void attention_prefil
             const bool more = p < p_hi;
             const int key0 = page_of_row<KEPT>(p, page_lo, front) * PAGE_TOKENS;
             if constexpr (KEPT) {
-                if (at_an_edge(key0)) wild |= __syncthreads_or(tame_values(v_lds + buf * V_TILE, seq_tail - key0));
+                if (at_an_edge(key0)) {
+                    if (tame_values(v_lds + buf * V_TILE, seq_tail - key0)) wild = 1;
+                    __syncthreads();
+                }
             } else if (seq_tail - key0 < PAGE_TOKENS - 1) {         // the sequence's last page (no page follows it)
                 blank_values_after(v_lds + buf * V_TILE, seq_tail - key0);
                 __syncthreads();
@@ -1360,7 +1364,10 @@ __global__ __launch_bounds__(PF_THREADS) PF_WAVES_PER_SIMD void attention_prefil
             stage_values(pf, v_lds);
             __syncthreads();
             if constexpr (KEPT) {
-                if (at_an_edge(key0)) wild |= __syncthreads_or(tame_values(v_lds, seq_tail - key0));
+                if (at_an_edge(key0)) {
+                    if (tame_values(v_lds, seq_tail - key0)) wild = 1;
+                    __syncthreads();
+                }
             } else if (seq_tail - key0 < PAGE_TOKENS - 1) {
                 blank_values_after(v_lds, seq_tail - key0);
                 __syncthreads();
@@ -1633,7 +1640,8 @@ __global__ __launch_bounds__(HALVES * PF_THREADS) PF_WAVES_PER_SIMD void attenti
                 const int key0 = page_of_row<KEPT>(p, page_lo, front) * PAGE_TOKENS;
                 return p <= p_hi && (start + tile_first < key0 + PAGE_TOKENS - 1 || (start + tile_last - window + 1 > key0 && kept < key0 + PAGE_TOKENS));
             };
-            int wild = 0;                                             // some such page held values that were taken out
+            __shared__ int wild;                                      // some such page held values that were taken out
+            if (KEPT && threadIdx.x == 0) wild = 0;
             wait_for_all_but_the_youngest_loads<0>();                 // the queries
             if (p_lo + half <= p_hi) load_page(p_lo + half, 0);
             wait_for_all_but_the_youngest_loads<0>();
@@ -1644,8 +1652,10 @@ __global__ __launch_bounds__(HALVES * PF_THREADS) PF_WAVES_PER_SIMD void attenti
                 bf16_t* v_page = v_half + step % 2 * V_TILE;
                 const int tail_page = seq_tail / PAGE_TOKENS, tail = seq_tail % PAGE_TOKENS, key0 = page_of_row<KEPT>(p, page_lo, front) * PAGE_TOKENS;
                 if constexpr (KEPT) {
-                    if (at_an_edge(p_step) || (HALVES > 1 && at_an_edge(p_step + 1)))
-                        wild |= __syncthreads_or(at_an_edge(p) && tame_values(v_page, seq_tail - key0));
+                    if (at_an_edge(p_step) || (HALVES > 1 && at_an_edge(p_step + 1))) {
+                        if (at_an_edge(p) && tame_values(v_page, seq_tail - key0)) wild = 1;
+                        page_barrier();
+                    }
                 } else if (tail < PAGE_TOKENS - 1 && p_step <= tail_page && tail_page < p_step + HALVES) {   // the sequence's last page: none follows it
                     if (p == tail_page) blank_values_after(v_page, tail);
                     __syncthreads();
@@ -1760,12 +1770,12 @@ __device__ __forceinline__ float wide_max(float a, float b, float c) {         /
     return most;
 }
 
-template <bool PRESCALED>
+template <bool PRESCALED, bool KEPT>
 __global__ __launch_bounds__(PF_THREADS) __attribute__((amdgpu_waves_per_eu(1, 1))) void attention_prefill_wide_kernel(
     const bf16_t* __restrict__ q, const bf16_t* __restrict__ k_cache, const bf16_t* __restrict__ v_cache,
     const int* __restrict__ block_table, int max_pages, const int* __restrict__ seq_slot,
     const int* __restrict__ seq_start, const int* __restrict__ seq_new, const int* __restrict__ cu_new, int nh,
-    int nkv, float scale_log2, int window, int qb, int hg, bf16_t* __restrict__ out) {
+    int nkv, float scale_log2, int window, int qb, int hg, bf16_t* __restrict__ out, int kept) {
     if constexpr (PF_WIDE) {
         constexpr int K_TILE = PAGE_TOKENS * K_STRIDE, V_TILE = HD * V_STRIDE, PAGE_LOADS = 2 * PF_LOADS;
         constexpr int QK = 8 * KSTEPS, PV = 4 * DTILES + 4;         // products of a pair of units
@@ -1818,7 +1828,15 @@ __global__ __launch_bounds__(PF_THREADS) __attribute__((amdgpu_waves_per_eu(1, 1
         }
         const int tile_last = min(tile_first + qb - 1, n_new - 1);
         const int p_hi = (start + tile_last) / PAGE_TOKENS;
-        const int p_lo = first_key(start + tile_first) / PAGE_TOKENS;
+        const int page_lo = first_key(start + tile_first) / PAGE_TOKENS;
+        const int front = pages_in_front<KEPT>(kept, page_lo), p_lo = page_lo - front;      // the row of pages, see page_of_row
+        auto page_number = [&](int p) { return page_of_row<KEPT>(p, page_lo, front); };
+        // with KEPT: does some query of the tile see less than all keys of a page? (the same for all waves)
+        auto at_an_edge = [&](int key0) {
+            return start + tile_first < key0 + PAGE_TOKENS - 1 || (start + tile_last - window + 1 > key0 && kept < key0 + PAGE_TOKENS);
+        };
+        __shared__ int wild;                                          // some such page held values that were taken out
+        if (KEPT && threadIdx.x == 0) wild = 0;
 
         const uint32_t k_at = lds_address(k_lds) + wave * 1024, v_at = lds_address(v_lds) + wave * 1024;
         auto page_offset = [&](int page) { return ((size_t)page * nkv + kvh) * (PAGE_TOKENS * HD * sizeof(bf16_t)); };
@@ -1885,7 +1903,7 @@ __global__ __launch_bounds__(PF_THREADS) __attribute__((amdgpu_waves_per_eu(1, 1
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const int key = tile_key(t, 0) + quad / 4 * 8 + i;
-                            s[pair][x][t][i] = (key >= lo && key <= hi) ? s[pair][x][t][i] : -INFINITY;
+                            s[pair][x][t][i] = key_is_seen<KEPT>(key, lo, hi, kept - page_first_key) ? s[pair][x][t][i] : -INFINITY;
                             top[x] = fmaxf(top[x], s[pair][x][t][i]);
                         }
                 }
@@ -1942,7 +1960,7 @@ __global__ __launch_bounds__(PF_THREADS) __attribute__((amdgpu_waves_per_eu(1, 1
 
         wait_for_all_but_the_youngest_loads<0>();                     // the queries
         // 64 entries of the page table, a lane each (read through the scalar unit, each would be waited for together with all reads of LDS)
-        int ids = pages[min(p_lo + lane, p_hi)];
+        int ids = pages[page_number(min(p_lo + lane, p_hi))];
         auto load_k = [&](size_t page, int stage, int i) __attribute__((always_inline)) {
             row_chunk_into_lds(reinterpret_cast<const char*>(k_cache) + page, sources.k[i], k_at + stage * (K_TILE * 2) + i * PF_WAVES * 1024);
         };
@@ -1967,14 +1985,19 @@ __global__ __launch_bounds__(PF_THREADS) __attribute__((amdgpu_waves_per_eu(1, 1
         int stage = 0, p = p_lo;
         do {                                                          // (there is a first page: a test before it would keep the sums of a way past the loop)
             const int next = (stage + 1) % WIDE_STAGES, free_stage = (stage + 3) % WIDE_STAGES;
-            const int first = p * PAGE_TOKENS;
-            const bool masked = last_first > first || least_pos < first + PAGE_TOKENS - 1;
-            if (seq_tail - first < PAGE_TOKENS - 1) {                 // the sequence's last page: no page follows it
+            const int first = page_number(p) * PAGE_TOKENS;
+            const bool masked = (last_first > first && !(KEPT && kept >= first + PAGE_TOKENS)) || least_pos < first + PAGE_TOKENS - 1;
+            if constexpr (KEPT) {
+                if (at_an_edge(first)) {
+                    if (tame_values(v_lds + stage * V_TILE, seq_tail - first)) wild = 1;
+                    page_barrier();
+                }
+            } else if (seq_tail - first < PAGE_TOKENS - 1) {                 // the sequence's last page: no page follows it
                 blank_values_after(v_lds + stage * V_TILE, seq_tail - first);
                 __syncthreads();
             }
             if (((p + 3 - p_lo) & 63) == 0) {
-                ids = pages[min(p + 3 + lane, p_hi)];
+                ids = pages[page_number(min(p + 3 + lane, p_hi))];
                 asm volatile("" : "+v"(ids));                         // (waited for here: where it is used, every page would wait for all loads)
             }
             WIDE_FENCE;
@@ -2055,6 +2078,18 @@ __global__ __launch_bounds__(PF_THREADS) __attribute__((amdgpu_waves_per_eu(1, 1
         WIDE_FENCE;
 #undef WIDE_FENCE
 #undef WIDE_NOP
+        if (KEPT && wild) {
+            for (int row = p_lo; row <= p_hi; ++row) {
+                const int page = page_number(row), key0 = page * PAGE_TOKENS;
+                if (!at_an_edge(key0)) continue;
+#pragma unroll
+                for (int x = 0; x < WIDE_UNITS; ++x) {
+                    const int pos = start + min(first_query(x) + r, n_new - 1);
+                    add_wild_values(v_cache + ((size_t)pages[page] * nkv + kvh) * PAGE_TOKENS * HD, o[x], g,
+                                    [&](int key) { return key_is_seen<true>(key, first_key(pos) - key0, pos - key0, kept - key0); });
+                }
+            }
+        }
 #pragma unroll
         for (int x = 0; x < WIDE_UNITS; ++x) {
             const int qi = first_query(x) + r;
@@ -2188,10 +2223,11 @@ PALM_API int palm_attention_prefill(hipStream_t stream, const void* q, const voi
 PALM_API int palm_attention_prefill_takes_prescaled() { return PF_DMA ? 1 : 0; }
 
 // The same by the kernel for long prompts, where palm_attention_prefill_wide_serves() says so.
-PALM_API int palm_attention_prefill_wide(hipStream_t stream, const void* q, const void* k_cache, const void* v_cache,
+template <bool KEPT>
+static int launch_attention_wide(hipStream_t stream, const void* q, const void* k_cache, const void* v_cache,
                                          const int* block_table, int max_pages, const int* seq_slot, const int* seq_start,
                                          const int* seq_new, const int* cu_new, int n_seqs, int max_new, int nh, int nkv,
-                                         int hd, float scale, int window, int q_prescaled, void* out) {
+                                         int hd, float scale, int window, int q_prescaled, void* out, int kept) {
     PALM_CHECK(PF_WIDE && hd == HD, "attention_prefill_wide: not for head size %d (this library's is %d)", hd, HD);
     PALM_CHECK(n_seqs >= 0 && max_new >= 0 && nh > 0 && nkv > 0 && nh % nkv == 0,
                "attention_prefill_wide: seqs=%d max_new=%d heads=%d kv=%d", n_seqs, max_new, nh, nkv);
@@ -2202,13 +2238,29 @@ PALM_API int palm_attention_prefill_wide(hipStream_t stream, const void* q, cons
     PALM_CHECK(nkv * n_hg <= 65535 && n_seqs <= 65535 && (max_new + qb - 1) / qb <= 65535, "attention_prefill_wide: grid too large");
     const dim3 grid(nkv * n_hg, (max_new + qb - 1) / qb, n_seqs);       // (the kv head fastest: see palm_attention_prefill)
     const float scale_log2 = q_prescaled ? 1.0f : scale * LOG2E;
-#define PALM_WIDE(PRE) attention_prefill_wide_kernel<PRE><<<grid, PF_THREADS, 0, stream>>>( \
+#define PALM_WIDE(PRE) attention_prefill_wide_kernel<PRE, KEPT><<<grid, PF_THREADS, 0, stream>>>( \
         (const bf16_t*)q, (const bf16_t*)k_cache, (const bf16_t*)v_cache, block_table, max_pages, seq_slot, seq_start, seq_new, \
-        cu_new, nh, nkv, scale_log2, window, qb, hg, (bf16_t*)out)
+        cu_new, nh, nkv, scale_log2, window, qb, hg, (bf16_t*)out, kept)
     if (q_prescaled) PALM_WIDE(true); else PALM_WIDE(false);
 #undef PALM_WIDE
     PALM_LAUNCHED();
     return 0;
+}
+PALM_API int palm_attention_prefill_wide(hipStream_t stream, const void* q, const void* k_cache, const void* v_cache,
+                                         const int* block_table, int max_pages, const int* seq_slot, const int* seq_start,
+                                         const int* seq_new, const int* cu_new, int n_seqs, int max_new, int nh, int nkv,
+                                         int hd, float scale, int window, int q_prescaled, void* out) {
+    return launch_attention_wide<false>(stream, q, k_cache, v_cache, block_table, max_pages, seq_slot, seq_start, seq_new, cu_new, n_seqs, max_new, nh, nkv, hd, scale,
+                                        window, q_prescaled, out, 0);
+}
+// The same with the sequences' first `kept` keys visible behind the window (> 0).
+PALM_API int palm_attention_prefill_wide_kept(hipStream_t stream, const void* q, const void* k_cache, const void* v_cache,
+                                         const int* block_table, int max_pages, const int* seq_slot, const int* seq_start,
+                                         const int* seq_new, const int* cu_new, int n_seqs, int max_new, int nh, int nkv,
+                                         int hd, float scale, int window, int q_prescaled, void* out, int kept) {
+    PALM_CHECK(window > 0 && kept >= 0 && window < 1 << 30 && kept < 1 << 30, "attention_prefill_wide: window=%d kept=%d", window, kept);
+    return launch_attention_wide<true>(stream, q, k_cache, v_cache, block_table, max_pages, seq_slot, seq_start, seq_new, cu_new, n_seqs, max_new, nh, nkv, hd, scale,
+                                        window, q_prescaled, out, kept);
 }
 PALM_API int palm_attention_prefill_wide_serves() { return PF_WIDE ? 1 : 0; }
 

@@ -820,6 +820,8 @@ _ATTENTION_SIGNATURES = {
     "palm_attention_prefill_wide": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
                                     c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p],
     "palm_attention_prefill_wide_serves": [],
+    "palm_attention_prefill_wide_kept": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
+                                         c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p, c_int],
     "palm_attention_decode_fused": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_int,
                                     c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int,
                                     c_int, c_int, c_float, c_int, c_int, c_void_p, c_void_p],
@@ -2876,14 +2878,14 @@ def attention_kept_exact(q: torch.Tensor, k_cache, v_cache, block_table, seq_slo
 
 
 def attention_kept(q: torch.Tensor, k_cache, v_cache, block_table, seq_slot, seq_start, seq_new, cu_new, max_new: int, max_total: int, nh: int,
-                   nkv: int, hd: int, scale: float, window: int, kept: int, q_prescaled: bool = False) -> torch.Tensor:
+                   nkv: int, hd: int, scale: float, window: int, kept: int, q_prescaled: bool = False, wide: bool | None = None, halves: int = 0) -> torch.Tensor:
     """Causal attention of the step's queries over the cache of which a query at position p sees the last ``window`` positions (p - window < j <= p) and the
     sequence's first ``kept`` ones (j < kept): what keeps a stream without an end within a bounded number of pages.
 
     q [n, nh hd]; sequence b has seq_new[b] queries (none, if it is zero) from row cu_new[b] on, at positions seq_start[b] and up, whose keys and values are
     in the cache; ``max_new`` and ``max_total``: the most new tokens of a sequence and the longest sequence with them, or more.  Pages that no query of
     the step sees are not read, whatever the page table says of them; what masked places hold (an infinity, a NaN) does not show.
-    ``q_prescaled``: see ``attention_prefill``."""
+    ``q_prescaled``, ``wide``, ``halves``: see ``attention_prefill`` (None: by the sizes)."""
     what = "attention_kept"
     _dev(what, q, k_cache, v_cache, block_table, seq_slot, seq_start, seq_new, cu_new)
     _i32(what, block_table, seq_slot, seq_start, seq_new, cu_new)
@@ -2917,8 +2919,10 @@ def attention_kept(q: torch.Tensor, k_cache, v_cache, block_table, seq_slot, seq
         _call_on(q.device, lib, "palm_attention_decode_kept", _p(q), _p(k_cache), _p(v_cache), _p(block_table), block_table.shape[1], _p(seq_slot),
                  _p(seq_start), B, nh, nkv, hd, float(scale), window, n_slices, _p(work), _p(out), kept)
         return out
-    _call_on(q.device, lib, "palm_attention_prefill_kept", _p(q), _p(k_cache), _p(v_cache), _p(block_table), block_table.shape[1], _p(seq_slot),
-             _p(seq_start), _p(seq_new), _p(cu_new), B, max_new, nh, nkv, hd, float(scale), window, int(bool(q_prescaled)), max_total, 0, _p(out), kept)
+    more = () if wide else (max_total, int(halves))
+    _call_on(q.device, lib, "palm_attention_prefill_wide_kept" if wide else "palm_attention_prefill_kept", _p(q), _p(k_cache), _p(v_cache),
+             _p(block_table), block_table.shape[1], _p(seq_slot), _p(seq_start), _p(seq_new), _p(cu_new), B, max_new, nh, nkv, hd, float(scale), window,
+             int(bool(q_prescaled)), *more, _p(out), kept)
     return out
 
 
