@@ -1568,13 +1568,14 @@ __global__ __launch_bounds__(HALVES * PF_THREADS) PF_WAVES_PER_SIMD void attenti
     const bf16_t* __restrict__ q, const bf16_t* __restrict__ k_cache, const bf16_t* __restrict__ v_cache,
     const int* __restrict__ block_table, int max_pages, const int* __restrict__ seq_slot,
     const int* __restrict__ seq_start, const int* __restrict__ seq_new, const int* __restrict__ cu_new, int nh,
-    int nkv, float scale_log2, int window, int qb, int hg, int partners_follow, bf16_t* __restrict__ out, int kept) {
+    int nkv, float scale_log2, int window, int qb, int hg, int partners_follow, bf16_t* __restrict__ out, int kept, int slices,
+    float* __restrict__ work) {
     if constexpr (PF_DMA) {
         constexpr int K_TILE = PAGE_TOKENS * K_STRIDE, V_TILE = HD * V_STRIDE;
         __shared__ __attribute__((aligned(16))) bf16_t k_lds[HALVES * 2 * K_TILE];
         __shared__ __attribute__((aligned(16))) bf16_t v_lds[HALVES * 2 * V_TILE];
 
-        const int b = blockIdx.z;
+        const int b = KEPT ? blockIdx.z / slices : blockIdx.z, slice = KEPT ? blockIdx.z % slices : 0;
         const int G = nh / nkv, n_hg = (G + hg - 1) / hg;
         const int kvh = blockIdx.x / n_hg, hgi = blockIdx.x % n_hg;   // the kv head runs fastest over the blocks, see the launch
         const int n_new = seq_new[b];
@@ -1599,14 +1600,24 @@ __global__ __launch_bounds__(HALVES * PF_THREADS) PF_WAVES_PER_SIMD void attenti
             PairedUnit u[PF_UNITS];
 #pragma unroll
             for (int x = 0; x < PF_UNITS; ++x) {
-                const int unit = wave + x * PF_WAVES;
-                const int sub = unit / heads_here;                    // the unit's 16 queries within the tile
-                const int q_first = tile_first + sub * 16;
-                u[x].live = unit < n_units && q_first < n_new;
-                const int qi = q_first + r;
-                u[x].head = kvh * G + hgi * hg + (unit < n_units ? unit % heads_here : 0);
-                u[x].valid = u[x].live && qi < n_new;
-                const int qc = min(qi, n_new - 1);
+                int qi, qc;
+                if constexpr (KEPT) {
+                    const int column = (wave * PF_UNITS + x) * 16 + r, query = column / hg;     // of the tile's (position, head) pairs
+                    qi = tile_first + query;
+                    u[x].live = tile_first + (wave * PF_UNITS + x) * 16 / hg <= min(tile_first + qb, n_new) - 1;
+                    u[x].valid = query < qb && qi < n_new && column % hg < heads_here;
+                    u[x].head = kvh * G + hgi * hg + min(column % hg, heads_here - 1);
+                    qc = min(qi, min(tile_first + qb, n_new) - 1);
+                } else {
+                    const int unit = wave + x * PF_WAVES;
+                    const int sub = unit / heads_here;                // the unit's 16 queries within the tile
+                    const int q_first = tile_first + sub * 16;
+                    u[x].live = unit < n_units && q_first < n_new;
+                    qi = q_first + r;
+                    u[x].head = kvh * G + hgi * hg + (unit < n_units ? unit % heads_here : 0);
+                    u[x].valid = u[x].live && qi < n_new;
+                    qc = min(qi, n_new - 1);
+                }
                 u[x].pos = start + qc;
                 u[x].first = window > 0 ? max(0, u[x].pos - window + 1) : 0;
                 u[x].row = (size_t)cu_new[b] + qc;
@@ -1618,9 +1629,11 @@ __global__ __launch_bounds__(HALVES * PF_THREADS) PF_WAVES_PER_SIMD void attenti
             }
             // the pages any query of the tile sees (the same for all waves)
             const int tile_last = min(tile_first + qb - 1, n_new - 1);
-            const int p_hi = (start + tile_last) / PAGE_TOKENS;
+            const int row_hi = (start + tile_last) / PAGE_TOKENS;
             const int page_lo = window > 0 ? max(0, start + tile_first - window + 1) / PAGE_TOKENS : 0;
-            const int front = pages_in_front<KEPT>(kept, page_lo), p_lo = page_lo - front;          // the row of pages, see page_of_row
+            const int front = pages_in_front<KEPT>(kept, page_lo), row_lo = page_lo - front;        // the row of pages, see page_of_row
+            const int per = KEPT ? (row_hi - row_lo + slices) / slices : 0;                         // pages of a slice of it
+            const int p_lo = KEPT ? row_lo + slice * per : row_lo, p_hi = KEPT ? min(row_hi, p_lo + per - 1) : row_hi;
             // of every HALVES pages in turn each half takes one, into two places of its own
             bf16_t *k_half = k_lds + half * 2 * K_TILE, *v_half = v_lds + half * 2 * V_TILE;
             auto load_page = [&](int p, int step) {
@@ -1664,7 +1677,7 @@ __global__ __launch_bounds__(HALVES * PF_THREADS) PF_WAVES_PER_SIMD void attenti
                 wait_for_all_but_the_youngest_loads<0>();             // the half's next page has landed
                 page_barrier();
             }
-            if (HALVES > 1 && p_lo == p_hi) {                         // one page: the first half had it
+            if (HALVES > 1 && p_lo >= p_hi) {                         // one page: the first half had it
                 if (half == 1) return;
             } else if constexpr (HALVES > 1) {
                 // the second half's sums go through LDS (nobody reads pages any more, none is on its way) to the same lanes of the first
@@ -1689,6 +1702,7 @@ __global__ __launch_bounds__(HALVES * PF_THREADS) PF_WAVES_PER_SIMD void attenti
                     const float top = fmaxf(u[x].m, other.x), from = top == -INFINITY ? 0.f : top;   // (a half may have seen none of the column's keys)
                     const float mine = exp2_weight(u[x].m - from), its = exp2_weight(other.x - from);
                     u[x].weights[0] = u[x].weights[0] * mine + other.y * its;
+                    if (KEPT) u[x].m = top;
 #pragma unroll
                     for (int dt = 0; dt < DTILES; ++dt) {
                         const float4 o = o_lds[((wave * PF_UNITS + x) * DTILES + dt) * WAVE + lane];
@@ -1706,6 +1720,20 @@ __global__ __launch_bounds__(HALVES * PF_THREADS) PF_WAVES_PER_SIMD void attenti
                                         [&](int key) { return key_is_seen<true>(key, u[x].first - key0, u[x].pos - key0, kept - key0); });
                 }
             }
+            if (KEPT && slices > 1) {
+                // a record for each (row, head, slice): reference, sum, two floats unused, the unnormalised output; an empty one has no output
+#pragma unroll
+                for (int x = 0; x < PF_UNITS; ++x) {
+                    if (!u[x].valid) continue;
+                    float* record = work + ((u[x].row * nh + u[x].head) * slices + slice) * WORK_STRIDE;
+                    if (g == 0) *reinterpret_cast<float2*>(record) = make_float2(u[x].m, u[x].weights[0]);
+                    if (u[x].m == -INFINITY) continue;
+#pragma unroll
+                    for (int dt = 0; dt < DTILES; ++dt)
+                        *reinterpret_cast<float4*>(record + WORK_O + dt * 16 + 4 * g) = make_float4(u[x].o[dt][0], u[x].o[dt][1], u[x].o[dt][2], u[x].o[dt][3]);
+                }
+                return;
+            }
 #pragma unroll
             for (int x = 0; x < PF_UNITS; ++x) {
                 if (u[x].valid) {
@@ -1722,6 +1750,30 @@ __global__ __launch_bounds__(HALVES * PF_THREADS) PF_WAVES_PER_SIMD void attenti
             }
         }
     }
+}
+
+// A wave for each (row, head) of a prompt whose rows of pages were cut: the slices' records in their order.
+constexpr int JOIN_WAVES = 4;
+__global__ __launch_bounds__(JOIN_WAVES * WAVE) void attention_prefill_join_kernel(const float* __restrict__ work, int slices, long long heads, bf16_t* __restrict__ out) {
+    constexpr int PER = (HD + WAVE - 1) / WAVE;
+    const long long head = (long long)blockIdx.x * JOIN_WAVES + threadIdx.x / WAVE;
+    if (head >= heads) return;
+    const int lane = threadIdx.x % WAVE;
+    const float* w = work + head * slices * WORK_STRIDE;
+    const float2 mine = *reinterpret_cast<const float2*>(w + (size_t)min(lane, slices - 1) * WORK_STRIDE);
+    const float m = wave_max(lane < slices ? mine.x : -INFINITY);
+    const float wt = lane < slices ? exp2_weight(mine.x - m) : 0.f;        // (an empty slice's: zero)
+    const float l = wave_sum(lane < slices ? mine.y * wt : 0.f);
+    float o[PER] = {};
+    for (int s = 0; s < slices; ++s) {
+        const float ws = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wt), s));
+        if (__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine.x), s)) == -INFINITY) continue;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) o[i] += w[(size_t)s * WORK_STRIDE + WORK_O + min(lane + i * WAVE, HD - 1)] * ws;
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+        if (lane + i * WAVE < HD) out[head * HD + lane + i * WAVE] = f32_to_bf16(o[i] / l);
 }
 
 // ---- prefill of long prompts: 64 columns a wave -----------------------------------------------------
@@ -2150,7 +2202,7 @@ template <bool KEPT>
 static int launch_attention_prefill(hipStream_t stream, const void* q, const void* k_cache, const void* v_cache,
                                        const int* block_table, int max_pages, const int* seq_slot, const int* seq_start,
                                        const int* seq_new, const int* cu_new, int n_seqs, int max_new, int nh, int nkv,
-                                       int hd, float scale, int window, int q_prescaled, int max_keys, int halves, void* out, int kept) {
+                                       int hd, float scale, int window, int q_prescaled, int max_keys, int halves, void* out, int kept, int rows, int slices, float* work) {
     PALM_CHECK(hd == HD, "attention_prefill: this library was built for head size %d, not %d", HD, hd);
     PALM_CHECK(n_seqs >= 0 && max_new >= 0 && nh > 0 && nkv > 0 && nh % nkv == 0,
                "attention_prefill: seqs=%d max_new=%d heads=%d kv=%d", n_seqs, max_new, nh, nkv);
@@ -2159,8 +2211,9 @@ static int launch_attention_prefill(hipStream_t stream, const void* q, const voi
     if (n_seqs == 0 || max_new == 0) return 0;
     const int G = nh / nkv;
     constexpr int UNITS = PF_UNITS * PF_WAVES;                 // (head, 16 queries) units a block holds
-    const int hg = G < UNITS ? G : UNITS;                      // query heads of the group served by one block
-    const int qb = 16 * (UNITS / hg > 0 ? UNITS / hg : 1);     // query positions in a tile
+    constexpr bool COLUMNS = KEPT && PF_DMA;                   // (position, head) pairs are columns one by one, not by 16 positions
+    const int hg = COLUMNS ? min(G, UNITS * 16) : min(G, UNITS);                              // query heads of the group served by one block
+    const int qb = COLUMNS ? UNITS * 16 / hg : 16 * (UNITS / hg > 0 ? UNITS / hg : 1);        // query positions in a tile
     const int n_hg = (G + hg - 1) / hg;
     PALM_CHECK(nkv * n_hg <= 65535 && n_seqs <= 65535, "attention_prefill: grid too large");
     const float scale_log2 = q_prescaled ? 1.0f : scale * LOG2E;
@@ -2170,17 +2223,23 @@ static int launch_attention_prefill(hipStream_t stream, const void* q, const voi
     if constexpr (PF_DMA) {
         const int n_q = (max_new + qb - 1) / qb;
         PALM_CHECK(n_q <= 65535, "attention_prefill: %d new tokens are more than one launch takes", max_new);
-        dim3 grid(nkv * n_hg, n_q, n_seqs);
+        PALM_CHECK(slices >= 1 && slices <= WAVE && (long long)n_seqs * slices <= 65535 && (slices == 1 || work), "attention_prefill: %d slices", slices);
+        dim3 grid(nkv * n_hg, n_q, n_seqs * slices);
         const long long blocks = (long long)grid.x * grid.y * grid.z;
         const bool few = halves ? halves == 2 : prefill_takes_halves(n_seqs, max_new, max_keys, nh, nkv, KEPT ? window + kept : window);
         const int partners_follow = !few && blocks <= 512 && n_seqs == 1;     // all blocks run at once, two a unit
 #define PALM_PAIRED(HALVES, PRE) attention_prefill_paired_kernel<HALVES, PRE, KEPT><<<grid, HALVES * PF_THREADS, 0, stream>>>( \
         (const bf16_t*)q, (const bf16_t*)k_cache, (const bf16_t*)v_cache, block_table, max_pages, seq_slot, seq_start, seq_new, \
-        cu_new, nh, nkv, scale_log2, window, qb, hg, partners_follow, (bf16_t*)out, kept)
+        cu_new, nh, nkv, scale_log2, window, qb, hg, partners_follow, (bf16_t*)out, kept, slices, work)
         if (few) { if (q_prescaled) PALM_PAIRED(2, true); else PALM_PAIRED(2, false); }
         else { if (q_prescaled) PALM_PAIRED(1, true); else PALM_PAIRED(1, false); }
 #undef PALM_PAIRED
         PALM_LAUNCHED();
+        if (slices > 1) {
+            const long long heads = (long long)rows * nh;
+            attention_prefill_join_kernel<<<(unsigned)((heads + JOIN_WAVES - 1) / JOIN_WAVES), JOIN_WAVES * WAVE, 0, stream>>>(work, slices, heads, (bf16_t*)out);
+            PALM_LAUNCHED();
+        }
         return 0;
     }
     PALM_CHECK(!q_prescaled, "attention_prefill: head size %d takes its queries as they are and applies the scale itself", HD);
@@ -2200,16 +2259,17 @@ PALM_API int palm_attention_prefill_in(hipStream_t stream, const void* q, const 
                                        const int* seq_new, const int* cu_new, int n_seqs, int max_new, int nh, int nkv,
                                        int hd, float scale, int window, int q_prescaled, int max_keys, int halves, void* out) {
     return launch_attention_prefill<false>(stream, q, k_cache, v_cache, block_table, max_pages, seq_slot, seq_start, seq_new, cu_new, n_seqs, max_new, nh, nkv, hd, scale,
-                                           window, q_prescaled, max_keys, halves, out, 0);
+                                           window, q_prescaled, max_keys, halves, out, 0, 0, 1, nullptr);
 }
-// The same with the sequences' first `kept` keys visible behind the window (> 0).
+// The same with the sequences' first `kept` keys visible behind the window (> 0).  Each sequence's pages may be cut into slices whose
+// results meet in `work`: rows (of q) * nh * slices * (hd + 4) floats.
 PALM_API int palm_attention_prefill_kept(hipStream_t stream, const void* q, const void* k_cache, const void* v_cache,
                                        const int* block_table, int max_pages, const int* seq_slot, const int* seq_start,
                                        const int* seq_new, const int* cu_new, int n_seqs, int max_new, int nh, int nkv,
-                                       int hd, float scale, int window, int q_prescaled, int max_keys, int halves, void* out, int kept) {
+                                       int hd, float scale, int window, int q_prescaled, int max_keys, int halves, void* out, int kept, int rows, int slices, float* work) {
     PALM_CHECK(window > 0 && kept >= 0 && window < 1 << 30 && kept < 1 << 30, "attention_prefill: window=%d kept=%d", window, kept);
     return launch_attention_prefill<true>(stream, q, k_cache, v_cache, block_table, max_pages, seq_slot, seq_start, seq_new, cu_new, n_seqs, max_new, nh, nkv, hd, scale,
-                                           window, q_prescaled, max_keys, halves, out, kept);
+                                           window, q_prescaled, max_keys, halves, out, kept, rows, slices, work);
 }
 
 PALM_API int palm_attention_prefill(hipStream_t stream, const void* q, const void* k_cache, const void* v_cache,

@@ -831,7 +831,8 @@ _ATTENTION_SIGNATURES = {
     "palm_attention_decode_kept": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int,
                                    c_int, c_int, c_float, c_int, c_int, c_void_p, c_void_p, c_int],
     "palm_attention_prefill_kept": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
-                                    c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_int, c_void_p, c_int],
+                                    c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_int, c_void_p, c_int, c_int,
+                                    c_int, c_void_p],
     "palm_attention_decode_fused_kept": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_int,
                                          c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int,
                                          c_int, c_int, c_float, c_int, c_int, c_void_p, c_void_p, c_int],
@@ -2878,14 +2879,14 @@ def attention_kept_exact(q: torch.Tensor, k_cache, v_cache, block_table, seq_slo
 
 
 def attention_kept(q: torch.Tensor, k_cache, v_cache, block_table, seq_slot, seq_start, seq_new, cu_new, max_new: int, max_total: int, nh: int,
-                   nkv: int, hd: int, scale: float, window: int, kept: int, q_prescaled: bool = False, wide: bool | None = None, halves: int = 0) -> torch.Tensor:
+                   nkv: int, hd: int, scale: float, window: int, kept: int, q_prescaled: bool = False, plan: tuple | None = None) -> torch.Tensor:
     """Causal attention of the step's queries over the cache of which a query at position p sees the last ``window`` positions (p - window < j <= p) and the
     sequence's first ``kept`` ones (j < kept): what keeps a stream without an end within a bounded number of pages.
 
     q [n, nh hd]; sequence b has seq_new[b] queries (none, if it is zero) from row cu_new[b] on, at positions seq_start[b] and up, whose keys and values are
     in the cache; ``max_new`` and ``max_total``: the most new tokens of a sequence and the longest sequence with them, or more.  Pages that no query of
     the step sees are not read, whatever the page table says of them; what masked places hold (an infinity, a NaN) does not show.
-    ``q_prescaled``, ``wide``, ``halves``: see ``attention_prefill`` (None: by the sizes)."""
+    ``q_prescaled``: see ``attention_prefill``.  ``plan``: (wide, halves, slices), how a prompt goes on the matrix cores (None: ``kept_plan``)."""
     what = "attention_kept"
     _dev(what, q, k_cache, v_cache, block_table, seq_slot, seq_start, seq_new, cu_new)
     _i32(what, block_table, seq_slot, seq_start, seq_new, cu_new)
@@ -2919,11 +2920,60 @@ def attention_kept(q: torch.Tensor, k_cache, v_cache, block_table, seq_slot, seq
         _call_on(q.device, lib, "palm_attention_decode_kept", _p(q), _p(k_cache), _p(v_cache), _p(block_table), block_table.shape[1], _p(seq_slot),
                  _p(seq_start), B, nh, nkv, hd, float(scale), window, n_slices, _p(work), _p(out), kept)
         return out
-    more = () if wide else (max_total, int(halves))
-    _call_on(q.device, lib, "palm_attention_prefill_wide_kept" if wide else "palm_attention_prefill_kept", _p(q), _p(k_cache), _p(v_cache),
-             _p(block_table), block_table.shape[1], _p(seq_slot), _p(seq_start), _p(seq_new), _p(cu_new), B, max_new, nh, nkv, hd, float(scale), window,
-             int(bool(q_prescaled)), *more, _p(out), kept)
+    wide, halves, slices = plan or kept_plan(n, B, max_total, nh, nkv, hd, window, kept)
+    if wide:
+        _call_on(q.device, lib, "palm_attention_prefill_wide_kept", _p(q), _p(k_cache), _p(v_cache), _p(block_table), block_table.shape[1], _p(seq_slot),
+                 _p(seq_start), _p(seq_new), _p(cu_new), B, max_new, nh, nkv, hd, float(scale), window, int(bool(q_prescaled)), _p(out), kept)
+        return out
+    work = torch.empty((n * nh * slices * (hd + 4),), dtype=F32, device=q.device) if slices > 1 else None
+    _call_on(q.device, lib, "palm_attention_prefill_kept", _p(q), _p(k_cache), _p(v_cache), _p(block_table), block_table.shape[1], _p(seq_slot),
+             _p(seq_start), _p(seq_new), _p(cu_new), B, max_new, nh, nkv, hd, float(scale), window, int(bool(q_prescaled)), max_total, int(halves),
+             _p(out), kept, n, int(slices), _p(work))
     return out
+
+
+@functools.lru_cache(maxsize=4096)
+def kept_plan(rows: int, n_seqs: int, max_total: int, nh: int, nkv: int, hd: int, window: int, kept: int) -> tuple:
+    """How ``attention_kept`` takes a step of ``rows`` queries of several a sequence: (by the kernel of 64 columns a wave, halves of a block, slices of a
+    row of pages).
+
+    A block holds 128 columns, (position, head) pairs of a kv head, and walks its row of pages.  With one half two blocks share a compute unit; with
+    two, which take every other page, it has it to itself.  Slices are blocks of their own whose results a second kernel joins: it starts in some 5 us
+    and passes every slice's output through memory.  us, (halves, slices): 64 tokens behind 6,000, window 4,096, 32 heads of 128 on 8 (16 blocks of 66 pages) (1, 1) 121,
+    (2, 1) 89, (2, 4) 34, (2, 12) 26, (2, 16) 28; 517 behind 6,000, window 1,000 (136 blocks of 19) 42, 36, 49, (1, 3) 35; 16 heads of 64 on 4 (68 blocks) 30, 26,
+    (2, 3) 20; 7 behind 8,000 in a window of 8,000 (8 blocks of 126) 185, 137, (2, 16) 25; three times 700 behind 5,000 to 9,000, window 2,048 (528 of 34) 151, 151,
+    (1, 2) 130; 1,000 from the start, window 128 (256 of 4) 19, 17, (2, 2) 36; 8,192, window 2,048 (2,048 of 34) 291, 351.
+
+    The other kernel is sooner where rows are long, blocks many and its sixteen units all used (16 heads of 128 on 2, 16,000 tokens, window 8,192: 670 and 768; 32 on
+    8, 5,000, window 4,000: 198 and 213; 8,192, window 4,096 428 and 432, 2,048 328 and 291)."""
+    if hd not in (64, 128):
+        return False, 0, 1
+    group = nh // nkv
+    heads = min(group, 128)
+    queries = 128 // heads                                       # of a block
+    blocks = nkv * -(-group // heads) * (-(-rows // queries) + n_seqs // 2)
+    keys = min(max_total, window + queries + PAGE_TOKENS + (kept + PAGE_TOKENS - 1) // PAGE_TOKENS * PAGE_TOKENS)
+    pages = -(-keys // PAGE_TOKENS)
+    if hd == 128 and pages >= 64 and 16 % group == 0 and blocks >= 512 and attention_lib(hd).palm_attention_prefill_wide_serves():
+        return True, 0, 1
+    # Fitted to 62 such steps: the way taken is 2 % slower than the best of them in the mean.  A page takes 1.6 us where one half has the unit to itself, 1.75
+    # beside another block, 0.97 by two halves, and 0.8 of it more for up to four pages with masks.  Blocks beyond those that run at once come in further
+    # rounds, which prompts from their start, whose first tiles are short, do not fill.
+    page = 0.3 + 0.7 * hd / 128
+    from_start = max_total * n_seqs < 2 * rows
+    best = None
+    for slices in (1, 2, 3, 4, 6, 8, 12, 16):
+        if slices > 1 and (slices > pages or blocks * slices > 4 * COMPUTE_UNITS or n_seqs * slices > 65535):
+            break
+        each, launched = -(-pages // slices), blocks * slices
+        walk = page * (each + 0.8 * min(each, 4))
+        join = 0.0 if slices == 1 else 3.0 + 0.2 * slices + rows * nh * slices * (hd + 4) * 8 / 8e6
+        for halves, at_once, us in ((1, 2 * COMPUTE_UNITS, 7.0 + (1.6 if launched <= COMPUTE_UNITS else 1.75) * walk), (2, COMPUTE_UNITS, 9.0 + 0.97 * walk)):
+            if launched > at_once:
+                us *= launched / at_once + 0.3 if from_start else -(-launched // at_once)
+            if best is None or us + join < best[0]:
+                best = us + join, halves, slices
+    return False, best[1], best[2]
 
 
 def _kept_keys(max_total: int, window: int, kept: int) -> int:

@@ -146,6 +146,39 @@ def test_what_masked_places_hold_does_not_show(ops, nh, nkv, hd, seqs, dtype):
     case.check(case.run(ops))
 
 
+PLANS = [(False, 1, 1), (False, 2, 1), (False, 1, 3), (False, 2, 5), (False, 1, 16), (False, 2, 2), (True, 0, 1)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("plan", PLANS)
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 128), (5, 1, 128), (24, 1, 64), (40, 1, 128), (2, 2, 64), (3, 1, 128), (140, 1, 64)])
+@pytest.mark.parametrize("window,kept", [(40, 4), (200, 65)])
+def test_every_way_a_prompt_goes(ops, nh, nkv, hd, window, kept, plan):
+    """Two halves, slices (more of them than pages too), 64 columns a wave: whatever the plan, and with values that only some queries see."""
+    if plan[0] and hd != 128:
+        pytest.skip("heads of 128 only")
+    case = Case([(0, 60), (500, 37), (130, 0), (320, 1)], nh, nkv, hd, window, kept, BF16, seed=nh)
+    case.check(case.run(ops, plan=plan))
+    for b, j in ((0, 10), (1, 480), (1, 520), (3, 300), (1, 2)):
+        case.v[case.place(b, j)[0], 0, :5, j % 64] = math.inf if j % 20 else math.nan
+    case.check(case.run(ops, plan=plan))
+
+
+@pytest.mark.gpu
+def test_prescaled_queries(ops):
+    """Queries that carry scale and log2 e already, rounded with them: as the step hands them over."""
+    case = Case([(0, 60), (500, 37)], 8, 2, 128, 90, 4, BF16, seed=2)
+    plain = Case([(0, 60), (500, 37)], 8, 2, 128, 90, 4, BF16, seed=2)
+    factor = ops.prefill_q_scale(128, BF16, 128 ** -0.5)
+    assert factor != 1.0
+    case.q = (case.q.float() * factor).to(BF16)
+    plain.q = case.q.double() / (128 ** -0.5 * ops.LOG2E)
+    want, off = plain.plain()
+    for plan in [p for p in PLANS] + [None]:
+        got = case.run(ops, plan=plan, q_prescaled=True)
+        assert bool(((got.double() - want).abs() <= off).all())
+
+
 @pytest.mark.gpu
 def test_without_first_positions_it_is_the_window_alone(ops):
     """The framework's other window, on the same step."""
@@ -207,6 +240,22 @@ def test_refusals(ops, monkeypatch):
     _refused(ops, "room for 256", max_total=257)
     _refused(ops, "3 new tokens", max_new=3, max_total=2)
     _refused(ops, "int32", seq_slot=z(2, dtype=torch.int64))
+
+
+def test_plans_of_prompts(ops, monkeypatch):
+    """A way that there is, for any sizes; slices only where they find pages, and not where blocks are many."""
+    class Lib:
+        palm_attention_prefill_wide_serves = staticmethod(lambda: 1)
+    monkeypatch.setattr(ops, "attention_lib", lambda hd: Lib)
+    ops.kept_plan.cache_clear()
+    assert ops.kept_plan(100, 1, 100, 4, 2, 80, 64, 4) == (False, 0, 1)
+    for rows, n, total, nh, nkv, hd, window, kept in [(2, 1, 2, 4, 2, 64, 1, 0), (64, 1, 6064, 32, 8, 128, 4096, 4), (8192, 1, 8192, 32, 8, 128, 2048, 64), (5, 64, 900, 64, 1, 64, 1 << 29, 1 << 29),
+                                                      (60000, 1, 60000, 32, 8, 128, 8192, 4), (300, 300, 40000, 160, 1, 128, 5000, 0)]:
+        wide, halves, slices = ops.kept_plan(rows, n, total, nh, nkv, hd, window, kept)
+        assert (wide and (halves, slices) == (0, 1) and hd == 128) or (halves in (1, 2) and 1 <= slices <= 16)
+        assert slices <= -(-total // 64)
+    assert ops.kept_plan(64, 1, 6064, 32, 8, 128, 4096, 4)[2] >= 8 and ops.kept_plan(8192, 1, 8192, 32, 8, 128, 2048, 64) == (False, 1, 1)
+    ops.kept_plan.cache_clear()
 
 
 def test_slices_fill_the_chip_and_leave_no_wave_without_a_page(ops):

@@ -145,3 +145,16 @@ def test_wide_attention_waits_for_loads_where_it_says_so_and_keeps_nothing_in_me
     waits = [i for i, one in enumerate(code) if one.name == "s_waitcnt" and "vmcnt" in one.text and products[0] < i < products[-1]]
     of_the_table = [i for i in waits if "vmcnt(0)" in code[i].text and code[i - 1].name == "global_load_dword"]
     assert len(of_the_table) <= 1 and ["vmcnt(8)" in code[i].text for i in waits if i not in of_the_table] == [True]
+
+
+@pytest.mark.parametrize("prescaled", [1, 0])
+def test_wide_attention_that_keeps_first_positions_keeps_its_products_distances(attention_of_heads_of_128, prescaled):
+    """With the sequence's first positions visible too; loads stay on their way there as well, and nothing goes through memory."""
+    code, following = kernel(attention_of_heads_of_128, f"attention_prefill_wide_kernelILb{prescaled}ELb1E")
+    assert sum(one.written_out for one in code) == 4 * 34
+    assert too_near(code, following) == []
+    assert not any(one.name.startswith("scratch_") for one in code)
+    products = [i for i, one in enumerate(code) if one.written_out]
+    waits = [i for i, one in enumerate(code) if one.name == "s_waitcnt" and "vmcnt" in one.text and products[0] < i < products[-1]]
+    of_the_table = [i for i in waits if "vmcnt(0)" in code[i].text and code[i - 1].name == "global_load_dword"]
+    assert len(of_the_table) <= 1 and ["vmcnt(8)" in code[i].text for i in waits if i not in of_the_table] == [True]
