@@ -1323,8 +1323,10 @@ def pages_lib():
 
 
 def logprobs_lib():
-    lib = _small("logprobs", _LOGPROBS_SIGNATURES)
-    lib.palm_token_logprobs_work.restype = c_longlong
+    lib = _small_libraries.get("logprobs")
+    if lib is None:
+        lib = _small("logprobs", _LOGPROBS_SIGNATURES)
+        lib.palm_token_logprobs_work.restype = c_longlong
     return lib
 
 
@@ -2872,25 +2874,17 @@ def attention_kept_exact(q: torch.Tensor, k_cache, v_cache, block_table, seq_slo
         return out
     slices = _kept_slices(B, max_new, max_total, nh, nkv, window, kept)
     work = torch.empty((n * nh * slices * (hd + 4),), dtype=F32, device=q.device) if slices > 1 else None
-    _call_on(q.device, attention_kept_lib(), "palm_attention_kept", _p(q), _code(q, "attention_kept q"), _p(k_cache), _p(v_cache), _p(block_table),
+    _call_on(q.get_device(), attention_kept_lib(), "palm_attention_kept", _p(q), _code(q, "attention_kept q"), _p(k_cache), _p(v_cache), _p(block_table),
              block_table.shape[1], _p(seq_slot), _p(seq_start), _p(seq_new), _p(cu_new), B, n, int(max_new), nh, nkv, hd, float(scale), window, kept,
              slices, _p(work), _p(out))
     return out
 
 
-def attention_kept(q: torch.Tensor, k_cache, v_cache, block_table, seq_slot, seq_start, seq_new, cu_new, max_new: int, max_total: int, nh: int,
-                   nkv: int, hd: int, scale: float, window: int, kept: int, q_prescaled: bool = False, plan: tuple | None = None) -> torch.Tensor:
-    """Causal attention of the step's queries over the cache of which a query at position p sees the last ``window`` positions (p - window < j <= p) and the
-    sequence's first ``kept`` ones (j < kept): what keeps a stream without an end within a bounded number of pages.
-
-    q [n, nh hd]; sequence b has seq_new[b] queries (none, if it is zero) from row cu_new[b] on, at positions seq_start[b] and up, whose keys and values are
-    in the cache; ``max_new`` and ``max_total``: the most new tokens of a sequence and the longest sequence with them, or more.  Pages that no query of
-    the step sees are not read, whatever the page table says of them; what masked places hold (an infinity, a NaN) does not show.
-    ``q_prescaled``: see ``attention_prefill``.  ``plan``: (wide, halves, slices), how a prompt goes on the matrix cores (None: ``kept_plan``)."""
+def _refuse_kept(q, k_cache, v_cache, block_table, seq_slot, seq_start, seq_new, cu_new, max_new, max_total, nh, nkv, hd, window, kept) -> None:
+    """Says what ``attention_kept`` does not take of these."""
     what = "attention_kept"
     _dev(what, q, k_cache, v_cache, block_table, seq_slot, seq_start, seq_new, cu_new)
     _i32(what, block_table, seq_slot, seq_start, seq_new, cu_new)
-    window, kept, max_new, max_total = int(window), int(kept), int(max_new), int(max_total)
     if not (nh > 0 and nkv > 0 and nh % nkv == 0):
         raise KernelError(f"{what}: {nh} heads are not a multiple of {nkv} kv heads")
     if not (q.dim() == 2 and q.shape[1] == nh * hd):
@@ -2906,27 +2900,50 @@ def attention_kept(q: torch.Tensor, k_cache, v_cache, block_table, seq_slot, seq
         raise KernelError(f"{what}: a window of {window} positions and {kept} first ones: at least one, and none or more")
     if not (0 <= max_new <= max_total <= block_table.shape[1] * PAGE_TOKENS):
         raise KernelError(f"{what}: {max_new} new tokens in sequences of up to {max_total}; the page table has room for {block_table.shape[1] * PAGE_TOKENS}")
-    if not mfma_attention_serves(q, hd):
+    raise KernelError(f"{what}: sizes are whole numbers")
+
+
+def attention_kept(q: torch.Tensor, k_cache, v_cache, block_table, seq_slot, seq_start, seq_new, cu_new, max_new: int, max_total: int, nh: int,
+                   nkv: int, hd: int, scale: float, window: int, kept: int, q_prescaled: bool = False, plan: tuple | None = None) -> torch.Tensor:
+    """Causal attention of the step's queries over the cache of which a query at position p sees the last ``window`` positions (p - window < j <= p) and the
+    sequence's first ``kept`` ones (j < kept): what keeps a stream without an end within a bounded number of pages.
+
+    q [n, nh hd]; sequence b has seq_new[b] queries (none, if it is zero) from row cu_new[b] on, at positions seq_start[b] and up, whose keys and values are
+    in the cache; ``max_new`` and ``max_total``: the most new tokens of a sequence and the longest sequence with them, or more.  Pages that no query of
+    the step sees are not read, whatever the page table says of them; what masked places hold (an infinity, a NaN) does not show.
+    ``q_prescaled``: see ``attention_prefill``.  ``plan``: (wide, halves, slices), how a prompt goes on the matrix cores (None: ``kept_plan``)."""
+    dev = q.get_device()
+    n, B = q.shape[0], seq_slot.shape[0]
+    # what is wrong is looked for only where something is (the checks one by one took the host 6 us at every call, together 2)
+    if not (dev >= 0 and dev == k_cache.get_device() == v_cache.get_device() == block_table.get_device() == seq_slot.get_device() == seq_start.get_device()
+            == seq_new.get_device() == cu_new.get_device() and q.is_contiguous() and k_cache.is_contiguous() and v_cache.is_contiguous()
+            and block_table.is_contiguous() and seq_slot.is_contiguous() and seq_start.is_contiguous() and seq_new.is_contiguous() and cu_new.is_contiguous()
+            and block_table.dtype is seq_slot.dtype is seq_start.dtype is seq_new.dtype is cu_new.dtype is torch.int32
+            and q.dtype is k_cache.dtype is v_cache.dtype and q.dtype in _CODES and nh > 0 and nkv > 0 and nh % nkv == 0
+            and q.shape == (n, nh * hd) and k_cache.shape[1:] == (nkv, PAGE_TOKENS, hd) and v_cache.shape == (k_cache.shape[0], nkv, hd, PAGE_TOKENS)
+            and seq_start.shape == seq_new.shape == seq_slot.shape == (B,) and cu_new.shape == (B + 1,) and 1 <= window < 1 << 30 and 0 <= kept < 1 << 30
+            and block_table.dim() == 2 and 0 <= max_new <= max_total <= block_table.shape[1] * PAGE_TOKENS):
+        _refuse_kept(q, k_cache, v_cache, block_table, seq_slot, seq_start, seq_new, cu_new, max_new, max_total, nh, nkv, hd, window, kept)
+    if not (q.dtype is BF16 and hd in MFMA_HEAD_DIMS):
         _need(not q_prescaled, "attention_kept: only the prompt kernel takes scaled queries")
         return attention_kept_exact(q, k_cache, v_cache, block_table, seq_slot, seq_start, seq_new, cu_new, max_new, max_total, nh, nkv, hd, scale, window, kept)
     out = torch.empty_like(q)
-    n = q.shape[0]
     if n == 0 or B == 0 or max_new == 0:
         return out
     lib = attention_lib(hd)
     if max_new == 1 and n == B and not q_prescaled:              # (one token each: as many as there are sequences)
         n_slices = decode_slices(B, nh, nkv, _kept_keys(max_total, window, kept))
         work = torch.empty((B * nh * n_slices * (hd + 4),), dtype=F32, device=q.device) if n_slices > 1 else None
-        _call_on(q.device, lib, "palm_attention_decode_kept", _p(q), _p(k_cache), _p(v_cache), _p(block_table), block_table.shape[1], _p(seq_slot),
+        _call_on(q.get_device(), lib, "palm_attention_decode_kept", _p(q), _p(k_cache), _p(v_cache), _p(block_table), block_table.shape[1], _p(seq_slot),
                  _p(seq_start), B, nh, nkv, hd, float(scale), window, n_slices, _p(work), _p(out), kept)
         return out
     wide, halves, slices = plan or kept_plan(n, B, max_total, nh, nkv, hd, window, kept)
     if wide:
-        _call_on(q.device, lib, "palm_attention_prefill_wide_kept", _p(q), _p(k_cache), _p(v_cache), _p(block_table), block_table.shape[1], _p(seq_slot),
+        _call_on(q.get_device(), lib, "palm_attention_prefill_wide_kept", _p(q), _p(k_cache), _p(v_cache), _p(block_table), block_table.shape[1], _p(seq_slot),
                  _p(seq_start), _p(seq_new), _p(cu_new), B, max_new, nh, nkv, hd, float(scale), window, int(bool(q_prescaled)), _p(out), kept)
         return out
     work = torch.empty((n * nh * slices * (hd + 4),), dtype=F32, device=q.device) if slices > 1 else None
-    _call_on(q.device, lib, "palm_attention_prefill_kept", _p(q), _p(k_cache), _p(v_cache), _p(block_table), block_table.shape[1], _p(seq_slot),
+    _call_on(q.get_device(), lib, "palm_attention_prefill_kept", _p(q), _p(k_cache), _p(v_cache), _p(block_table), block_table.shape[1], _p(seq_slot),
              _p(seq_start), _p(seq_new), _p(cu_new), B, max_new, nh, nkv, hd, float(scale), window, int(bool(q_prescaled)), max_total, int(halves),
              _p(out), kept, n, int(slices), _p(work))
     return out
@@ -2983,9 +3000,9 @@ def _kept_keys(max_total: int, window: int, kept: int) -> int:
 
 # ---- pages of the cache copied to other pages (library ``pages``) ----------------------------------------------------
 
-def _call_on(device: torch.device, lib, fn_name: str, *args) -> None:
-    """``library.call`` with ``device`` current, on torch's current stream there."""
-    if device.index == torch._C._cuda_getDevice():
+def _call_on(device, lib, fn_name: str, *args) -> None:
+    """``library.call`` with ``device`` (or its number) current, on torch's current stream there."""
+    if (device if device.__class__ is int else device.index) == torch._C._cuda_getDevice():
         library.call(lib, fn_name, _stream(), *args)
         return
     with torch.cuda.device(device):
@@ -3086,11 +3103,12 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
     if not (0 <= top <= min(LOGPROBS_MOST, V)):
         raise KernelError(f"{what}: the {top} likeliest of {V} tokens ({LOGPROBS_MOST} at most)")
     dev = logits.device
-    out = torch.empty((n * (2 + top),), dtype=F32, device=dev)
-    given, entropy, best = out[:n], out[n:2 * n], out[2 * n:].view(n, top)
+    given = torch.empty((n,), dtype=F32, device=dev) if tokens is not None else None
+    entropy = torch.empty((n,), dtype=F32, device=dev)
     ids = torch.empty((n, top), dtype=torch.int32, device=dev)
+    best = torch.empty((n, top), dtype=F32, device=dev)
     if n:
         needed = _logprobs_work(n, V, top)
         work = torch.empty((needed,), dtype=torch.uint8, device=dev) if needed else None
         _call_on(dev, logprobs_lib(), "palm_token_logprobs", _p(logits), n, V, _p(tokens), top, _p(work), needed, _p(given), _p(entropy), _p(ids), _p(best))
-    return (given if tokens is not None else None), entropy, ids, best
+    return given, entropy, ids, best
