@@ -14,6 +14,8 @@ other kinds of layers, fixed-size state buffers without a length that ``reset()`
   batch write there.
 * State groups are ``[layers of the group, slots + 1, *shape]``, zeroed when a slot is opened.
 * ``lengths[slot]`` is the whole state of a sequence's progress.
+* A sequence may be forked: the branches share its full pages (nothing writes those any more) and have copies of what its
+  last page holds and of its states; ``compact`` moves the held pages to the lowest numbers.
 """
 from __future__ import annotations
 
@@ -24,6 +26,7 @@ import copy
 import numpy as np
 import torch
 
+from ..kernels import ops
 from .pool import PAGE_TOKENS, CacheFull, CacheMisuse, FreeList, PageTable, pages_for
 
 
@@ -37,9 +40,11 @@ from .pool import PAGE_TOKENS, CacheFull, CacheMisuse, FreeList, PageTable, page
 # None; its ``window`` says whether pages are given back as a sequence grows); ``sync()`` (bring device copies of
 # host bookkeeping up to date, without making the host wait for the device); ``on_open(slot)``; ``nbytes()``;
 # ``attach(layer_cache, entry)``, which hangs what the part is to see on the entry's ``LayerCache`` under a field of
-# the need's choosing (the shipped ones use ``kv``, ``rows[name]`` and ``states[name]``).  Storage in pages derives
-# from ``PagedGroup``, which reads two things of its need: ``window`` (absent or None: every position is kept) and
-# ``chunked`` (absent: false; the window is a chunk of positions that only queries of the same chunk read).
+# the need's choosing (the shipped ones use ``kv``, ``rows[name]`` and ``states[name]``); and, where its sequences can be
+# forked, ``copy(src, dst, tokens)``: what the pages (or, without pages, the slots) ``src`` hold goes to ``dst``, of a page the
+# first ``tokens`` positions (None: all).  Storage in pages derives from ``PagedGroup``, which reads three things of its need:
+# ``window`` (absent or None: every position is kept), ``chunked`` (absent: false; the window is a chunk of positions that only
+# queries of the same chunk read) and ``kept`` (absent: none; the first positions, which stay behind the window).
 
 @dataclass(frozen=True)
 class KVNeed:
@@ -54,6 +59,8 @@ class KVNeed:
     value_dim: int | None = None
     # a query reads the positions of its own chunk of ``window`` positions (counted from the sequence's start) only
     chunked: bool = False
+    # a query also reads the sequence's first ``kept`` positions, however far behind its window they lie
+    kept: int = 0
 
     def make_group(self, n_entries, n_pages, n_slots, max_pages_per_slot, dtype, device):
         return KVGroup(self, n_entries, n_pages, n_slots, max_pages_per_slot, dtype, device)
@@ -90,7 +97,8 @@ class PagedGroup:
 
     def __init__(self, need, n_entries: int, n_pages: int, n_slots: int, max_pages_per_slot: int, device):
         self.need, self.n_entries, self.n_pages = need, n_entries, n_pages
-        self.table = PageTable(n_pages, n_slots, max_pages_per_slot, getattr(need, "window", None), getattr(need, "chunked", False))
+        self.table = PageTable(n_pages, n_slots, max_pages_per_slot, getattr(need, "window", None), getattr(need, "chunked", False),
+                               getattr(need, "kept", 0))
         self.pad_page = n_pages
         self.table_host = torch.full((n_slots + 1, max_pages_per_slot), self.pad_page, dtype=torch.int32)
         self.table_dev = self.table_host.to(device)
@@ -133,6 +141,12 @@ class PagedGroup:
     def on_open(self, slot: int) -> None:
         pass                                                    # nothing is read beyond a sequence's length
 
+    # storage on the host is there for its books alone (no kernel reads it): torch copies there
+    @staticmethod
+    def _copy_on_host(data: torch.Tensor, axis: int, src, dst, tokens) -> None:
+        for s, d, n in zip(src, dst, tokens or [PAGE_TOKENS] * len(src)):
+            data[:, d].narrow(axis - 1, 0, n).copy_(data[:, s].narrow(axis - 1, 0, n))
+
 
 class KVGroup(PagedGroup):
     def __init__(self, need: KVNeed, n_entries: int, n_pages: int, n_slots: int, max_pages_per_slot: int,
@@ -144,6 +158,13 @@ class KVGroup(PagedGroup):
                              device=device)
         self.v = torch.zeros((n_entries, n_pages + 1, need.value_heads or need.num_kv_heads, need.value_dim or need.head_dim,
                               PAGE_TOKENS), dtype=dtype, device=device)
+
+    def copy(self, src, dst, tokens=None) -> None:
+        if self.k.is_cuda:
+            ops.copy_pages(self.k, self.v, src, dst, tokens)
+        else:
+            self._copy_on_host(self.k, 3, src, dst, tokens)
+            self._copy_on_host(self.v, 4, src, dst, tokens)
 
     def nbytes(self) -> int:
         return (self.k.numel() + self.v.numel()) * self.k.element_size()
@@ -174,6 +195,13 @@ class RowsGroup(PagedGroup):
         dt = getattr(torch, need.dtype) if need.dtype else dtype
         self.data = torch.zeros((n_entries, n_pages + 1, PAGE_TOKENS) + tuple(need.row_shape), dtype=dt, device=device)
 
+    def copy(self, src, dst, tokens=None) -> None:
+        # whole pages: how a page's rows lie in it is the part's own affair (one keeps them transposed)
+        if self.data.is_cuda:
+            ops.copy_rows(self.data, src, dst)
+        else:
+            self._copy_on_host(self.data, 2, src, dst, None)
+
     def nbytes(self) -> int:
         return self.data.numel() * self.data.element_size()
 
@@ -197,6 +225,12 @@ class StateGroup:
 
     def on_open(self, slot: int) -> None:
         self.data[:, slot].zero_()
+
+    def copy(self, src, dst, tokens=None) -> None:
+        if self.data.is_cuda:
+            ops.copy_states(self.data, src, dst)
+        else:
+            self.data[:, list(dst)] = self.data[:, list(src)]
 
     def nbytes(self) -> int:
         return self.data.numel() * self.data.element_size()
@@ -229,8 +263,11 @@ class ModelCache:
     entry's cache: ``shares[i]`` is that entry's index)."""
 
     def __init__(self, needs: list[list], shares: list[int | None], max_tokens: int, max_seqs: int | None,
-                 max_positions: int | None, dtype: torch.dtype, device, page_slack: int = 0):
-        """``page_slack``: pages beyond those of ``max_tokens``, for a caller whose ``max_tokens`` counts the tokens that
+                 max_positions: int | None, dtype: torch.dtype, device, page_slack: int = 0, stream_tokens: int | None = None):
+        """``stream_tokens``: the longest sequence, also beyond ``max_tokens``, where every layer that keeps positions has a window and so
+        gives pages back as a sequence grows (else, and if None: what ``max_tokens`` and ``max_positions`` allow).
+
+        ``page_slack``: pages beyond those of ``max_tokens``, for a caller whose ``max_tokens`` counts the tokens that
         live sequences hold and not the part of each one's last page that stays empty: one page for each sequence that may
         be live at once.  The longest sequence stays what ``max_tokens`` allows."""
         if max_tokens <= 0:
@@ -242,6 +279,12 @@ class ModelCache:
         n_pages = pages_for(max_tokens) + int(page_slack)
         self.max_seqs = int(max_seqs) if max_seqs else min(n_pages, 1024)
         self.max_seq_tokens = min(max_positions, self.max_tokens) if max_positions else self.max_tokens
+        if stream_tokens is not None:
+            unbounded = [need for entry in needs for need in entry if hasattr(need, "window") and not need.window]
+            if stream_tokens < 1 or unbounded:
+                raise ValueError(f"sequences of up to {stream_tokens} tokens: every layer that keeps positions needs a window"
+                                 + (f", and {unbounded[0]} has none" if unbounded else ""))
+            self.max_seq_tokens = min(max_positions, int(stream_tokens)) if max_positions else int(stream_tokens)
         max_pages_per_slot = pages_for(self.max_seq_tokens)
         self.pad_slot = self.max_seqs
         self.slots = FreeList(self.max_seqs, "slot")
@@ -292,6 +335,53 @@ class ModelCache:
             g.table.release(slot)
         self.lengths[slot] = 0
         self.slots.give_back(slot)
+
+    def fork(self, slot: int, n: int = 1) -> list[int]:
+        """``n`` new sequences that begin as the one in ``slot``, with its length: its full pages are shared, what its last page
+        holds and its states are copied, on the current stream.  From then on they are sequences like any other.  Nothing is
+        taken (``CacheFull``) if not all of it fits."""
+        if not self.slots.is_held(slot):
+            raise CacheMisuse(f"slot {slot} is forked but not open")
+        if n < 1:
+            raise CacheMisuse(f"slot {slot}: {n} branches")
+        length = self.lengths[slot]
+        for g in self.groups:
+            if not hasattr(g, "copy"):
+                raise CacheMisuse(f"sequences with storage of {type(g.need).__name__} cannot be forked")
+        if n > self.slots.free_count:
+            raise CacheFull(f"{n} branches of slot {slot}; {self.slots.free_count} of {self.max_seqs} slots are free")
+        for g in self.paged_groups:
+            need = n * g.table.fork_needs(slot, length)
+            if need > g.table.pages.free_count:
+                raise CacheFull(f"{n} branches of slot {slot} need {need} more pages of {PAGE_TOKENS} tokens; "
+                                f"{g.table.pages.free_count} of {g.n_pages} are free")
+        new = self.slots.take_many(n)
+        for g in self.groups:
+            if g.table is None:
+                g.copy([slot] * n, new)
+                continue
+            copies = [c for c in (g.table.fork(slot, s, length) for s in new) if c is not None]
+            if copies:
+                g.copy([a for a, _ in copies], [b for _, b in copies], [length % PAGE_TOKENS] * len(copies))
+            g.sync()
+        for s in new:
+            self.lengths[s] = length
+        return new
+
+    def compact(self) -> int:
+        """Move the held pages of every group to its lowest numbers, on the current stream, and say how many were moved.  A step
+        that is still running or queued on that stream reads what it was launched with."""
+        moved = 0
+        for g in self.paged_groups:
+            if not hasattr(g, "copy"):
+                raise CacheMisuse(f"pages of {type(g.need).__name__} cannot be moved")
+        for g in self.paged_groups:
+            moves = g.table.compact()
+            if moves:
+                g.copy([a for a, _ in moves], [b for _, b in moves])
+                g.sync()
+            moved += len(moves)
+        return moved
 
     def check_room(self, growth: list[tuple[int, int]], in_pieces: bool = False) -> None:
         """Raise ``CacheFull`` (or ``CacheMisuse``) if the step does not fit; take nothing.  ``in_pieces``: the

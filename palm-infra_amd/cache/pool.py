@@ -3,6 +3,9 @@
 Keys and values are kept in pages of ``PAGE_TOKENS`` positions.  A sequence has a slot; the slot has a
 list of pages, as many as its length needs.  When a sequence ends its pages and its slot go back and
 are handed out again without being cleared: nothing reads a page beyond its slot's length.
+
+A full page is never written again, so sequences that begin alike may share it (a sequence and its branches): a page
+goes back when the last slot that lists it lets go of it.
 """
 from __future__ import annotations
 
@@ -63,6 +66,14 @@ class FreeList:
         # keep "lowest first": the list is small next to the work of a step
         self._free.sort(reverse=True)
 
+    def exchange(self, moves) -> None:
+        """For each (held, free): the one is given back and the other taken in its place."""
+        for held, free in moves:
+            if not self.is_held(held) or not 0 <= free < self.n or self._held[free]:
+                raise CacheMisuse(f"{self.what} {held} cannot be exchanged for {free}")
+            self._held[held], self._held[free] = False, True
+        self._free = [i for i in range(self.n - 1, -1, -1) if not self._held[i]]
+
     def check(self) -> None:
         """Every number is either free once or held; none lost, none twice."""
         free = sorted(self._free)
@@ -79,14 +90,19 @@ class PageTable:
     ``window``: if set, only the last ``window`` positions before a query are ever read, so pages
     that lie wholly below ``length - window`` are given back as the sequence grows (their entries in
     the slot's list become -1).  ``chunked``: a query only ever reads positions of its own chunk of ``window``
-    positions, so what lies wholly below the next query's chunk is given back."""
+    positions, so what lies wholly below the next query's chunk is given back.  ``kept``: the sequence's first so many
+    positions are read by every query beside its window, and their pages stay."""
 
-    def __init__(self, n_pages: int, n_slots: int, max_pages_per_slot: int, window: int | None = None, chunked: bool = False):
+    def __init__(self, n_pages: int, n_slots: int, max_pages_per_slot: int, window: int | None = None, chunked: bool = False, kept: int = 0):
         self.pages = FreeList(n_pages, "page")
         self.n_slots, self.max_pages_per_slot, self.window = n_slots, max_pages_per_slot, window
         if chunked and not window:
             raise ValueError("storage by chunks needs their size")
-        self.chunked = bool(chunked)
+        if kept < 0 or (kept and (chunked or not window)):
+            raise ValueError(f"first positions that stay ({kept}) stay behind a sliding window")
+        self.chunked, self.kept = bool(chunked), int(kept)
+        self.users = [0] * n_pages                              # slots that list the page
+        self._trimmed = [pages_for(self.kept)] * n_slots        # pages of a slot below this one were looked at already
         self.slot_pages: list[list[int]] = [[] for _ in range(n_slots)]
         self.dirty: set[int] = set()  # slots whose device copy of the list is stale
 
@@ -101,8 +117,16 @@ class PageTable:
                             f"{self.max_pages_per_slot}")
         have = self.slot_pages[slot]
         if need > len(have):
-            have.extend(self.pages.take_many(need - len(have)))
+            new = self.pages.take_many(need - len(have))
+            for p in new:
+                self.users[p] = 1
+            have.extend(new)
             self.dirty.add(slot)
+
+    def _let_go(self, page: int) -> None:
+        self.users[page] -= 1
+        if self.users[page] == 0:
+            self.pages.give_back(page)
 
     def trim(self, slot: int, length: int) -> None:
         """After a step: give back pages no later query can read (windowed groups only)."""
@@ -111,23 +135,71 @@ class PageTable:
         # the next query sits at position `length`
         first_needed = length - length % self.window if self.chunked else max(0, length - self.window + 1)
         have = self.slot_pages[slot]
-        for j in range(min(first_needed // PAGE_TOKENS, len(have))):
+        end = min(first_needed // PAGE_TOKENS, len(have))
+        for j in range(self._trimmed[slot], end):
             if have[j] >= 0:
-                self.pages.give_back(have[j])
+                self._let_go(have[j])
                 have[j] = -1
                 self.dirty.add(slot)
+        self._trimmed[slot] = max(self._trimmed[slot], end)
 
     def release(self, slot: int) -> None:
         for p in self.slot_pages[slot]:
             if p >= 0:
-                self.pages.give_back(p)
+                self._let_go(p)
         self.slot_pages[slot] = []
+        self._trimmed[slot] = pages_for(self.kept)
         self.dirty.add(slot)
+
+    def fork_needs(self, slot: int, length: int) -> int:
+        """Pages that a branch of the slot takes of its own: one, if its last page is not full."""
+        last = length // PAGE_TOKENS
+        return int(length % PAGE_TOKENS != 0 and last < len(self.slot_pages[slot]) and self.slot_pages[slot][last] >= 0)
+
+    def fork(self, slot: int, new: int, length: int):
+        """The empty slot ``new`` lists the pages of ``slot`` up to ``length``; the last one, if it is not full, a page of its own.
+        Returns (page, its copy) then, which is to be made, else None."""
+        pages, copy = self.slot_pages[slot][:pages_for(length)], None
+        if self.fork_needs(slot, length):
+            own = self.pages.take()
+            copy, pages[-1] = (pages[-1], own), own
+            self.users[own] = 0                                 # (counted below like the others)
+        for p in pages:
+            if p >= 0:
+                self.users[p] += 1
+        self.slot_pages[new] = pages
+        self._trimmed[new] = self._trimmed[slot]
+        self.dirty.add(new)
+        return copy
+
+    def compact(self) -> list[tuple[int, int]]:
+        """The held pages become the pages numbered lowest, with as few moves as it takes: (page, its new number) each, whose contents
+        are to be moved.  No page is both read and written by them."""
+        n = self.pages.held_count
+        moves = list(zip([p for p in range(n, self.pages.n) if self.pages.is_held(p)], [p for p in range(n) if not self.pages.is_held(p)]))
+        if not moves:
+            return moves
+        self.pages.exchange(moves)
+        for old, new in moves:
+            self.users[new], self.users[old] = self.users[old], 0
+        where = dict(moves)
+        for slot, pages in enumerate(self.slot_pages):
+            if any(p in where for p in pages):
+                self.slot_pages[slot] = [where.get(p, p) for p in pages]
+                self.dirty.add(slot)
+        return moves
 
     def check(self) -> None:
         self.pages.check()
-        held = [p for pages in self.slot_pages for p in pages if p >= 0]
-        if len(set(held)) != len(held):
-            raise CacheMisuse("a page is in two slots")
-        if len(held) != self.pages.held_count:
-            raise CacheMisuse(f"{self.pages.held_count} pages are held but slots list {len(held)}")
+        listed: dict[int, int] = {}
+        for pages in self.slot_pages:
+            own = [p for p in pages if p >= 0]
+            if len(set(own)) != len(own):
+                raise CacheMisuse("a slot lists a page twice")
+            for p in own:
+                listed[p] = listed.get(p, 0) + 1
+        for p, n in listed.items():
+            if self.users[p] != n:
+                raise CacheMisuse(f"page {p} is in {n} slots and counted for {self.users[p]}")
+        if len(listed) != self.pages.held_count or sum(self.users) != sum(listed.values()):
+            raise CacheMisuse(f"{self.pages.held_count} pages are held but slots list {len(listed)}")
