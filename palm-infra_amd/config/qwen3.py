@@ -8,7 +8,7 @@ Keys and defaults follow the reference's reader (models/qwen3.py:175-184): ``hid
 """
 from __future__ import annotations
 
-from dataclasses import dataclass, asdict
+from dataclasses import dataclass, asdict, replace
 
 from .registry import ConfigError, register_architecture
 from .spec import LayerCall, ModelSpec, PartSpec, joined, tensor
@@ -42,6 +42,18 @@ class Qwen3Config:
     # (models/qwen3.py:89-95, 162-165)
     tie_word_embeddings: bool | None = None
     eos_token_ids: tuple[int, ...] = ()
+    # how a run reads the cache, not a property of the checkpoint (``with_window``): each query sees the last `window` positions
+    # and the sequence's first `kept` ones
+    window: int | None = None
+    kept: int = 0
+
+    def with_window(self, window: int, kept: int = 0) -> "Qwen3Config":
+        """The same model with attention over the last ``window`` positions and the first ``kept`` ones of a sequence: streams without an
+        end, at a bounded cost a token.  (The first positions draw much of the weight in models trained without a window, and
+        a window that loses them loses the model.)"""
+        cfg = replace(self, window=int(window), kept=int(kept))
+        cfg.validate()
+        return cfg
 
     @classmethod
     def from_dict(cls, raw: dict) -> "Qwen3Config":
@@ -92,12 +104,16 @@ class Qwen3Config:
             raise ConfigError(f"config.json: head_dim = {self.head_dim} must be even (rotation works on pairs)")
         if not self.rms_norm_eps > 0.0:
             raise ConfigError(f"config.json: rms_norm_eps = {self.rms_norm_eps} must be positive")
+        if self.kept < 0 or (self.window is None and self.kept) or (self.window is not None and self.window < 1):
+            raise ConfigError(f"attention over the last {self.window} positions and the first {self.kept}: a window has at least one, and "
+                              "first positions stand behind a window")
         if not self.rope_theta > 0.0:
             raise ConfigError(f"config.json: rope_theta = {self.rope_theta} must be positive")
 
     def to_dict(self) -> dict:
         d = asdict(self)
         eos = d.pop("eos_token_ids")
+        d.pop("window"), d.pop("kept")                  # of a run, not of the model's folder
         if d["tie_word_embeddings"] is None:
             d.pop("tie_word_embeddings")
         if eos:
@@ -133,7 +149,7 @@ class Qwen3Config:
             mixer = PartSpec(
                 "mixer", "attention",
                 {"hidden_size": H, "num_heads": nh, "num_kv_heads": nkv, "head_dim": hd,
-                 "scale": hd ** -0.5, "window": None},
+                 "scale": hd ** -0.5, "window": self.window, "kept": self.kept},
                 {"qkv": joined((a + "q_proj.weight", a + "k_proj.weight", a + "v_proj.weight"),
                                ((nh * hd, H), (nkv * hd, H), (nkv * hd, H))),
                  "out": tensor(a + "o_proj.weight", (H, nh * hd))},

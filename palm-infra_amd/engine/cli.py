@@ -7,7 +7,7 @@ Options keep the reference's names and meanings where it has them (examples/cli_
 ``--presence-penalty``, ``--frequency-penalty``, ``--seed``, ``--output kv|human``, ``--profile``,
 ``--trace``.  ``--package`` names a
 model folder here (``--model`` is the same): there is no packaging step.  New: ``--dtype``, ``--batch``, ``--stop-token-ids``, ``--ignore-eos``,
-``--prompt-ids``, ``--prompt-lengths``, ``--random-config`` (random weights from a config.json or a named size),
+``--prompt-ids``, ``--prompt-lengths``, ``--window``, ``--kept``, ``--stream-tokens``, ``--answers``, ``--logprobs``, ``--score``, ``--random-config`` (random weights from a config.json or a named size),
 ``--allow-extra-tensors`` (tensors the model does not name are listed and left alone instead of refused).  Options of
 the reference that select a backend, offload, vision or speculation have no meaning here and are
 refused by the parser.
@@ -48,6 +48,13 @@ def build_parser(prog: str, bench: bool) -> argparse.ArgumentParser:
                                              "eos_token_id of config.json and generation_config.json)")
     ap.add_argument("--ignore-eos", action="store_true", help="never stop before --max-new-tokens")
     ap.add_argument("--n-ctx", type=int, default=16384, help="tokens the cache holds for all live sequences together")
+    ap.add_argument("--window", type=int, help="every query sees the last so many positions only (designs without windows of their own)")
+    ap.add_argument("--kept", type=int, default=0, help="and the sequence's first so many")
+    ap.add_argument("--stream-tokens", type=int, help="with --window: the longest sequence, also beyond --n-ctx")
+    ap.add_argument("--answers", type=int, default=1, help="answers to each prompt (the prompt runs once)")
+    ap.add_argument("--logprobs", type=int, metavar="N", help="print each token's log probability and its N likeliest alternatives")
+    ap.add_argument("--score", action="store_true", help="generate nothing: print the log probabilities of the prompts' own tokens "
+                                                         "(with --logprobs N each one's alternatives too)")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
     ap.add_argument("--warmup", type=int, default=1, help="warm-up runs before the timed run (bench)")
     ap.add_argument("--temperature", type=float, default=0.6, help="0 = greedy")
@@ -120,10 +127,11 @@ def collect_prompts(args, tokenizer, vocab_size: int):
 
 def make_engine(args):
     from .engine import Engine
+    options = dict(dtype=args.dtype, max_tokens=args.n_ctx, window=args.window, kept=args.kept, stream_tokens=args.stream_tokens)
     if args.model:
-        return Engine.from_dir(args.model, dtype=args.dtype, max_tokens=args.n_ctx, strict_weights=not args.allow_extra_tensors)
+        return Engine.from_dir(args.model, strict_weights=not args.allow_extra_tensors, **options)
     if args.random_config:
-        return Engine.from_config(config_source(args.random_config), seed=args.seed, dtype=args.dtype, max_tokens=args.n_ctx)
+        return Engine.from_config(config_source(args.random_config), seed=args.seed, **options)
     raise SystemExit("--package <model folder> (or --random-config <config.json>) is required")
 
 
@@ -150,6 +158,15 @@ def print_human(load_ms, m, total_ms, n_requests, finish) -> None:
     print(f"  prompt    {m.prompt_tokens:10d} tokens   prefill {m.ttft_ms:10.1f} ms   {m.prefill_tps:12.1f} tok/s")
     print(f"  decoded   {m.decode_tokens:10d} tokens   decode  {m.total_ms - m.ttft_ms:10.1f} ms   {m.decode_tps:12.1f} tok/s")
     print(f"  tpot      {m.tpot_ms:10.2f} ms      total   {total_ms:10.1f} ms")
+
+
+def scores_text(token_ids, scores, tokenizer, offset: int = 0) -> str:
+    """A line a token: its log probability, the entropy there, and the alternatives."""
+    name = (lambda t: repr(tokenizer.decode([t]))) if tokenizer else str
+    lines = [f"total {scores.total:.4f} of {len(scores.logprobs)} tokens"]
+    for tok, lp, entropy, others in zip(token_ids[offset:], scores.logprobs, scores.entropies, scores.alternatives):
+        lines.append(f"  {name(tok)}  {lp:.4f}  entropy {entropy:.4f}" + "".join(f"  {name(t)} {p:.4f}" for t, p in others))
+    return "\n".join(lines)
 
 
 def run(argv, bench: bool) -> int:
@@ -185,6 +202,17 @@ def run(argv, bench: bool) -> int:
         except ValueError:
             print(f"{ap.prog}: --stop-token-ids takes comma-separated whole numbers", file=sys.stderr)
             return 1
+    if args.score:
+        if bench or not prompts:
+            print(f"{ap.prog}: --score scores the prompts given to palm_chat", file=sys.stderr)
+            return 1
+        try:
+            for i, (ids, scores) in enumerate(zip(prompts, engine.score(prompts, args.logprobs or 0))):
+                print(f"[{i}] {scores_text(ids, scores, tokenizer, 1)}")
+        except (ValueError, CacheFull) as e:
+            print(f"{ap.prog}: {type(e).__name__}: {e}", file=sys.stderr)
+            return 1
+        return 0
     if not bench and not prompts:
         return repl(engine, sampling, tokenizer, args, stop_ids)
     if not prompts:
@@ -202,7 +230,7 @@ def _generate_and_report(ap, args, engine, sampling, tokenizer, prompts, stop_id
     if bench:
         for _ in range(max(0, args.warmup)):
             engine.generate(prompts, sampling, args.max_new_tokens, stop_token_ids=stop_ids, ignore_eos=no_stop,
-                            max_batch=max(1, args.batch))
+                            max_batch=max(1, args.batch, args.answers), answers=args.answers, logprobs=args.logprobs)
     recorder = None
     if args.profile or args.trace:
         # after the warm-up, so that what is timed has loaded its libraries and the tables show the timed run alone
@@ -211,13 +239,14 @@ def _generate_and_report(ap, args, engine, sampling, tokenizer, prompts, stop_id
     t1 = time.perf_counter()
 
     def stream(i, tok):
-        if not bench and len(prompts) == 1:
+        if not bench and len(prompts) == 1 and args.answers == 1:
             piece = tokenizer.decode([tok]) if tokenizer else f"{tok} "
             print(piece, end="", flush=True)
 
     try:
         results, metrics = engine.generate(prompts, sampling, args.max_new_tokens, stop_token_ids=stop_ids,
-                                           ignore_eos=no_stop, max_batch=max(1, args.batch), on_token=stream)
+                                           ignore_eos=no_stop, max_batch=max(1, args.batch, args.answers), on_token=stream,
+                                           answers=args.answers, logprobs=args.logprobs)
     finally:
         if recorder is not None:
             recorder.remove()
@@ -225,17 +254,20 @@ def _generate_and_report(ap, args, engine, sampling, tokenizer, prompts, stop_id
     if args.trace:
         recorder.write_chrome_trace(args.trace)
     if bench:
-        (print_human if args.output == "human" else print_kv)(load_ms, metrics, total_ms, len(prompts),
+        (print_human if args.output == "human" else print_kv)(load_ms, metrics, total_ms, len(results),
                                                                [r.finish_reason for r in results])
         if args.profile:
             print(recorder.format())
         return 0
-    if len(prompts) == 1:
+    if len(results) == 1:
         print()
     else:
         for i, r in enumerate(results):
             text = tokenizer.decode(r.token_ids) if tokenizer else " ".join(map(str, r.token_ids))
             print(f"[{i}] {text}")
+    if args.logprobs is not None:
+        for i, r in enumerate(results):
+            print(f"[{i}] {scores_text(r.token_ids, r.scores, tokenizer)}")
     if args.profile:
         print(recorder.format(), file=sys.stderr)
     print(f"ttft {metrics.ttft_ms:.1f} ms | tpot {metrics.tpot_ms:.2f} ms | prefill {metrics.prefill_tps:.1f} tok/s | "

@@ -15,9 +15,9 @@ from pathlib import Path
 import numpy as np
 import torch
 
-from ..cache import ModelCache
+from ..cache import PAGE_TOKENS, ModelCache, pages_for
 from ..config import config_from_dict, config_from_dir
-from ..kernels import profile
+from ..kernels import ops, profile
 from ..parts import context_ints, make_context
 from ..weights import ModelFiles, load_weights, random_weights
 from .model import DecoderModel
@@ -60,7 +60,7 @@ class Engine:
     takes_fed = True             # step(entries, fed=..) takes tokens that are still on the device
 
     def __init__(self, config, spec, weights, dtype: torch.dtype, max_tokens: int, max_seqs: int | None = None,
-                 device="cuda:0", graphs: bool = True, max_step_tokens: int = 32768, page_slack: int = 0):
+                 device="cuda:0", graphs: bool = True, max_step_tokens: int = 32768, page_slack: int = 0, stream_tokens: int | None = None):
         self.device = torch.device(device)
         if self.device.type != "cuda":
             raise RuntimeError(f"the engine runs on a GPU; device {device!r} was asked for and there is no CPU path")
@@ -70,7 +70,9 @@ class Engine:
         self.config, self.spec, self.dtype = config, spec, dtype
         self.model = DecoderModel(spec, weights, dtype, self.device)
         needs, shares = self.model.cache_plan()
-        self.cache = ModelCache(needs, shares, max_tokens, max_seqs, spec.max_positions, dtype, self.device, page_slack=page_slack)
+        self.cache = ModelCache(needs, shares, max_tokens, max_seqs, spec.max_positions, dtype, self.device, page_slack=page_slack,
+                                stream_tokens=stream_tokens)
+        self.streams = stream_tokens is not None          # sequences may be longer than the cache
         self.vocab_size = spec.vocab_size
         self.graphs_enabled = bool(graphs)
         self._decode_graphs: dict = {}            # (batch bucket, length bucket, parts' choices) -> recorded step, least recently used first
@@ -89,29 +91,43 @@ class Engine:
         self.max_step_tokens = int(max_step_tokens)
 
     # ---- construction ------------------------------------------------------------------------
+    @staticmethod
+    def _windowed(config, window: int | None, kept: int):
+        if window is None:
+            if kept:
+                raise ValueError(f"kept = {kept} first positions stand behind a window, and none is given")
+            return config
+        if not hasattr(config, "with_window"):
+            raise ValueError(f"{type(config).__name__}: the windows of this design's layers are part of the model; window and kept are for designs without")
+        return config.with_window(window, kept)
+
     @classmethod
     def from_dir(cls, model_dir, dtype="bfloat16", max_tokens: int | None = None, device="cuda:0",
-                 strict_weights: bool = True, **options):
+                 strict_weights: bool = True, window: int | None = None, kept: int = 0, **options):
         """A folder with config.json and safetensors; the model class is chosen by config.json.  ``strict_weights``
         false: tensors of the checkpoint that the model does not name are listed on standard error and left alone
-        instead of refused."""
+        instead of refused.  ``window``, ``kept``: every query sees the last ``window`` positions and the sequence's first
+        ``kept`` ones (designs whose layers have no windows of their own); with ``stream_tokens`` sequences may then be that
+        long, whatever ``max_tokens``: the cache holds a window of each."""
         dt = resolve_dtype(dtype)
         model_dir = Path(model_dir)
         config = config_from_dir(model_dir)
         files = ModelFiles(model_dir)
         if hasattr(config, "with_tensor_shapes"):       # an architecture some of whose sizes only the tensors' shapes give
             config = config.with_tensor_shapes({name: files.shape(name) for name in files.names()})
+        config = cls._windowed(config, window, kept)
         spec = config.spec(files.names())
         weights = load_weights(spec, files, dt, device, strict=strict_weights)
         return cls(config, spec, weights, dt, max_tokens or 16384, device=device, **options)
 
     @classmethod
     def from_config(cls, config, seed: int = 0, dtype="bfloat16", max_tokens: int | None = None, device="cuda:0",
-                    **options):
-        """Random weights made on the device (no folder is written)."""
+                    window: int | None = None, kept: int = 0, **options):
+        """Random weights made on the device (no folder is written).  ``window``, ``kept``: see ``from_dir``."""
         dt = resolve_dtype(dtype)
         if isinstance(config, dict):
             config = config_from_dict(config)
+        config = cls._windowed(config, window, kept)
         spec = config.spec()
         weights = random_weights(spec, seed, dt, device)
         return cls(config, spec, weights, dt, max_tokens or 16384, device=device, **options)
@@ -127,6 +143,25 @@ class Engine:
 
     def length(self, slot: int) -> int:
         return self.cache.lengths[slot]
+
+    def fork(self, slot: int, n: int = 1) -> list[int]:
+        """``n`` new sequences that begin as the one in ``slot`` (see ``ModelCache.fork``)."""
+        return self.cache.fork(slot, n)
+
+    def compact(self) -> int:
+        """Move the pages that sequences hold together; how many were moved (see ``ModelCache.compact``)."""
+        return self.cache.compact()
+
+    def held_tokens(self, length: int) -> int:
+        """Room in the cache, in tokens, that a sequence takes at most while it grows to ``length``: all of it, or where every layer has a
+        window the window, the first positions that stay, and the piece of a prompt that goes through between two steps."""
+        most = 0
+        for g in self.cache.paged_groups:
+            pages = pages_for(length)
+            if g.table.window:
+                pages = min(pages, pages_for(g.table.window + self.step_tokens_least) + 1 + pages_for(g.table.kept))
+            most = max(most, pages)
+        return (most or pages_for(length)) * PAGE_TOKENS
 
     # ---- the step ----------------------------------------------------------------------------
     @staticmethod
@@ -416,9 +451,11 @@ class Engine:
 
     # ---- generation --------------------------------------------------------------------------
     def generate(self, prompts, sampling=None, max_new_tokens: int = 2048, stop_token_ids=None, ignore_eos: bool = False,
-                 max_batch: int = 64, on_token=None, **sampling_options):
+                 max_batch: int = 64, on_token=None, answers: int = 1, logprobs: int | None = None, **sampling_options):
         """Token ids in, token ids out: ``prompts`` is a list of lists of ids; returns (results, metrics),
-        the results in the order of the prompts.  ``sampling`` is a ``SamplingParams``; its fields may also be
+        the results in the order of the prompts.  ``answers``: so many results for each prompt, one behind the other; the prompt runs once
+        and its sequence is forked.  ``logprobs``: the results tell how likely their tokens were, by the model's logits as they are (before
+        temperature, cuts and penalties), and so many alternatives of each (0 to 64).  ``sampling`` is a ``SamplingParams``; its fields may also be
         given by name (``temperature=0.7, seed=1``) and then replace those of ``sampling`` or of the defaults.
         ``stop_token_ids`` defaults to the model's ``eos_token_id``; ``ignore_eos`` switches stopping off, as
         the reference's benchmark does (examples/bench.cpp:583)."""
@@ -438,7 +475,37 @@ class Engine:
         else:
             stop = self.spec.stop_token_ids if stop_token_ids is None else stop_token_ids
         return generate(self, sampler, prompts, max_new_tokens=max_new_tokens, stop_token_ids=stop, max_batch=max_batch,
-                        on_token=on_token, sync=torch.cuda.synchronize)
+                        on_token=on_token, sync=torch.cuda.synchronize, answers=answers, logprobs=logprobs,
+                        held_tokens=self.held_tokens if self.streams else None)
+
+    SCORED_ROWS = 2048           # positions whose logits are held at once (float32: 1.2 GB for a vocabulary of 151,936)
+
+    def score(self, sequences, alternatives: int = 0) -> list:
+        """How likely each token of given sequences (lists of ids) is behind those before it: a ``TokenScores`` for each, with what is said of the
+        second token and those behind it, and so many alternatives of each (0 to 64).  The sequences run one after the other, in
+        pieces, through slots of their own."""
+        from .generate import TokenScores
+        if not 0 <= int(alternatives) <= ops.LOGPROBS_MOST:
+            raise ValueError(f"alternatives = {alternatives}: 0 to {ops.LOGPROBS_MOST}")
+        out = []
+        for tokens in sequences:
+            tokens = [int(t) for t in tokens]
+            if not tokens:
+                raise ValueError("a sequence to be scored has at least one token")
+            scores = TokenScores()
+            slot = self.open()
+            try:
+                for lo in range(0, len(tokens) - 1, self.SCORED_ROWS):
+                    piece = tokens[lo:min(lo + self.SCORED_ROWS, len(tokens) - 1)]
+                    logits = self.step([StepEntry(slot, piece, list(range(len(piece))))])
+                    following = torch.tensor(tokens[lo + 1:lo + 1 + len(piece)], dtype=torch.int32)
+                    if int(following[-1]) < 0 or int(following[-1]) >= self.vocab_size:
+                        raise StepError(f"token id {int(following[-1])} lies outside the vocabulary of {self.vocab_size}")
+                    scores.take(*ops.token_logprobs(logits, following.to(self.device), int(alternatives)))
+            finally:
+                self.close(slot)
+            out.append(scores)
+        return out
 
     def conversation(self, sampling=None, stop_token_ids=None, ignore_eos: bool = False):
         """A sequence that stays in the cache from turn to turn: ``say(new tokens)`` feeds only what is new and

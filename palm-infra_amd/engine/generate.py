@@ -50,6 +50,46 @@ class TokenFetch:
 
 
 @dataclass
+class TokenScores:
+    """Of a run of tokens: the log probability of each, the entropy of the distribution that it was one of (natural logarithms), and the
+    likeliest tokens there with their log probabilities, if they were asked for."""
+    logprobs: list = field(default_factory=list)
+    entropies: list = field(default_factory=list)
+    alternatives: list = field(default_factory=list)      # for each token [(id, log probability), ..], the likeliest first
+
+    @property
+    def total(self) -> float:
+        return sum(self.logprobs)
+
+    def take(self, given, entropy, ids, best) -> None:
+        """What ``ops.token_logprobs`` returned of the tokens that follow."""
+        self.logprobs += given.tolist()
+        self.entropies += entropy.tolist()
+        self.alternatives += [list(zip(i, b)) for i, b in zip(ids.tolist(), best.tolist())]
+
+
+class DrawFetch:
+    """A step's drawn tokens, and what is told of them if it was asked for, on their way to the host."""
+
+    def __init__(self, ids, logits, logprobs, scorer):
+        self.ids = ids
+        self.fetched = TokenFetch(ids)
+        self.scores = None if logprobs is None else [TokenFetch(t) for t in scorer(logits, ids, logprobs)]
+        self.told = None
+
+    def tokens(self) -> list:
+        return self.fetched.tokens()
+
+    def score(self, row: int, scores: TokenScores) -> None:
+        if self.scores is not None:
+            self.told = self.told or [s.tokens() for s in self.scores]
+            given, entropy, ids, best = self.told
+            scores.logprobs.append(given[row])
+            scores.entropies.append(entropy[row])
+            scores.alternatives.append(list(zip(ids[row], best[row])))
+
+
+@dataclass
 class GenerationResult:
     """Of one request.  ``finish_reason``: "stop" (a stop token came, and is the last token), "length"
     (max_new_tokens), "context" (the sequence filled the longest context the cache takes)."""
@@ -58,6 +98,7 @@ class GenerationResult:
     finish_reason: str = ""
     prefill_ms: float = 0.0
     decode_ms: float = 0.0
+    scores: TokenScores | None = None      # of the tokens in ``token_ids``, if they were asked for
 
     @property
     def hit_eos(self) -> bool:
@@ -95,12 +136,17 @@ class RequestTooLong(ValueError):
     pass
 
 
-def plan_batches(prompt_lengths, max_new_tokens: int, max_batch: int, cache_tokens: int, max_seq_tokens: int):
+def plan_batches(prompt_lengths, max_new_tokens: int, max_batch: int, cache_tokens: int, max_seq_tokens: int, answers: int = 1, held_tokens=None):
     """Which requests run together: in the order given, as many as ``max_batch`` allows and as the cache
-    can hold when every sequence of the batch grows to its full length (pages of PAGE_TOKENS each).
-    Returns lists of request indices."""
+    can hold when every sequence of the batch grows to its full length (pages of PAGE_TOKENS each;
+    ``held_tokens(length)``: what it takes then, if it is less).  Each request is ``answers`` sequences (that they share their
+    prompt's pages is not counted on).  Returns lists of request indices."""
     if max_batch < 1:
         raise ValueError("max_batch must be at least 1")
+    if answers < 1:
+        raise ValueError("answers must be at least 1")
+    if answers > max_batch:
+        raise RequestTooLong(f"{answers} answers to a prompt are more sequences than the {max_batch} that run together")
     batches, current, held = [], [], 0
     for i, n in enumerate(prompt_lengths):
         if n < 1:
@@ -109,10 +155,10 @@ def plan_batches(prompt_lengths, max_new_tokens: int, max_batch: int, cache_toke
             raise RequestTooLong(f"request {i}: a prompt of {n} tokens exceeds the longest sequence the cache takes "
                                  f"({max_seq_tokens})")
         full = min(n + max_new_tokens, max_seq_tokens)
-        need = pages_for(full) * PAGE_TOKENS
+        need = answers * (held_tokens(full) if held_tokens else pages_for(full) * PAGE_TOKENS)
         if need > cache_tokens:
-            raise RequestTooLong(f"request {i}: {full} tokens do not fit a cache of {cache_tokens}")
-        if current and (len(current) >= max_batch or held + need > cache_tokens):
+            raise RequestTooLong(f"request {i}: {full} tokens{f' in {answers} sequences' if answers > 1 else ''} do not fit a cache of {cache_tokens}")
+        if current and ((len(current) + 1) * answers > max_batch or held + need > cache_tokens):
             batches.append(current)
             current, held = [], 0
         current.append(i)
@@ -123,39 +169,56 @@ def plan_batches(prompt_lengths, max_new_tokens: int, max_batch: int, cache_toke
 
 
 def generate(engine, sampler, prompts, max_new_tokens: int = 2048, stop_token_ids=(), max_batch: int = 64,
-             on_token=None, timer=time.perf_counter, sync=None):
-    """Generate for every prompt (a list of token ids); results come in the order of the prompts.
+             on_token=None, timer=time.perf_counter, sync=None, answers: int = 1, logprobs: int | None = None, scorer=None,
+             held_tokens=None):
+    """Generate for every prompt (a list of token ids); results come in the order of the prompts, ``answers`` of each one behind
+    the other (a prompt runs once; ``engine.fork(slot, n)`` makes the other sequences).  ``logprobs``: the results' ``scores`` tell how
+    likely their tokens were and so many alternatives of each; ``scorer(logits, ids, alternatives)`` finds out (``ops.token_logprobs``).
 
     ``engine``: ``open() -> slot``, ``close(slot)``, ``step(entries) -> logits [rows, vocab]``,
     ``cache.max_tokens``, ``cache.max_seq_tokens``.  ``sampler``: ``sample(logits, states) -> ids`` (anything
     with ``.tolist()``).  ``on_token(request index, token id)`` is called for every token as it comes.
-    ``sync()`` waits for the device before a time is taken.  Returns (results, metrics).
+    ``held_tokens``: see ``plan_batches``.  ``sync()`` waits for the device before a time is taken.  Returns (results, metrics).
     """
     if max_new_tokens < 1:
         raise ValueError("max_new_tokens must be >= 1")
+    if logprobs is not None:
+        from ..kernels import ops
+        scorer = scorer or ops.token_logprobs
+        if not 0 <= logprobs <= ops.LOGPROBS_MOST:
+            raise ValueError(f"logprobs = {logprobs}: 0 to {ops.LOGPROBS_MOST} alternatives of each token")
     prompts = [list(map(int, p)) for p in prompts]
     stop = set(int(t) for t in stop_token_ids)
     max_seq = engine.cache.max_seq_tokens
-    results = [GenerationResult(prompt_tokens=len(p)) for p in prompts]
+    asked = prompts
+    prompts = [p for p in asked for _ in range(max(answers, 1))]         # of each result
+    results = [GenerationResult(prompt_tokens=len(p), scores=None if logprobs is None else TokenScores()) for p in prompts]
     # a batch holds no more sequences than the cache has slots for
     max_batch = min(max_batch, getattr(engine.cache, "max_seqs", max_batch))
-    batches = plan_batches([len(p) for p in prompts], max_new_tokens, max_batch, engine.cache.max_tokens, max_seq)
+    batches = plan_batches([len(p) for p in asked], max_new_tokens, max_batch, engine.cache.max_tokens, max_seq, answers, held_tokens)
     sync = sync or (lambda: None)
     total_prefill = total_decode = 0.0
 
-    for batch in batches:
+    for requests in batches:
+        batch = [r * answers + j for r in requests for j in range(answers)]
         slots = {}
         states = {i: SequenceSampling(stream=i) for i in batch}
         try:
-            for i in batch:                  # one by one inside the try: if a slot cannot be had, those taken go back
+            firsts = batch[::answers]
+            for i in firsts:                 # one by one inside the try: if a slot cannot be had, those taken go back
                 slots[i] = engine.open()
             # ---- all prompts in one step; it yields each request's first token ----
             sync()
             t0 = timer()
-            logits = engine.step([StepEntry(slots[i], prompts[i], [len(prompts[i]) - 1]) for i in batch])
+            logits = engine.step([StepEntry(slots[i], prompts[i], [len(prompts[i]) - 1]) for i in firsts])
+            if answers > 1:
+                for i in firsts:
+                    slots.update(zip(range(i + 1, i + answers), engine.fork(slots[i], answers - 1)))
+                logits = logits.repeat_interleave(answers, dim=0)
             for i in batch:
                 states[i].accept(prompts[i])
-            tokens = sampler.sample(logits, [states[i] for i in batch]).tolist()
+            drawn = DrawFetch(sampler.sample(logits, [states[i] for i in batch]), logits, logprobs, scorer)
+            tokens = drawn.tokens()
             sync()
             prefill_ms = (timer() - t0) * 1000.0
             total_prefill += prefill_ms
@@ -179,8 +242,9 @@ def generate(engine, sampler, prompts, max_new_tokens: int = 2048, stop_token_id
                 return True
 
             live = []
-            for i, tok in zip(batch, tokens):
+            for row, (i, tok) in enumerate(zip(batch, tokens)):
                 results[i].prefill_ms = prefill_ms
+                drawn.score(row, results[i].scores)
                 if take(i, int(tok)):
                     live.append(i)
 
@@ -194,7 +258,7 @@ def generate(engine, sampler, prompts, max_new_tokens: int = 2048, stop_token_id
                 logits = engine.step([StepEntry(slots[i], [results[i].token_ids[-1]], [0]) for i in live])
                 for i in live:
                     states[i].accept([results[i].token_ids[-1]])
-                pending = TokenFetch(sampler.sample(logits, [states[i] for i in live]))
+                pending = DrawFetch(sampler.sample(logits, [states[i] for i in live]), logits, logprobs, scorer)
                 order = [(i, row) for row, i in enumerate(live)]        # whose newest token is which row of `pending`
                 while order:
                     ahead = [(i, row) for i, row in order if goes_on(i, len(results[i].token_ids) + 1)]
@@ -202,11 +266,12 @@ def generate(engine, sampler, prompts, max_new_tokens: int = 2048, stop_token_id
                     if ahead:
                         logits = engine.step([StepEntry(slots[i], [0], [0]) for i, _ in ahead],
                                              fed=FedTokens(pending.ids, [row for _, row in ahead]))
-                        following = TokenFetch(sampler.sample(logits, [states[i] for i, _ in ahead]))
+                        following = DrawFetch(sampler.sample(logits, [states[i] for i, _ in ahead]), logits, logprobs, scorer)
                     toks = pending.tokens()                              # the device runs the next step meanwhile
                     alive = set()
                     for i, row in order:
                         states[i].accept([int(toks[row])])
+                        pending.score(row, results[i].scores)
                         if take(i, int(toks[row])):
                             alive.add(i)
                     # a sequence that ended on a stop token was stepped once more: its draw is dropped with it
@@ -218,8 +283,10 @@ def generate(engine, sampler, prompts, max_new_tokens: int = 2048, stop_token_id
                 logits = engine.step([StepEntry(slots[i], [last[i]], [0]) for i in live])
                 for i in live:
                     states[i].accept([last[i]])
-                tokens = sampler.sample(logits, [states[i] for i in live]).tolist()
-                live = [i for i, tok in zip(live, tokens) if take(i, int(tok))]
+                drawn = DrawFetch(sampler.sample(logits, [states[i] for i in live]), logits, logprobs, scorer)
+                for row, i in enumerate(live):
+                    drawn.score(row, results[i].scores)
+                live = [i for i, tok in zip(live, drawn.tokens()) if take(i, int(tok))]
             sync()
             decode_ms = (timer() - t1) * 1000.0
             total_decode += decode_ms

@@ -976,14 +976,16 @@ def decode_pages_pays(lengths, nh: int, nkv: int, hd: int, max_keys: int) -> boo
 def attention_decode_fused(qkv, k_cache, v_cache, block_table, seq_slot, seq_start, nh: int, nkv: int, hd: int, scale: float,
                            window: int | None, n_slices: int, *, q_norm_w=None, k_norm_w=None, eps: float = 0.0, cos=None,
                            sin=None, rotary_dim: int = 0, pairing: int = 0, write_cache: bool = True,
-                           work: torch.Tensor | None = None, pages: bool = False, arrivals: torch.Tensor | None = None) -> torch.Tensor:
+                           work: torch.Tensor | None = None, pages: bool = False, arrivals: torch.Tensor | None = None, kept: int = 0) -> torch.Tensor:
     """A decode step's attention from the joined projection's rows: qk_norm_rope_store and attention_decode in one
     launch.  qkv is [B, (nh + 2 nkv) hd] bfloat16 or float32 planes [P, B, (nh + 2 nkv) hd]; sequence b's token is
     row b, at position seq_start[b]; cos, sin are [B, hd / 2] rows of those positions.  Returns [B, nh hd] bfloat16.
 
     ``pages``: by the kernel whose work is cut by pages (attention_decode_pages.h), whatever ``n_slices``, where ``decode_pages_serves``.
     ``arrivals``: its counters, int32 [B * nh] or more, zero before the call and left zero by it, not shared by calls that may overlap in
-    time (made here if None)."""
+    time (made here if None).
+
+    ``kept``: the sequence's first so many positions are seen behind the window (``attention_kept``); by slices only."""
     what = "attention_decode_fused"
     _dev(what, qkv, k_cache, v_cache, block_table, seq_slot, seq_start, q_norm_w, k_norm_w, cos, sin)
     _i32(what, block_table, seq_slot, seq_start)
@@ -1007,6 +1009,8 @@ def attention_decode_fused(qkv, k_cache, v_cache, block_table, seq_slot, seq_sta
         if not (tab is None or (tab.dtype == F32 and tab.shape == (B, hd // 2) and tab.is_contiguous() and rotary_dim == hd)):
             raise KernelError(f"{what}: a rotation table is float32 [{B}, {hd // 2}] over the whole head")
     out = torch.empty((B, nh * hd), dtype=BF16, device=qkv.device)
+    if kept and (pages or not window or kept < 0):
+        raise KernelError(f"{what}: {kept} first positions stand behind a window ({window}), and are walked over by slices")
     if pages:
         if arrivals is None:
             arrivals = torch.zeros((B * nh,), dtype=torch.int32, device=qkv.device)
@@ -1023,11 +1027,12 @@ def attention_decode_fused(qkv, k_cache, v_cache, block_table, seq_slot, seq_sta
                      int(window or 0), _p(work), _p(arrivals), _p(out))
         return out
     work = _slices_workspace(what, work, B, nh, n_slices, hd, qkv.device)
-    library.call(attention_lib(hd), "palm_attention_decode_fused", _stream(), _p(qkv), int(as_planes),
+    more = (int(kept),) if kept else ()
+    library.call(attention_lib(hd), "palm_attention_decode_fused_kept" if kept else "palm_attention_decode_fused", _stream(), _p(qkv), int(as_planes),
                  qkv.shape[0] if as_planes else 1, _p(q_norm_w), _p(k_norm_w), float(eps), _p(cos), _p(sin),
                  int(rotary_dim if cos is not None else 0), int(pairing), int(write_cache), _p(k_cache), _p(v_cache),
                  _p(block_table), block_table.shape[1], _p(seq_slot), _p(seq_start), B, nh, nkv, hd, float(scale),
-                 int(window or 0), int(n_slices), _p(work), _p(out))
+                 int(window or 0), int(n_slices), _p(work), _p(out), *more)
     return out
 
 
@@ -1103,16 +1108,26 @@ def wide_prompt_attention(starts, counts, nh: int, nkv: int) -> bool:
     return wide_us < other_us
 
 
-def slices_of_step(ctx, nh: int, nkv: int, window: int | None) -> int:
+def slices_of_step(ctx, nh: int, nkv: int, window: int | None, kept: int = 0) -> int:
     """The slices of a decode step's key ranges: what a recorded step was cut for, else what fills the chip."""
-    keys = min(ctx.max_total, window) if window else ctx.max_total
+    keys = _kept_keys(ctx.max_total, window, kept) if kept else min(ctx.max_total, window) if window else ctx.max_total
     return ctx.decode_slices or decode_slices(ctx.n_seqs, nh, nkv, keys)
 
 
 def attention(q, k_cache, v_cache, block_table, ctx, nh: int, nkv: int, hd: int, scale: float, window: int | None,
-              q_prescaled: bool = False):
+              q_prescaled: bool = False, kept: int = 0):
     """The step's queries over the cache; picks the kernel by element type, head size and step shape.
-    ``q_prescaled``: see ``attention_prefill`` (only a prompt step on the matrix cores takes such queries)."""
+    ``q_prescaled``: see ``attention_prefill`` (only a prompt step on the matrix cores takes such queries).
+    ``kept``: the sequences' first so many positions are seen behind the window (``attention_kept``)."""
+    if kept:
+        _need(bool(window), "attention: first positions that stay visible stand behind a window")
+        # a recorded prompt is replayed behind histories of any length (it is sized for more new tokens than the recorded one has), a recorded step of
+        # single tokens for lengths rounded up, also beyond the longest sequence that there can be
+        room = block_table.shape[1] * PAGE_TOKENS
+        any_length = ctx.host and ctx.max_new > max(ctx.host["counts"], default=0)
+        return attention_kept(q, k_cache, v_cache, block_table, ctx.seq_slot, ctx.seq_start, ctx.seq_new, ctx.cu_new, ctx.max_new,
+                              room if any_length else min(ctx.max_total, room), nh, nkv, hd, scale, window, kept, q_prescaled=q_prescaled)
+
     def wide():
         # (a window leaves a block few pages, which the wide kernel's start and end outweigh: not measured)
         if window or not ctx.host or not attention_lib(hd).palm_attention_prefill_wide_serves():
@@ -2872,7 +2887,7 @@ def attention_kept_exact(q: torch.Tensor, k_cache, v_cache, block_table, seq_slo
     out = torch.empty_like(q)
     if n == 0 or B == 0 or max_new == 0:
         return out
-    slices = _kept_slices(B, max_new, max_total, nh, nkv, window, kept)
+    slices = _kept_slices(B, max_new, max(max_new, max_total), nh, nkv, window, kept)
     work = torch.empty((n * nh * slices * (hd + 4),), dtype=F32, device=q.device) if slices > 1 else None
     _call_on(q.get_device(), attention_kept_lib(), "palm_attention_kept", _p(q), _code(q, "attention_kept q"), _p(k_cache), _p(v_cache), _p(block_table),
              block_table.shape[1], _p(seq_slot), _p(seq_start), _p(seq_new), _p(cu_new), B, n, int(max_new), nh, nkv, hd, float(scale), window, kept,
@@ -2898,7 +2913,7 @@ def _refuse_kept(q, k_cache, v_cache, block_table, seq_slot, seq_start, seq_new,
           "attention_kept: per-sequence arrays differ in length")
     if not (window >= 1 and kept >= 0 and window < 1 << 30 and kept < 1 << 30):
         raise KernelError(f"{what}: a window of {window} positions and {kept} first ones: at least one, and none or more")
-    if not (0 <= max_new <= max_total <= block_table.shape[1] * PAGE_TOKENS):
+    if not (0 <= max_new and 0 <= max_total <= block_table.shape[1] * PAGE_TOKENS):
         raise KernelError(f"{what}: {max_new} new tokens in sequences of up to {max_total}; the page table has room for {block_table.shape[1] * PAGE_TOKENS}")
     raise KernelError(f"{what}: sizes are whole numbers")
 
@@ -2909,7 +2924,8 @@ def attention_kept(q: torch.Tensor, k_cache, v_cache, block_table, seq_slot, seq
     sequence's first ``kept`` ones (j < kept): what keeps a stream without an end within a bounded number of pages.
 
     q [n, nh hd]; sequence b has seq_new[b] queries (none, if it is zero) from row cu_new[b] on, at positions seq_start[b] and up, whose keys and values are
-    in the cache; ``max_new`` and ``max_total``: the most new tokens of a sequence and the longest sequence with them, or more.  Pages that no query of
+    in the cache; ``max_new``: the most new tokens of a sequence, or more; ``max_total``: the longest sequence with them, which sizes how the work is
+    cut and nothing else.  Pages that no query of
     the step sees are not read, whatever the page table says of them; what masked places hold (an infinity, a NaN) does not show.
     ``q_prescaled``: see ``attention_prefill``.  ``plan``: (wide, halves, slices), how a prompt goes on the matrix cores (None: ``kept_plan``)."""
     dev = q.get_device()
@@ -2922,7 +2938,7 @@ def attention_kept(q: torch.Tensor, k_cache, v_cache, block_table, seq_slot, seq
             and q.dtype is k_cache.dtype is v_cache.dtype and q.dtype in _CODES and nh > 0 and nkv > 0 and nh % nkv == 0
             and q.shape == (n, nh * hd) and k_cache.shape[1:] == (nkv, PAGE_TOKENS, hd) and v_cache.shape == (k_cache.shape[0], nkv, hd, PAGE_TOKENS)
             and seq_start.shape == seq_new.shape == seq_slot.shape == (B,) and cu_new.shape == (B + 1,) and 1 <= window < 1 << 30 and 0 <= kept < 1 << 30
-            and block_table.dim() == 2 and 0 <= max_new <= max_total <= block_table.shape[1] * PAGE_TOKENS):
+            and block_table.dim() == 2 and 0 <= max_new and 0 <= max_total <= block_table.shape[1] * PAGE_TOKENS):
         _refuse_kept(q, k_cache, v_cache, block_table, seq_slot, seq_start, seq_new, cu_new, max_new, max_total, nh, nkv, hd, window, kept)
     if not (q.dtype is BF16 and hd in MFMA_HEAD_DIMS):
         _need(not q_prescaled, "attention_kept: only the prompt kernel takes scaled queries")
@@ -2932,12 +2948,12 @@ def attention_kept(q: torch.Tensor, k_cache, v_cache, block_table, seq_slot, seq
         return out
     lib = attention_lib(hd)
     if max_new == 1 and n == B and not q_prescaled:              # (one token each: as many as there are sequences)
-        n_slices = decode_slices(B, nh, nkv, _kept_keys(max_total, window, kept))
+        n_slices = decode_slices(B, nh, nkv, _kept_keys(max(1, max_total), window, kept))
         work = torch.empty((B * nh * n_slices * (hd + 4),), dtype=F32, device=q.device) if n_slices > 1 else None
         _call_on(q.get_device(), lib, "palm_attention_decode_kept", _p(q), _p(k_cache), _p(v_cache), _p(block_table), block_table.shape[1], _p(seq_slot),
                  _p(seq_start), B, nh, nkv, hd, float(scale), window, n_slices, _p(work), _p(out), kept)
         return out
-    wide, halves, slices = plan or kept_plan(n, B, max_total, nh, nkv, hd, window, kept)
+    wide, halves, slices = plan or kept_plan(n, B, max(max_new, max_total), nh, nkv, hd, window, kept)
     if wide:
         _call_on(q.get_device(), lib, "palm_attention_prefill_wide_kept", _p(q), _p(k_cache), _p(v_cache), _p(block_table), block_table.shape[1], _p(seq_slot),
                  _p(seq_start), _p(seq_new), _p(cu_new), B, max_new, nh, nkv, hd, float(scale), window, int(bool(q_prescaled)), _p(out), kept)

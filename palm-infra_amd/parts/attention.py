@@ -1,5 +1,5 @@
 """Causal grouped-query attention over the cache, with optional per-head RMSNorm of q and k, a
-rotation of both, and an optional window.
+rotation of both, an optional window and, behind it, optional first positions that every query sees (``kept``).
 
 Order of operations as the reference builds it (models/qwen3.py:290-349): one joined q/k/v projection;
 per-head norm of q and k over head_dim with one weight vector for all heads; rotation of q and k; the
@@ -29,6 +29,9 @@ class Attention:
         self.nh, self.nkv, self.hd = int(p["num_heads"]), int(p["num_kv_heads"]), int(p["head_dim"])
         self.scale = float(p["scale"])
         self.window = int(p["window"]) if p.get("window") else None
+        self.kept = int(p.get("kept") or 0)
+        if self.kept < 0 or (self.kept and not self.window):
+            raise ValueError(f"attention: first positions that stay visible ({self.kept}) stand behind a window")
         if self.nh % self.nkv:
             raise ValueError(f"{self.nh} heads are not a multiple of {self.nkv} kv heads")
         bias = lambda name: builder.tensor(spec, name) if name in spec.tensors else None
@@ -48,12 +51,12 @@ class Attention:
             raise ValueError("attention: q_norm and k_norm must be over head_dim with one eps")
         self.position = builder.build(spec.parts["position"]) if "position" in spec.parts else None
         self.dtype = builder.dtype
-        self.decode_shape = (self.nh, self.nkv, self.hd, self.window)
+        self.decode_shape = (self.nh, self.nkv, self.hd, self.window, self.kept)
 
     def decode_form(self, starts: list[int], max_total: int) -> bool:
         """Whether the attention of a decode step of sequences that hold ``starts`` tokens is cut by pages; ``max_total``: the longest sequence that
         the step is sized for."""
-        if self.dtype != torch.bfloat16 or self.hd not in ops.MFMA_HEAD_DIMS or len(starts) > ops.DECODE_FUSED_ROWS:
+        if self.kept or self.dtype != torch.bfloat16 or self.hd not in ops.MFMA_HEAD_DIMS or len(starts) > ops.DECODE_FUSED_ROWS:
             return False
         most = self.window or max_total
         return ops.decode_pages_pays([min(n + 1, most) for n in starts], self.nh, self.nkv, self.hd, min(max_total, most))
@@ -61,7 +64,8 @@ class Attention:
     @staticmethod
     def cache_needs(spec):
         p = spec.params
-        return [KVNeed(int(p["num_kv_heads"]), int(p["head_dim"]), int(p["window"]) if p.get("window") else None)]
+        return [KVNeed(int(p["num_kv_heads"]), int(p["head_dim"]), int(p["window"]) if p.get("window") else None,
+                       kept=int(p.get("kept") or 0))]
 
     takes_sink = True
     takes_prenormed = True
@@ -95,10 +99,10 @@ class Attention:
             pages = self._by_pages(ctx) and ops.decode_pages_serves(ctx.n_seqs, self.nh, self.nkv, self.hd, lc.kv.table_dev.shape[1])
             o = ops.attention_decode_fused(
                 qkv, lc.k, lc.v, lc.kv.table_dev, ctx.seq_slot, ctx.seq_start, self.nh, self.nkv, self.hd, self.scale,
-                self.window, ops.slices_of_step(ctx, self.nh, self.nkv, self.window),
+                self.window, ops.slices_of_step(ctx, self.nh, self.nkv, self.window, self.kept),
                 q_norm_w=self.q_norm.weight if self.q_norm else None, k_norm_w=self.k_norm.weight if self.k_norm else None,
                 eps=self.q_norm.eps if self.q_norm else 0.0, cos=cos, sin=sin, rotary_dim=rotary_dim, pairing=pairing,
-                write_cache=lc.writes, pages=pages, arrivals=self._arrivals(ctx) if pages else None)
+                write_cache=lc.writes, pages=pages, arrivals=self._arrivals(ctx) if pages else None, kept=self.kept)
             return self.out(o, sink=sink)
         # a prompt's queries carry the scale (times log2 e) into their one rounding where the prompt kernel of this
         # head size takes them so: a score then leaves the matrix cores as the exponent of its weight
@@ -111,5 +115,5 @@ class Attention:
             k_cache=lc.k, v_cache=lc.v, block_table=lc.kv.table_dev, tok_slot=ctx.tok_slot, write_cache=lc.writes,
             out_dtype=self.dtype, q_scale=q_scale)
         o = ops.attention(q, lc.k, lc.v, lc.kv.table_dev, ctx, self.nh, self.nkv, self.hd, self.scale, self.window,
-                          q_prescaled=q_scale != 1.0)
+                          q_prescaled=q_scale != 1.0, kept=self.kept)
         return self.out(o, sink=sink)
