@@ -30,28 +30,51 @@ constexpr int KA_MAX_HD = 512;
 
 __device__ inline f32x4 mfma_16x16x4(float a, float b, f32x4 acc) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, acc, 0, 0, 0); }
 
-// Four consecutive elements from d on, widened; beyond hd zeros.  FOURS: hd is a multiple of four and rows start on their sizes.
-template <bool FOURS, typename T> __device__ inline f32x4 four_at(const T* row, int d, int hd) {
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if constexpr (FOURS) {
-        if (d < hd) {
-            if constexpr (sizeof(T) == 4) {
-                const float4 four = *reinterpret_cast<const float4*>(row + d);
-                v = f32x4{four.x, four.y, four.z, four.w};
-            } else {
-                const uint2 u = *reinterpret_cast<const uint2*>(row + d);
-                v = f32x4{__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u)};
-            }
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (d + e < hd) v[e] = to_float(row[d + e]);
-    }
+// A value the compiler knows nothing of: what is computed from it is computed there, and not kept in registers for the whole kernel.
+__device__ inline int fresh(int v) {
+    asm volatile("" : "+v"(v));
     return v;
 }
 
+// How a row of a head's elements is read: FULL: hd is all 16 DT of them; FOURS: hd is a multiple of four and rows start on their sizes; ANY.
+enum Rows { FULL, FOURS, ANY };
+
+// Four consecutive elements from d on, widened; beyond hd zeros.  Every read is unconditional (an absent one reads what is there and is made zero by a
+// select): behind a branch reads would be waited for one by one.
+template <Rows ROWS, typename T> __device__ inline f32x4 four_at(const T* row, int d, int hd) {
+    f32x4 v;
+    if constexpr (ROWS == ANY) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[e] = to_float(row[min(d + e, hd - 1)]);
+            v[e] = d + e < hd ? v[e] : 0.f;
+        }
+        return v;
+    } else {
+        const T* at = row + (ROWS == FULL ? d : min(d, hd - 4));
+        if constexpr (sizeof(T) == 4) {
+            const float4 four = *reinterpret_cast<const float4*>(at);
+            v = f32x4{four.x, four.y, four.z, four.w};
+        } else {
+            const uint2 u = *reinterpret_cast<const uint2*>(at);
+            v = f32x4{__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u)};
+        }
+        if constexpr (ROWS != FULL) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = d < hd ? v[e] : 0.f;
+        }
+        return v;
+    }
+}
+
+// `places` elements on: the same start in all lanes and an offset of 32 bits, which is how a load takes them without an address of 64 bits
+template <typename T> __device__ inline const T* further(const T* start, unsigned places) {
+    return reinterpret_cast<const T*>(reinterpret_cast<const char*>(start) + places * (unsigned)sizeof(T));
+}
+
 __device__ inline bool finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
+// e^x for x <= 0 (minus infinity: 0), to 2^-24 |x| and the hardware's 2^x's last place; what is below 2^-126 is zero beside a sum of at least 1
+__device__ inline float exp_weight(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
 
 // The pages that queries at positions lo .. hi see, as one row of n.
 struct SeenRow {
@@ -66,11 +89,20 @@ struct SeenRow {
 
 // grid (kv heads * groups of heads, tiles of positions, sequences * slices).  A record of the workspace, for each (row, head, slice): maximum, sum, two
 // floats unused, then the unnormalised output.
-template <typename T, int DT, bool FOURS>
-__global__ __launch_bounds__(KA_WAVES * WAVE) void attention_kept_kernel(
+//
+// Up to 128 elements a head (AHEAD) a page's keys are asked for together, and its values as the keys' registers come free: a wave has few pages, and
+// what it waits for memory is what a short prompt takes.  A page is 256 products of 32 clocks for heads of 128, 3.4 us of a wave.  A prompt of
+// 157 tokens, 32 heads of 128 over 8, a window of 64 takes 13.7 us (20.6 with reads behind branches, waited for one by one; 32 with two pages' reads in flight
+// and half the waves), 8.0 with heads of 64; 600 tokens with a window of 512: 76 us, 38 TFLOP/s, bounded by the products' own rate and the
+// causal half of each page that is computed and masked.  Longer heads have no registers for it and read as they go: heads of 256 take 53 us for the
+// 157 tokens.
+template <typename T, int DT, Rows ROWS>
+__global__ __launch_bounds__(KA_WAVES * WAVE) __attribute__((amdgpu_waves_per_eu(DT <= 8 ? 2 : 1))) void attention_kept_kernel(
     const T* __restrict__ q, const T* __restrict__ k_cache, const T* __restrict__ v_cache, const int* __restrict__ block_table, int max_pages,
     const int* __restrict__ seq_slot, const int* __restrict__ seq_start, const int* __restrict__ seq_new, const int* __restrict__ cu_new, int nh,
-    int nkv, int hd, float scale, int window, int kept, int heads, int slices, float* __restrict__ work, T* __restrict__ out) {
+    int nkv, int head_size, float scale, int window, int kept, int heads, int slices, float* __restrict__ work, T* __restrict__ out) {
+    constexpr bool AHEAD = DT <= 4 || (DT == 8 && ROWS == FULL);       // (more than that is more than the registers hold)
+    const int hd = ROWS == FULL ? DT * 16 : head_size;
     __shared__ f32x4 o_lds[KA_WAVES - 1][DT][WAVE];
     __shared__ float m_lds[KA_WAVES - 1][WAVE], l_lds[KA_WAVES - 1][WAVE];
     const int b = blockIdx.z / slices, slice = blockIdx.z % slices;
@@ -91,79 +123,135 @@ __global__ __launch_bounds__(KA_WAVES * WAVE) void attention_kept_kernel(
     const int per = (seen.n + slices - 1) / slices, begin = slice * per, end = min(seen.n, begin + per);
     const int all_first = max(0, start + last - window + 1), all_last = start + tile;   // keys from all_first to all_last: seen by every column
     const int* pages = block_table + (size_t)seq_slot[b] * max_pages;
+    auto place = [&](int i) { return ((size_t)__builtin_amdgcn_readfirstlane(pages[seen.page(i)]) * nkv + kvh) * PAGE_TOKENS * hd; };
 
-    f32x4 qv[DT], o[DT];
+    f32x4 qv[DT], o[DT], kd[AHEAD ? 4 : 1][DT], vd[AHEAD ? DT : 1][4];
+    auto read_key = [&](size_t at, int t, int dt) __attribute__((always_inline)) {
+        const T* page = k_cache + at;
+        if constexpr (ROWS == FULL) return four_at<FULL>(further(page, ((16 * t + r) * hd + dt * 16 + 4 * g)), 0, hd);
+        return four_at<ROWS>(further(page, (16 * t + r) * hd), dt * 16 + 4 * fresh(g), hd);
+    };
+    auto read_values = [&](size_t at, int dt, f32x4 (&to)[4]) __attribute__((always_inline)) {
+        const int d = dt * 16 + (AHEAD ? r : fresh(r));
+        const T* page = v_cache + at;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            to[t] = four_at<FULL>(further(page, (ROWS == FULL ? d : min(d, hd - 1)) * PAGE_TOKENS + 16 * t + 4 * g), 0, PAGE_TOKENS);
+            if constexpr (ROWS != FULL) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) to[t][e] = d < hd ? to[t][e] : 0.f;
+            }
+        }
+    };
     float m = -INFINITY, l = 0.f;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
-        qv[dt] = four_at<FOURS>(q + (row * nh + head) * hd, dt * 16 + 4 * g, hd);
+        qv[dt] = four_at<ROWS>(q + (row * nh + head) * hd, dt * 16 + 4 * g, hd);
         o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     for (int i = begin + wave; i < end; i += KA_WAVES) {
-        const int page = seen.page(i), key0 = page * PAGE_TOKENS;
-        const size_t at = ((size_t)pages[page] * nkv + kvh) * PAGE_TOKENS * hd;
-        const T *kp = k_cache + at, *vp = v_cache + at;
+        const int key0 = seen.page(i) * PAGE_TOKENS;
         const bool masked = all_last < key0 + PAGE_TOKENS - 1 || (all_first > key0 && kept < key0 + PAGE_TOKENS);   // the same in every lane
-        auto sees = [&](int in_page) { const int key = key0 + in_page; return key <= pos && (key >= first || key < kept); };
+        const size_t at = place(i);
+        if constexpr (AHEAD) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) kd[t][dt] = read_key(at, t, dt);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        // (no && or ||: a select, not a branch for every key)
+        auto sees = [&](int in_page) { const int key = key0 + in_page; return (key <= pos) & ((key >= first) | (key < kept)); };
         f32x4 s[4];
-        float mx = -INFINITY;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
-                const f32x4 kd = four_at<FOURS>(kp + (size_t)(16 * t + r) * hd, dt * 16 + 4 * g, hd);
+                if constexpr (!AHEAD)
+                    if (dt % 8 == 0) {
+                        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc = mfma_16x16x4(kd[e], qv[dt][e], acc);
+                        for (int x = dt; x < dt + 8 && x < DT; ++x) kd[0][x] = read_key(at, t, x);
+                    }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc = mfma_16x16x4(kd[AHEAD ? t : 0][dt][e], qv[dt][e], acc);
             }
+            s[t] = acc * scale;
+            if constexpr (AHEAD) {
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                s[t][e] = !masked || sees(16 * t + 4 * g + e) ? acc[e] * scale : -INFINITY;
-                mx = fmaxf(mx, s[t][e]);
+                for (int dt = 0; dt < DT; ++dt)
+                    if (dt * 4 / DT == t - 1 || (t == 3 && dt * 4 / DT == 3)) read_values(at, dt, vd[dt]);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
+        if (masked) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[t][e] = sees(16 * t + 4 * g + e) ? s[t][e] : -INFINITY;
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[t][e]);
         mx = fmaxf(mx, __shfl_xor(mx, 16, WAVE));
         mx = fmaxf(mx, __shfl_xor(mx, 32, WAVE));
         const float m_new = fmaxf(m, mx), from = m_new == -INFINITY ? 0.f : m_new;      // (a column may see no key of its tile's first pages)
-        const float alpha = m == -INFINITY ? 0.f : expf(m - from);
+        const float alpha = exp_weight(m - from);
         m = m_new;
         l *= alpha;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                s[t][e] = expf(s[t][e] - from);
+                s[t][e] = exp_weight(s[t][e] - from);
                 l += s[t][e];
             }
-        bool wild = false;
+        float wild = 0.f;                                       // a NaN: the page has values that are none
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
             f32x4 acc = o[dt] * alpha;
-            const int d = dt * 16 + r;
-            const T* vrow = vp + (size_t)min(d, hd - 1) * PAGE_TOKENS;
+            f32x4 (&v_of)[4] = vd[AHEAD ? dt : 0];
+            if constexpr (!AHEAD) {
+                if (dt % 2 == 0) __builtin_amdgcn_sched_barrier(0);     // (two tiles' values at a time: the outputs need the registers)
+                read_values(at, dt, v_of);
+            }
+            if (masked) {
+                float odd = 0.f;
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                f32x4 vd = four_at<true>(vrow, 16 * t + 4 * g, PAGE_TOKENS);
+                for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if (masked && !finite(vd[e])) { wild = true; vd[e] = 0.f; }
-                    if (d >= hd) vd[e] = 0.f;
-                    acc = mfma_16x16x4(vd[e], s[t][e], acc);
+                    for (int e = 0; e < 4; ++e) odd = fmaf(v_of[t][e], 0.f, odd);
+                if (__any(odd != 0.f)) {
+                    wild = NAN;
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v_of[t][e] = finite(v_of[t][e]) ? v_of[t][e] : 0.f;
                 }
             }
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc = mfma_16x16x4(v_of[t][e], s[t][e], acc);
             o[dt] = acc;
         }
-        if (__any(wild)) {
+        if (wild != 0.f) {                                      // (the same in every lane)
+            for (int j = 0; j < PAGE_TOKENS; ++j) {
+                const bool seen_here = sees(j);
+                const int d0 = AHEAD ? 4 * g : fresh(4 * g);
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
+                for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int d = dt * 16 + 4 * g + e;
-                    for (int j = 0; j < PAGE_TOKENS && d < hd; ++j) {
-                        const float v = to_float(vp[(size_t)d * PAGE_TOKENS + j]);
-                        if (!finite(v) && sees(j)) o[dt][e] += v;
+                    for (int e = 0; e < 4; ++e) {
+                        const int d = dt * 16 + d0 + e;
+                        const float v = to_float(v_cache[at + (size_t)min(d, hd - 1) * PAGE_TOKENS + j]);
+                        o[dt][e] += seen_here & !finite(v) & (d < hd) ? v : 0.f;
                     }
-                }
+            }
         }
     }
     l += __shfl_xor(l, 16, WAVE);
@@ -180,7 +268,7 @@ __global__ __launch_bounds__(KA_WAVES * WAVE) void attention_kept_kernel(
     for (int w = 0; w < KA_WAVES - 1; ++w) {
         const float mw = m_lds[w][lane], top = fmaxf(m, mw);
         if (mw == -INFINITY) continue;                          // it saw none of the column's keys
-        const float mine = m == -INFINITY ? 0.f : expf(m - top), its = expf(mw - top);
+        const float mine = exp_weight(m - top), its = exp_weight(mw - top);
         l = l * mine + l_lds[w][lane] * its;
         m = top;
 #pragma unroll
@@ -198,11 +286,18 @@ __global__ __launch_bounds__(KA_WAVES * WAVE) void attention_kept_kernel(
         return;
     }
     T* to = out + (row * nh + head) * hd;
+    const float inv = 1.0f / l;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+    for (int dt = 0; dt < DT; ++dt) {
+        const int d = dt * 16 + 4 * g;
+        if constexpr (ROWS == FULL && sizeof(T) == 4) {
+            *reinterpret_cast<float4*>(to + d) = make_float4(o[dt][0] * inv, o[dt][1] * inv, o[dt][2] * inv, o[dt][3] * inv);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (dt * 16 + 4 * g + e < hd) to[dt * 16 + 4 * g + e] = from_float<T>(o[dt][e] / l);
+            for (int e = 0; e < 4; ++e)
+                if (d + e < hd) to[d + e] = from_float<T>(o[dt][e] * inv);
+        }
+    }
 }
 
 // A wave for each (row, head): the slices' records in their order.
@@ -213,13 +308,14 @@ __global__ __launch_bounds__(WAVE) void attention_kept_join_kernel(const float* 
     float m = -INFINITY, l = 0.f;
     for (int s = lane; s < slices; s += WAVE) m = fmaxf(m, w[(size_t)s * (hd + 4)]);
     m = wave_max(m);
-    for (int s = lane; s < slices; s += WAVE) l += w[(size_t)s * (hd + 4) + 1] * expf(w[(size_t)s * (hd + 4)] - m);
+    for (int s = lane; s < slices; s += WAVE) l += w[(size_t)s * (hd + 4) + 1] * exp_weight(w[(size_t)s * (hd + 4)] - m);
     l = wave_sum(l);
     for (int d = lane; d < hd; d += WAVE) {
         float o = 0.f;
+#pragma unroll 8
         for (int s = 0; s < slices; ++s) {
-            const float ms = w[(size_t)s * (hd + 4)];
-            if (ms != -INFINITY) o += w[(size_t)s * (hd + 4) + 4 + d] * expf(ms - m);       // (an empty slice has no output)
+            const float ms = w[(size_t)s * (hd + 4)], v = w[(size_t)s * (hd + 4) + 4 + d];
+            o += ms == -INFINITY ? 0.f : v * exp_weight(ms - m);       // (an empty slice has no output)
         }
         out[(size_t)blockIdx.x * hd + d] = from_float<T>(o / l);
     }
@@ -254,16 +350,18 @@ PALM_API int palm_attention_kept(hipStream_t stream, const void* q, int dtype, c
     PALM_CHECK(y <= 65535 && z <= 65535, "attention_kept: %d new tokens of %d sequences in %d slices are more than one launch takes", max_new, n_seqs, slices);
     const dim3 grid((unsigned)x, (unsigned)y, (unsigned)z);
     const bool fours = hd % 4 == 0 && ((uintptr_t)q | (uintptr_t)k_cache) % 16 == 0;
-    PALM_CHECK((uintptr_t)v_cache % 16 == 0, "attention_kept: values do not start on 16 bytes");
-#define PALM_KEPT(DT, FOURS) attention_kept_kernel<T, DT, FOURS><<<grid, KA_WAVES * WAVE, 0, stream>>>((const T*)q, (const T*)k_cache, (const T*)v_cache, \
+    PALM_CHECK((uintptr_t)v_cache % 16 == 0 && (uintptr_t)out % 16 == 0, "attention_kept: values or results do not start on 16 bytes");
+#define PALM_KEPT(DT, ROWS) attention_kept_kernel<T, DT, ROWS><<<grid, KA_WAVES * WAVE, 0, stream>>>((const T*)q, (const T*)k_cache, (const T*)v_cache, \
         block_table, max_pages, seq_slot, seq_start, seq_new, cu_new, nh, nkv, hd, scale, window, kept, heads, slices, work, (T*)out)
     PALM_DTYPE_SWITCH(dtype, T,
-        if (!fours) { if (hd <= 128) PALM_KEPT(8, false); else PALM_KEPT(32, false); }
-        else if (hd <= 32) PALM_KEPT(2, true);
-        else if (hd <= 64) PALM_KEPT(4, true);
-        else if (hd <= 128) PALM_KEPT(8, true);
-        else if (hd <= 256) PALM_KEPT(16, true);
-        else PALM_KEPT(32, true);
+        if (!fours) { if (hd <= 128) PALM_KEPT(8, ANY); else PALM_KEPT(32, ANY); }
+        else if (hd == 64) PALM_KEPT(4, FULL);
+        else if (hd == 128) PALM_KEPT(8, FULL);
+        else if (hd <= 32) PALM_KEPT(2, FOURS);
+        else if (hd <= 64) PALM_KEPT(4, FOURS);
+        else if (hd <= 128) PALM_KEPT(8, FOURS);
+        else if (hd <= 256) PALM_KEPT(16, FOURS);
+        else PALM_KEPT(32, FOURS);
         PALM_LAUNCHED();
         if (slices > 1) { attention_kept_join_kernel<T><<<rows * nh, WAVE, 0, stream>>>(work, slices, hd, (T*)out); PALM_LAUNCHED(); });
 #undef PALM_KEPT
