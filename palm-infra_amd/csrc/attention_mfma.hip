@@ -98,6 +98,16 @@ template <bool KEPT> __device__ inline int page_of_row(int p, int page_lo, int f
 template <bool KEPT> __device__ inline bool key_is_seen(int key, int lo, int hi, int kept) {
     return KEPT ? key <= hi && (key >= lo || key < kept) : key >= lo && key <= hi;
 }
+// The same for all keys of a page: bit k for key k.
+__device__ inline uint64_t keys_seen(int lo, int hi, int kept) {
+    auto below = [](int n) { return n >= PAGE_TOKENS ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; };
+    return below(hi + 1) & (~below(lo) | below(kept));
+}
+// s where bit `bit` of `mask` is set, minus infinity elsewhere: two instructions (a comparison with each border and their joining are six)
+__device__ inline float if_bit(uint32_t mask, int bit, float s) {
+    const uint32_t all = (uint32_t)((int32_t)(mask << (31 - bit)) >> 31);
+    return __uint_as_float((__float_as_uint(s) & all) | (0xff800000u & ~all));
+}
 
 // Scores of a page's 64 keys against the columns' queries and the online softmax; leaves the page's
 // weights as the B operands of the second product.  Keys outside [lo, hi] (in-page indices) are masked.
@@ -1023,22 +1033,28 @@ __device__ inline void blank_values_after(bf16_t* v_lds, int tail) {
 // of which some query of the tile sees less than all keys, such values are made zero in LDS, and added at the end, as they are, to the results of the
 // queries that do see them (add_wild_values; inside the walk it would cost its registers).  This also blanks the values behind the sequence's last key (`tail`, an in-page index).  True: there were some among those seen.
 __device__ inline bool tame_values(bf16_t* v_lds, int tail) {
+    constexpr int CHUNKS_OF_PAGE = HD * (PAGE_TOKENS / 8), MINE = (CHUNKS_OF_PAGE + PF_THREADS - 1) / PF_THREADS;
     bool found = false;
-    for (int idx = threadIdx.x % PF_THREADS; idx < HD * (PAGE_TOKENS / 8); idx += PF_THREADS) {
+#pragma unroll
+    for (int n = 0; n < MINE; ++n) {
+        // (where the threads do not come out even the last one's chunk is taken by several, which store the same)
+        const int idx = min((int)threadIdx.x % PF_THREADS + n * PF_THREADS, CHUNKS_OF_PAGE - 1);
         const int d = idx / (PAGE_TOKENS / 8), chunk = idx % (PAGE_TOKENS / 8);
         uint4* at = reinterpret_cast<uint4*>(v_lds + d * V_STRIDE + (chunk ^ v_swizzle(d)) * 8);
         uint4 v = *at;
         uint32_t* two = reinterpret_cast<uint32_t*>(&v);
-        bool change = false;
+        uint32_t carried = 0;                     // an exponent of ones and one more reach the next bit; both halves of a word at once
+#pragma unroll
+        for (int w = 0; w < 4; ++w) carried |= (two[w] & 0x7f807f80u) + 0x00800080u;
+        if ((carried & 0x80008000u) == 0 && chunk * 8 + 7 <= tail) continue;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const uint32_t mask = e % 2 ? 0xffff0000u : 0xffffu, exponent = e % 2 ? 0x7f800000u : 0x7f80u;
             const bool wild = (two[e / 2] & exponent) == exponent, behind = chunk * 8 + e > tail;
             found = found || (wild && !behind);
-            change = change || wild || behind;
             if (wild || behind) two[e / 2] &= ~mask;
         }
-        if (change) *at = v;
+        *at = v;
     }
     return found;
 }
@@ -1494,12 +1510,14 @@ __device__ __forceinline__ void paired_page(const bf16_t* k_lds, const bf16_t* v
         }
         if (masked) {
             const int lo = u[x].first - page_first_key, hi = u[x].pos - page_first_key;
+            const uint64_t seen = KEPT ? keys_seen(lo, hi, kept - page_first_key) >> 8 * g : 0;     // (the lane's keys are 8 g .. 8 g + 7 and 32 more)
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int key = tile_key(t, 4 * g + i);
-                    s[x][t][i] = key_is_seen<KEPT>(key, lo, hi, kept - page_first_key) ? s[x][t][i] : -INFINITY;
+                    if constexpr (KEPT) s[x][t][i] = if_bit((uint32_t)(seen >> t / 2 * 32), t % 2 * 4 + i, s[x][t][i]);
+                    else s[x][t][i] = key_is_seen<KEPT>(key, lo, hi, kept - page_first_key) ? s[x][t][i] : -INFINITY;
                 }
         }
         float top = s[x][0][0];
@@ -1563,28 +1581,75 @@ __device__ __forceinline__ void paired_page(const bf16_t* k_lds, const bf16_t* v
             for (int x = 0; x < PF_UNITS; ++x) u[x].o[dt] = mfma_16x16x32(vf[dt][h], pv[x][h], u[x].o[dt]);
 }
 
+// The `nth` of all sequences' tiles of qb queries, those of the highest number first and of one number by their sequence (sequence -1: there are
+// fewer); `most`: tiles of a sequence, or more.  In the sequences' order the last one's long tiles would be alone at the end; and a die hands its blocks to its four
+// engines in turn by their number, whether they have work or not, so blocks for tiles that a sequence lacks upset the engines' shares.  32 heads of 128 on
+// 8, a window of 1,024: 40 single tokens and a prompt of 800 46 us, 2,000 and 100 tokens 44; with such empty blocks, the sequences' order turned by one at every
+// number, 79 and 52 (not turned, four long prompts take twice as long); 48 prompts of 20 to 300 tokens, a window of 128: 66 and 60.
+struct NthTile {
+    int tile = 0, sequence = -1;
+    __device__ NthTile(int nth, const int* __restrict__ seq_new, int n_seqs, int qb, int most) {
+        const int lane = threadIdx.x % WAVE;
+        auto tiles_of = [&](int b) { return b < n_seqs ? (seq_new[b] + qb - 1) / qb : 0; };
+        const int mine = tiles_of(lane);
+        auto from_number = [&](int t) {           // tiles with that number or a higher one
+            int n = max(0, mine - t);
+            for (int b = lane + WAVE; b < n_seqs; b += WAVE) n += max(0, tiles_of(b) - t);
+            n += __builtin_amdgcn_update_dpp(0, n, 0x111, 0xf, 0xf, false);      // rows of 16 lanes: row_shr 1, 2, 4, 8
+            n += __builtin_amdgcn_update_dpp(0, n, 0x112, 0xf, 0xf, false);
+            n += __builtin_amdgcn_update_dpp(0, n, 0x114, 0xf, 0xf, false);
+            n += __builtin_amdgcn_update_dpp(0, n, 0x118, 0xf, 0xf, false);
+            return __builtin_amdgcn_readlane(n, 15) + __builtin_amdgcn_readlane(n, 31) + __builtin_amdgcn_readlane(n, 47) + __builtin_amdgcn_readlane(n, 63);
+        };
+        if (from_number(0) <= nth) return;
+        int above = most, behind = 0;             // `behind`: tiles that come before those of number `tile`
+        while (above - tile > 1) {
+            const int mid = (tile + above) / 2, n = from_number(mid);
+            if (n > nth) tile = mid; else above = mid, behind = n;
+        }
+        if (above == most) behind = 0;
+        int left = nth - behind;
+        for (int b0 = 0; b0 < n_seqs; b0 += WAVE) {
+            uint64_t who = __ballot((b0 == 0 ? mine : tiles_of(b0 + lane)) > tile);
+            const int here = __popcll(who);
+            if (left >= here) { left -= here; continue; }
+            for (; left > 0; --left) who &= who - 1;
+            sequence = b0 + __ffsll((unsigned long long)who) - 1;
+            return;
+        }
+    }
+};
+
 template <int HALVES, bool PRESCALED, bool KEPT>
 __global__ __launch_bounds__(HALVES * PF_THREADS) PF_WAVES_PER_SIMD void attention_prefill_paired_kernel(
     const bf16_t* __restrict__ q, const bf16_t* __restrict__ k_cache, const bf16_t* __restrict__ v_cache,
     const int* __restrict__ block_table, int max_pages, const int* __restrict__ seq_slot,
     const int* __restrict__ seq_start, const int* __restrict__ seq_new, const int* __restrict__ cu_new, int nh,
     int nkv, float scale_log2, int window, int qb, int hg, int partners_follow, bf16_t* __restrict__ out, int kept, int slices,
-    float* __restrict__ work) {
+    float* __restrict__ work, int n_seqs, int tiles_most) {
     if constexpr (PF_DMA) {
         constexpr int K_TILE = PAGE_TOKENS * K_STRIDE, V_TILE = HD * V_STRIDE;
         __shared__ __attribute__((aligned(16))) bf16_t k_lds[HALVES * 2 * K_TILE];
         __shared__ __attribute__((aligned(16))) bf16_t v_lds[HALVES * 2 * V_TILE];
 
-        const int b = KEPT ? blockIdx.z / slices : blockIdx.z, slice = KEPT ? blockIdx.z % slices : 0;
+        int b = blockIdx.z, y = blockIdx.y, slice = 0;
         const int G = nh / nkv, n_hg = (G + hg - 1) / hg;
         const int kvh = blockIdx.x / n_hg, hgi = blockIdx.x % n_hg;   // the kv head runs fastest over the blocks, see the launch
+        if constexpr (KEPT) {
+            slice = blockIdx.y, y = blockIdx.z, b = 0;
+            if (n_seqs > 1) {
+                const NthTile nth(y, seq_new, n_seqs, qb, tiles_most);
+                if (nth.sequence < 0) return;
+                b = nth.sequence, y = nth.tile;
+            }
+        }
         const int n_new = seq_new[b];
         const int subs = qb / 16, n_q = (n_new + qb - 1) / qb;        // tiles of qb queries in this sequence
-        if ((int)blockIdx.y >= n_q) return;
+        if (y >= n_q) return;
         // first the tiles from the back (the long ones), the last first; then, where the launch asks for it, their
         // partners from the front in the same order, else the rest from the back too
-        const int from_back = (n_q + 1) / 2, y = blockIdx.y;
-        const int tile = y < from_back || !partners_follow ? n_q - 1 - y : y - from_back;
+        const int from_back = (n_q + 1) / 2;
+        const int tile = KEPT && n_seqs > 1 ? y : y < from_back || !partners_follow ? n_q - 1 - y : y - from_back;
         const int lane = threadIdx.x % WAVE, r = lane % 16, g = lane / 16;
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE) % PF_WAVES;
         const int half = HALVES > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / PF_THREADS) : 0;
@@ -1597,6 +1662,21 @@ __global__ __launch_bounds__(HALVES * PF_THREADS) PF_WAVES_PER_SIMD void attenti
 
         {
             const int tile_first = tile * qb;                         // the tile's first query, within the step
+            // the pages any query of the tile sees (the same for all waves)
+            const int tile_last = min(tile_first + qb - 1, n_new - 1);
+            const int row_hi = (start + tile_last) / PAGE_TOKENS;
+            const int page_lo = window > 0 ? max(0, start + tile_first - window + 1) / PAGE_TOKENS : 0;
+            const int front = pages_in_front<KEPT>(kept, page_lo), row_lo = page_lo - front;        // the row of pages, see page_of_row
+            const int per = KEPT ? (row_hi - row_lo + slices) / slices : 0;                         // pages of a slice of it
+            const int p_lo = KEPT ? row_lo + slice * per : row_lo, p_hi = KEPT ? min(row_hi, p_lo + per - 1) : row_hi;
+            // of every HALVES pages in turn each half takes one, into two places of its own
+            bf16_t *k_half = k_lds + half * 2 * K_TILE, *v_half = v_lds + half * 2 * V_TILE;
+            auto load_page = [&](int p, int step) {
+                const size_t at = ((size_t)pages[page_of_row<KEPT>(p, page_lo, front)] * nkv + kvh) * PAGE_TOKENS * HD;
+                page_into_lds(k_cache + at, v_cache + at, sources, k_half + step % 2 * K_TILE, v_half + step % 2 * V_TILE);
+            };
+            // (with KEPT the first page is on its way before the queries are asked for)
+            if (KEPT && p_lo + half <= p_hi) load_page(p_lo + half, 0);
             PairedUnit u[PF_UNITS];
 #pragma unroll
             for (int x = 0; x < PF_UNITS; ++x) {
@@ -1627,19 +1707,6 @@ __global__ __launch_bounds__(HALVES * PF_THREADS) PF_WAVES_PER_SIMD void attenti
 #pragma unroll
                 for (int dt = 0; dt < DTILES; ++dt) u[x].o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
             }
-            // the pages any query of the tile sees (the same for all waves)
-            const int tile_last = min(tile_first + qb - 1, n_new - 1);
-            const int row_hi = (start + tile_last) / PAGE_TOKENS;
-            const int page_lo = window > 0 ? max(0, start + tile_first - window + 1) / PAGE_TOKENS : 0;
-            const int front = pages_in_front<KEPT>(kept, page_lo), row_lo = page_lo - front;        // the row of pages, see page_of_row
-            const int per = KEPT ? (row_hi - row_lo + slices) / slices : 0;                         // pages of a slice of it
-            const int p_lo = KEPT ? row_lo + slice * per : row_lo, p_hi = KEPT ? min(row_hi, p_lo + per - 1) : row_hi;
-            // of every HALVES pages in turn each half takes one, into two places of its own
-            bf16_t *k_half = k_lds + half * 2 * K_TILE, *v_half = v_lds + half * 2 * V_TILE;
-            auto load_page = [&](int p, int step) {
-                const size_t at = ((size_t)pages[page_of_row<KEPT>(p, page_lo, front)] * nkv + kvh) * PAGE_TOKENS * HD;
-                page_into_lds(k_cache + at, v_cache + at, sources, k_half + step % 2 * K_TILE, v_half + step % 2 * V_TILE);
-            };
             // is every key of page p visible to every column of this wave?
             auto interior = [&](int key0) -> bool {
                 bool inside = true;
@@ -1655,8 +1722,10 @@ __global__ __launch_bounds__(HALVES * PF_THREADS) PF_WAVES_PER_SIMD void attenti
             };
             __shared__ int wild;                                      // some such page held values that were taken out
             if (KEPT && threadIdx.x == 0) wild = 0;
-            wait_for_all_but_the_youngest_loads<0>();                 // the queries
-            if (p_lo + half <= p_hi) load_page(p_lo + half, 0);
+            if constexpr (!KEPT) {
+                wait_for_all_but_the_youngest_loads<0>();             // the queries
+                if (p_lo + half <= p_hi) load_page(p_lo + half, 0);
+            }
             wait_for_all_but_the_youngest_loads<0>();
             page_barrier();
             for (int step = 0; p_lo + step * HALVES <= p_hi; ++step) {    // the same number of steps for all waves
@@ -2223,14 +2292,17 @@ static int launch_attention_prefill(hipStream_t stream, const void* q, const voi
     if constexpr (PF_DMA) {
         const int n_q = (max_new + qb - 1) / qb;
         PALM_CHECK(n_q <= 65535, "attention_prefill: %d new tokens are more than one launch takes", max_new);
-        PALM_CHECK(slices >= 1 && slices <= WAVE && (long long)n_seqs * slices <= 65535 && (slices == 1 || work), "attention_prefill: %d slices", slices);
-        dim3 grid(nkv * n_hg, n_q, n_seqs * slices);
+        PALM_CHECK(slices >= 1 && slices <= WAVE && (slices == 1 || work), "attention_prefill: %d slices", slices);
+        // (with KEPT the sequences' tiles are counted through, see NthTile: at most one of each sequence is not full)
+        const int tiles = KEPT && n_seqs > 1 ? (int)min((long long)n_q * n_seqs, (long long)rows / qb + n_seqs) : n_q;
+        PALM_CHECK(tiles <= 65535, "attention_prefill: %d new tokens of %d sequences are more than one launch takes", rows, n_seqs);
+        const dim3 grid(nkv * n_hg, KEPT ? slices : n_q, KEPT ? tiles : n_seqs);
         const long long blocks = (long long)grid.x * grid.y * grid.z;
         const bool few = halves ? halves == 2 : prefill_takes_halves(n_seqs, max_new, max_keys, nh, nkv, KEPT ? window + kept : window);
         const int partners_follow = !few && blocks <= 512 && n_seqs == 1;     // all blocks run at once, two a unit
 #define PALM_PAIRED(HALVES, PRE) attention_prefill_paired_kernel<HALVES, PRE, KEPT><<<grid, HALVES * PF_THREADS, 0, stream>>>( \
         (const bf16_t*)q, (const bf16_t*)k_cache, (const bf16_t*)v_cache, block_table, max_pages, seq_slot, seq_start, seq_new, \
-        cu_new, nh, nkv, scale_log2, window, qb, hg, partners_follow, (bf16_t*)out, kept, slices, work)
+        cu_new, nh, nkv, scale_log2, window, qb, hg, partners_follow, (bf16_t*)out, kept, slices, work, n_seqs, n_q)
         if (few) { if (q_prescaled) PALM_PAIRED(2, true); else PALM_PAIRED(2, false); }
         else { if (q_prescaled) PALM_PAIRED(1, true); else PALM_PAIRED(1, false); }
 #undef PALM_PAIRED

@@ -117,6 +117,19 @@ def test_a_step_of_single_tokens(ops, nh, nkv, hd, window, kept, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("sequences", [2, 63, 64, 65, 130])
+@pytest.mark.parametrize("nh,nkv,hd", LONG)
+@pytest.mark.parametrize("plan", [None, (False, 1, 1), (False, 2, 3)])
+def test_prompts_of_many_sequences_beside_single_tokens(ops, nh, nkv, hd, sequences, plan):
+    """One long prompt (at either end or within), the others a token, some, or none."""
+    for longest in (0, sequences // 2, sequences - 1):
+        seqs = [(40 * b % 300, (0, 1, 33, 1)[b % 4]) for b in range(sequences)]
+        seqs[longest] = (17, 300)
+        case = Case(seqs, nh, nkv, hd, 100, 3, BF16, seed=longest)
+        case.check(case.run(ops, plan=plan))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("nh,nkv,hd", LONG)
 @pytest.mark.parametrize("seqs", [[(5000, 1)], [(3000, 1), (70, 1), (2047, 1)], [(3000, 5)], [(0, 700)], [(900, 300), (0, 65)]])
