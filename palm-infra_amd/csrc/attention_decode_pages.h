@@ -23,6 +23,9 @@
 // sequence alike, and so): 45 sequences of 70 to 1,500 tokens 44.9 and 35.2 (4.0 TB/s with all of it), 64 of 2,048 106.8 and 100.4, 8 of 2,048 20.8 and 17.7, one of
 // 777 8.9 and 12.0: ops.decode_pages_pays.  The pages pass once and are marked so (nt): without that 37.6 105.2 19.3 for the first three.  Pages through LDS in whole lines against fragments read as the matrix cores want them, 16 rows by 64 bytes: 45
 // sequences 39.6 and 37.9, one of 100 15.8 and 10.8.  Tried: rings of 16 KB (no change).
+//
+// With KEPT a sequence's first pages stand in front of its window's (SeenPages): 48 sequences of 300 to 9,000 tokens, the last 4,096 and the first 4 seen, 645 MB,
+// 106 us, 6.1 TB/s (by slices 121 and 5 to join them).  Its queries may also come finished (row_heads == nh), their keys in the cache.
 constexpr bool PAGES_SERVE_HEAD = HD == 64 || HD == 128;
 constexpr int DP_WAVES = 8, DP_THREADS = DP_WAVES * WAVE;
 constexpr int DP_BLOCKS = 256;               // one a compute unit
@@ -76,12 +79,15 @@ __device__ __forceinline__ int read_index(const int* p) { return *(const __attri
 
 // The keys of the cache that a new position sees, first .. last, as pages: lo and the n from there on.  With a key of its own making the step sees the
 // cache up to the position before.  A sequence that sees none has one page, all of it hidden, so that it is somebody's.
+// With KEPT the pages of the sequence's first `kept` keys that lie before `lo` stand in front, and count in n.
+template <bool KEPT>
 struct SeenPages {
-    int lo, n;
-    __device__ SeenPages(int pos, int window, bool writes) {
+    int lo, n, front;
+    __device__ SeenPages(int pos, int window, bool writes, int kept) {
         const int first = window > 0 ? max(0, pos - window + 1) : 0;
         lo = first / PAGE_TOKENS;
-        n = max(writes ? pos - 1 : pos, first) / PAGE_TOKENS - lo + 1;
+        front = pages_in_front<KEPT>(kept, lo);
+        n = max(writes ? pos - 1 : pos, first) / PAGE_TOKENS - lo + 1 + front;
     }
 };
 
@@ -119,10 +125,12 @@ __device__ __forceinline__ float max_of_8(float v) {
 }
 
 // The step's sequences, two a lane (l and l + 64): new position, slot, and the pages of the sequences before.
+template <bool KEPT>
 struct StepPages {
     const int* __restrict__ block_table;
     int pos[2], slot[2], before[2], total, n_seqs, nkv, kvh, window, max_pages;
     bool writes;
+    int kept;
     __device__ static int of(const int (&v)[2], int b) {                   // b the same in every lane
         const int low = __builtin_amdgcn_readlane(v[0], b % WAVE), high = __builtin_amdgcn_readlane(v[1], b % WAVE);
         return b < WAVE ? low : high;
@@ -134,12 +142,12 @@ struct StepPages {
             pos[i] = seq_start[min(lane + WAVE * i, n_seqs - 1)];
             slot[i] = seq_slot[min(lane + WAVE * i, n_seqs - 1)];
         }
-        const int n0 = lane < n_seqs ? SeenPages(pos[0], window, writes).n : 0, sum0 = lanes_up_to(n0);
+        const int n0 = lane < n_seqs ? SeenPages<KEPT>(pos[0], window, writes, kept).n : 0, sum0 = lanes_up_to(n0);
         before[0] = sum0 - n0;
         total = __builtin_amdgcn_readlane(sum0, WAVE - 1);
         before[1] = total;
         if (n_seqs > WAVE) {
-            const int n1 = lane + WAVE < n_seqs ? SeenPages(pos[1], window, writes).n : 0, sum1 = lanes_up_to(n1);
+            const int n1 = lane + WAVE < n_seqs ? SeenPages<KEPT>(pos[1], window, writes, kept).n : 0, sum1 = lanes_up_to(n1);
             before[1] = total + sum1 - n1;
             total += __builtin_amdgcn_readlane(sum1, WAVE - 1);
         }
@@ -154,26 +162,30 @@ struct StepPages {
 };
 
 // A page of the row: its sequence, and which of the sequence's pages it is.
+template <bool KEPT>
 struct PagePlace {
-    int b, p, n, lo, pos;
-    __device__ PagePlace(const StepPages& s, int x, int lane) {
+    using Step = StepPages<KEPT>;
+    int b, p, n, lo, pos, front;
+    __device__ PagePlace(const Step& s, int x, int lane) {
         b = s.sequence_of(x, lane);
         enter(s);
         p = x - s.begin(b);
     }
-    __device__ void enter(const StepPages& s) {
-        pos = StepPages::of(s.pos, b);
-        const SeenPages seen(pos, s.window, s.writes);
+    __device__ void enter(const Step& s) {
+        pos = Step::of(s.pos, b);
+        const SeenPages<KEPT> seen(pos, s.window, s.writes, s.kept);
         lo = seen.lo;
         n = seen.n;
+        front = seen.front;
     }
-    __device__ void advance(const StepPages& s) {                          // (there is a next one)
+    __device__ void advance(const Step& s) {                          // (there is a next one)
         if (++p < n) return;
         p = 0;
         ++b;
         enter(s);
     }
-    __device__ size_t bytes(const StepPages& s) const { return s.page_bytes(b, lo + p); }
+    __device__ int page() const { return page_of_row<KEPT>(lo - front + p, lo, front); }
+    __device__ size_t bytes(const Step& s) const { return s.page_bytes(b, page()); }
 };
 
 // A number that the compiler takes for a new one: what is made of it is made where it is used, not kept from the kernel's start.
@@ -219,15 +231,19 @@ struct RingPlaces {
 template <int P> using Part = std::integral_constant<int, P>;
 
 // score_page's softmax for scores that carry the scale and log2 e already; a page without hidden keys does without masks
-__device__ __forceinline__ float weigh_scores(f32x4 (&s)[4], int lo, int hi, Columns& c, int lane, bf16x8 (&pv)[2]) {
-    if (lo > 0 || hi < PAGE_TOKENS - 1) {
+// (`seen`: with KEPT which keys are seen, bit by bit)
+template <bool KEPT>
+__device__ __forceinline__ float weigh_scores(f32x4 (&s)[4], int lo, int hi, Columns& c, int lane, bf16x8 (&pv)[2], uint64_t seen) {
+    if (KEPT ? ~seen != 0 : lo > 0 || hi < PAGE_TOKENS - 1) {
         const int g = made_here(lane) / 16;
+        const uint64_t mine = KEPT ? seen >> 8 * g : 0;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int key = t / 2 * 32 + 8 * g + t % 2 * 4 + i;         // tile_key(t, 4 g + i)
-                s[t][i] = key >= lo && key <= hi ? s[t][i] : -INFINITY;
+                if constexpr (KEPT) s[t][i] = if_bit((uint32_t)(mine >> t / 2 * 32), t % 2 * 4 + i, s[t][i]);
+                else s[t][i] = key >= lo && key <= hi ? s[t][i] : -INFINITY;
             }
     }
     float mx = -INFINITY;
@@ -259,6 +275,13 @@ __device__ __forceinline__ bf16x8 seen_values(bf16x8 v, int last) {
     return v;
 }
 
+// Elements of a fragment whose bits are set, zeros in the others' place
+__device__ __forceinline__ bf16x8 seen_values(bf16x8 v, uint32_t bits) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = bits >> e & 1 ? v[e] : (__bf16)0.0f;
+    return v;
+}
+
 template <typename TIN, int PLANES>
 struct SequenceQueries {
     // What a wave makes of one sequence: the rows of G query heads, then the new key's and the new value's, CHUNKS lanes a row.
@@ -270,16 +293,16 @@ struct SequenceQueries {
     const TIN* row[PASSES];
 
     __device__ void ask(const TIN* __restrict__ qkv, size_t plane_stride, const float* q_norm_w, const float* k_norm_w, const float* cos_t,
-                        const float* sin_t, int b, int kvh, int G, int nh, int nkv, int lane) {
+                        const float* sin_t, int b, int kvh, int G, int nh, int row_heads, int lane) {
         const int sub = lane / CHUNKS, ch = lane % CHUNKS;
         const size_t turn = (size_t)b * (HD / 2) + ch % (CHUNKS / 2) * 8;
         cs.read(cos_t ? cos_t + turn : k_norm_w ? k_norm_w : (const float*)qkv);       // (something that is there, where nothing is asked for)
         sn.read(cos_t ? sin_t + turn : k_norm_w ? k_norm_w : (const float*)qkv);
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
-            const int t = min(i * ROWS + sub, G + 1);
+            const int t = min(i * ROWS + sub, row_heads > nh ? G + 1 : G - 1), nkv = (row_heads - nh) / 2;
             const int head = t < G ? kvh * G + t : t == G ? nh + kvh : nh + nkv + kvh;
-            row[i] = qkv + ((size_t)b * (nh + 2 * nkv) + head) * HD + ch * 8;
+            row[i] = qkv + ((size_t)b * row_heads + head) * HD + ch * 8;
 #pragma unroll
             for (int pl = 0; pl < HELD; ++pl) raw[i][pl].read(row[i] + pl * plane_stride);
             w[i].read(q_norm_w ? (t < G ? q_norm_w : k_norm_w) + ch * 8 : (const float*)qkv);
@@ -367,14 +390,14 @@ struct SequenceQueries {
     }
 };
 
-template <typename TIN, int PLANES>
+template <typename TIN, int PLANES, bool KEPT>
 __global__ __launch_bounds__(DP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) void attention_decode_pages_kernel(
     const TIN* __restrict__ qkv, int planes, size_t plane_stride, const float* __restrict__ q_norm_w,
     const float* __restrict__ k_norm_w, float eps, const float* __restrict__ cos_t, const float* __restrict__ sin_t,
     int write_cache, bf16_t* __restrict__ k_cache, bf16_t* __restrict__ v_cache,
     const int* __restrict__ block_table, int max_pages, const int* __restrict__ seq_slot,
     const int* __restrict__ seq_start, int n_seqs, int nh, int nkv, float scale_log2, int window,
-    float* work, int* arrivals, bf16_t* __restrict__ out) {
+    float* work, int* arrivals, bf16_t* __restrict__ out, int kept, int row_heads) {
     if constexpr (PAGES_SERVE_HEAD) {
         __shared__ __attribute__((aligned(1024))) char ring[DP_WAVES][DP_RING];
         __shared__ bf16x8 queries[DP_QUERIES][DP_HEADS * CHUNKS];
@@ -391,7 +414,7 @@ __global__ __launch_bounds__(DP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
         const int G = nh / nkv, kvh = blockIdx.y;
         if (wave == DP_WAVES - 1) __builtin_amdgcn_s_setprio(3);             // it makes queries, for which all wait
 
-        StepPages step{block_table, {0, 0}, {0, 0}, {0, 0}, 0, n_seqs, nkv, kvh, window, max_pages, write_cache != 0};
+        StepPages<KEPT> step{block_table, {0, 0}, {0, 0}, {0, 0}, 0, n_seqs, nkv, kvh, window, max_pages, write_cache != 0, kept};
         step.read(seq_start, seq_slot, lane0);
         const int runs = min((int)gridDim.x, step.total), run = blockIdx.x;
         if (run >= runs) return;
@@ -410,10 +433,10 @@ __global__ __launch_bounds__(DP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
             // the rows would be one for all loads before.
             const bool makes_queries = DP_WAVES - 1 - wave < n_here;
             if (makes_queries) {
-                const int s = DP_WAVES - 1 - wave, b = seq0 + s, pos = StepPages::of(step.pos, b), lane = made_here(lane0);
+                const int s = DP_WAVES - 1 - wave, b = seq0 + s, pos = StepPages<KEPT>::of(step.pos, b), lane = made_here(lane0);
                 const bool owner = write_cache && step.begin(b + 1) <= c1;                    // this block has the sequence's last page
                 SequenceQueries<TIN, PLANES> make;
-                make.ask(qkv, plane_stride, q_norm_w, k_norm_w, cos_t, sin_t, b, kvh, G, nh, nkv, lane);
+                make.ask(qkv, plane_stride, q_norm_w, k_norm_w, cos_t, sin_t, b, kvh, G, nh, KEPT ? row_heads : nh + 2 * nkv, lane);
                 const size_t new_page = owner ? step.page_bytes(b, pos / PAGE_TOKENS) / 2 : 0;
                 make.prepare(planes, plane_stride, q_norm_w != nullptr, eps, cos_t != nullptr, owner, G, scale_log2, lane, queries[s],
                              new_key[wave], new_value[s], new_score[s], k_cache + new_page + (size_t)(pos % PAGE_TOKENS) * HD,
@@ -422,7 +445,7 @@ __global__ __launch_bounds__(DP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
             const RingPlaces places(made_here(lane0));
             const uint32_t ring0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)ring[wave]);
             int ask_at = 0, use_at = 0;                                    // slots, as bytes
-            PagePlace at(step, min(w0, c1 - 1), lane0);
+            PagePlace<KEPT> at(step, min(w0, c1 - 1), lane0);
             const char* keys = reinterpret_cast<const char*>(k_cache);
             const char* values = reinterpret_cast<const char*>(v_cache);
             size_t base = at.bytes(step);
@@ -501,7 +524,7 @@ __global__ __launch_bounds__(DP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
             // of this page or of the next one.  `more` (a constant): there is a next one.
             auto walk_page = [&](int x, auto more) __attribute__((always_inline)) {
                 const bool ends = at.p + 1 == at.n;
-                PagePlace next = at;
+                PagePlace<KEPT> next = at;
                 size_t next_base = base;
                 if constexpr (more.value) {
                     next.advance(step);
@@ -519,8 +542,9 @@ __global__ __launch_bounds__(DP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
                     if constexpr (AHEAD < DP_PARTS) ask(base, AHEAD);
                     else if constexpr (more.value) ask(next_base, AHEAD - DP_PARTS);
                 };
-                const int key0 = (at.lo + at.p) * PAGE_TOKENS;
+                const int key0 = at.page() * PAGE_TOKENS;
                 const int lo = (window > 0 ? max(0, at.pos - window + 1) : 0) - key0, hi = (write_cache ? at.pos - 1 : at.pos) - key0;
+                const uint64_t seen = KEPT ? keys_seen(lo, hi, kept - key0) : 0;                      // the same in every lane
                 f32x4 s[4];
                 auto score = [&](auto part) __attribute__((always_inline)) {
                     const char* slot = slot_arrives(part);
@@ -532,7 +556,7 @@ __global__ __launch_bounds__(DP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
                 };
                 score(Part<0>{}), score(Part<1>{}), score(Part<2>{}), score(Part<3>{});
                 bf16x8 pv[2];
-                const float alpha = weigh_scores(s, lo, hi, c, lane0, pv);
+                const float alpha = weigh_scores<KEPT>(s, lo, hi, c, lane0, pv, seen);
                 auto weigh = [&](auto part) __attribute__((always_inline)) {
                     const char* slot = slot_arrives(part);
 #pragma unroll
@@ -542,7 +566,9 @@ __global__ __launch_bounds__(DP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             bf16x8 v = *reinterpret_cast<const bf16x8*>(slot + places.value[h] + i * 2048);
-                            if (hi < PAGE_TOKENS - 1) v = seen_values(v, hi - h * 32 - made_here(lane0) / 16 * 8);           // the same in every lane
+                            if constexpr (KEPT) {                          // (what is not seen may be an infinity, with weight zero)
+                                if (~seen != 0) v = seen_values(v, (uint32_t)(seen >> (h * 32 + made_here(lane0) / 16 * 8)));
+                            } else if (hi < PAGE_TOKENS - 1) v = seen_values(v, hi - h * 32 - made_here(lane0) / 16 * 8);    // the same in every lane
                             o = mfma_16x16x32(v, pv[h], o);
                         }
                     }

@@ -812,14 +812,11 @@ PALM_API int palm_attention_decode_pages_serves(int nh, int nkv, int n_seqs, int
 // What `work` has to hold, in floats.
 PALM_API int palm_attention_decode_pages_work(int nh, int nkv) { return 2 * max(DP_BLOCKS, nkv) * (nh / nkv) * WORK_STRIDE; }
 
-// palm_attention_decode_fused by the kernel that is cut by pages.  arrivals: n_seqs * nh counters, zero before the call and after it; calls
-// that overlap in time need counters and a workspace of their own.
-PALM_API int palm_attention_decode_pages(hipStream_t stream, const void* qkv, int qkv_is_planes, int planes,
-                                         const float* q_norm_w, const float* k_norm_w, float eps, const float* cos_t,
-                                         const float* sin_t, int rotary_dim, int pairing, int write_cache, void* k_cache,
-                                         void* v_cache, const int* block_table, int max_pages, const int* seq_slot,
-                                         const int* seq_start, int n_seqs, int nh, int nkv, int hd, float scale,
-                                         int window, float* work, int* arrivals, void* out) {
+template <bool KEPT>
+static int launch_decode_pages(hipStream_t stream, const void* qkv, int qkv_is_planes, int planes, const float* q_norm_w, const float* k_norm_w, float eps,
+                               const float* cos_t, const float* sin_t, int rotary_dim, int pairing, int write_cache, void* k_cache, void* v_cache,
+                               const int* block_table, int max_pages, const int* seq_slot, const int* seq_start, int n_seqs, int nh, int nkv, int hd,
+                               float scale, int window, float* work, int* arrivals, void* out, int kept, int row_heads) {
     PALM_CHECK(hd == HD, "attention_decode_pages: this library was built for head size %d, not %d", HD, hd);
     PALM_CHECK((cos_t == nullptr) == (sin_t == nullptr), "attention_decode_pages: cos and sin tables come together");
     PALM_CHECK(palm_attention_decode_fused_serves(cos_t ? rotary_dim : 0, pairing),
@@ -833,9 +830,9 @@ PALM_API int palm_attention_decode_pages(hipStream_t stream, const void* qkv, in
     if (n_seqs == 0) return 0;
     PALM_CHECK(work && arrivals, "attention_decode_pages: a workspace and counters are needed");
     const size_t plane_stride = (size_t)n_seqs * (nh + 2 * nkv) * HD;
-#define PALM_PAGES(TIN, P) attention_decode_pages_kernel<TIN, P><<<dim3(max(1, DP_BLOCKS / nkv), nkv), DP_THREADS, 0, stream>>>( \
+#define PALM_PAGES(TIN, P) attention_decode_pages_kernel<TIN, P, KEPT><<<dim3(max(1, DP_BLOCKS / nkv), nkv), DP_THREADS, 0, stream>>>( \
         (const TIN*)qkv, planes, plane_stride, q_norm_w, k_norm_w, eps, cos_t, sin_t, write_cache, (bf16_t*)k_cache, \
-        (bf16_t*)v_cache, block_table, max_pages, seq_slot, seq_start, n_seqs, nh, nkv, scale * LOG2E, window, work, arrivals, (bf16_t*)out)
+        (bf16_t*)v_cache, block_table, max_pages, seq_slot, seq_start, n_seqs, nh, nkv, scale * LOG2E, window, work, arrivals, (bf16_t*)out, kept, row_heads)
     if (!qkv_is_planes) PALM_PAGES(bf16_t, 1);
     else if (planes == 1) PALM_PAGES(float, 1);
     else if (planes == 2) PALM_PAGES(float, 2);
@@ -843,6 +840,31 @@ PALM_API int palm_attention_decode_pages(hipStream_t stream, const void* qkv, in
 #undef PALM_PAGES
     PALM_LAUNCHED();
     return 0;
+}
+
+// palm_attention_decode_fused by the kernel that is cut by pages.  arrivals: n_seqs * nh counters, zero before the call and after it; calls
+// that overlap in time need counters and a workspace of their own.
+PALM_API int palm_attention_decode_pages(hipStream_t stream, const void* qkv, int qkv_is_planes, int planes,
+                                         const float* q_norm_w, const float* k_norm_w, float eps, const float* cos_t,
+                                         const float* sin_t, int rotary_dim, int pairing, int write_cache, void* k_cache,
+                                         void* v_cache, const int* block_table, int max_pages, const int* seq_slot,
+                                         const int* seq_start, int n_seqs, int nh, int nkv, int hd, float scale,
+                                         int window, float* work, int* arrivals, void* out) {
+    return launch_decode_pages<false>(stream, qkv, qkv_is_planes, planes, q_norm_w, k_norm_w, eps, cos_t, sin_t, rotary_dim, pairing, write_cache, k_cache, v_cache,
+                                      block_table, max_pages, seq_slot, seq_start, n_seqs, nh, nkv, hd, scale, window, work, arrivals, out, 0, nh + 2 * nkv);
+}
+// The same with the sequence's first `kept` keys visible behind the window (> 0).  plain: qkv is finished queries [n_seqs, nh hd] and the cache holds
+// their own keys and values already.
+PALM_API int palm_attention_decode_pages_kept(hipStream_t stream, const void* qkv, int qkv_is_planes, int planes,
+                                         const float* q_norm_w, const float* k_norm_w, float eps, const float* cos_t,
+                                         const float* sin_t, int rotary_dim, int pairing, int write_cache, void* k_cache,
+                                         void* v_cache, const int* block_table, int max_pages, const int* seq_slot,
+                                         const int* seq_start, int n_seqs, int nh, int nkv, int hd, float scale,
+                                         int window, float* work, int* arrivals, void* out, int kept, int plain) {
+    PALM_CHECK(window > 0 && kept >= 0 && kept < 1 << 30, "attention_decode_pages: window=%d kept=%d", window, kept);
+    PALM_CHECK(!plain || (!qkv_is_planes && !q_norm_w && !cos_t && !write_cache), "attention_decode_pages: finished queries are rows without norm or rotation");
+    return launch_decode_pages<true>(stream, qkv, qkv_is_planes, planes, q_norm_w, k_norm_w, eps, cos_t, sin_t, rotary_dim, pairing, write_cache, k_cache, v_cache,
+                                      block_table, max_pages, seq_slot, seq_start, n_seqs, nh, nkv, hd, scale, window, work, arrivals, out, kept, plain ? nh : nh + 2 * nkv);
 }
 
 // ---- decode without a workspace argument ------------------------------------------------------------

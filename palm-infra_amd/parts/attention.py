@@ -56,9 +56,9 @@ class Attention:
     def decode_form(self, starts: list[int], max_total: int) -> bool:
         """Whether the attention of a decode step of sequences that hold ``starts`` tokens is cut by pages; ``max_total``: the longest sequence that
         the step is sized for."""
-        if self.kept or self.dtype != torch.bfloat16 or self.hd not in ops.MFMA_HEAD_DIMS or len(starts) > ops.DECODE_FUSED_ROWS:
+        if self.dtype != torch.bfloat16 or self.hd not in ops.MFMA_HEAD_DIMS or len(starts) > ops.DECODE_FUSED_ROWS:
             return False
-        most = self.window or max_total
+        most = self.window + self.kept if self.window else max_total
         return ops.decode_pages_pays([min(n + 1, most) for n in starts], self.nh, self.nkv, self.hd, min(max_total, most))
 
     @staticmethod

@@ -159,6 +159,87 @@ def test_what_masked_places_hold_does_not_show(ops, nh, nkv, hd, seqs, dtype):
     case.check(case.run(ops))
 
 
+PAGED = [(4, 2, 64), (8, 8, 64), (8, 1, 64), (8, 2, 128), (5, 1, 128), (16, 2, 128)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nh,nkv,hd", PAGED)
+@pytest.mark.parametrize("lengths", [[0], [63], [64, 0], [5000], [0, 1, 63, 64, 65, 127, 500, 301, 200], [3000, 70, 2047], [n * 37 % 700 for n in range(128)]])
+@pytest.mark.parametrize("window,kept", [(1, 0), (1, 1), (5, 4), (64, 64), (100, 3), (70, 130), (4096, 4)])
+def test_single_tokens_cut_by_pages(ops, nh, nkv, hd, lengths, window, kept):
+    """By pages, whatever the sizes; then with infinities and NaN where a query sees them, and where it does not."""
+    case = Case([(n, 1) for n in lengths], nh, nkv, hd, window, kept, BF16, seed=hd + window + len(lengths))
+    case.check(case.run(ops, by_pages=True))
+    if len(lengths) > 16:
+        return
+    for b, n in enumerate(lengths):
+        for j, what in ((2, math.inf), (n // 2, math.nan), (n - 70, -math.inf), (n - 101, math.inf)):
+            if 0 <= j < n and case.place(b, j)[0] != len(case.k) - 1:
+                case.v[case.place(b, j)[0], 0, :3, j % 64] = what
+                if kept <= j <= n - window:                      # (a key that is not seen too)
+                    case.k[case.place(b, j)[0], :, j % 64] = math.nan
+    case.check(case.run(ops, by_pages=True))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nh,nkv,hd", [(4, 2, 80), (24, 2, 128), (140, 1, 64)])
+def test_single_tokens_that_are_not_served_by_pages(ops, nh, nkv, hd):
+    case = Case([(200, 1), (70, 1)], nh, nkv, hd, 90, 4, BF16, seed=1)
+    assert torch.equal(case.run(ops, by_pages=True), case.run(ops, by_pages=False))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("by_pages", [True, False])
+@pytest.mark.parametrize("planes", [0, 1, 2, 3])
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 64), (8, 2, 128), (8, 1, 128)])
+@pytest.mark.parametrize("window,kept", [(1, 1), (64, 64), (100, 3), (70, 130), (4096, 4)])
+def test_from_the_projection(ops, nh, nkv, hd, window, kept, planes, by_pages):
+    """The step that makes queries, keys and values of the joined projection's rows: the new ones arrive in the cache, nothing else is touched."""
+    lengths = [0, 1, 63, 64, 300, 65, 500, 129, 1000]
+    case = Case([(n, 1) for n in lengths], nh, nkv, hd, window, kept, BF16, seed=window + planes)
+    k, v, B = case.k.clone(), case.v.clone(), len(lengths)
+    new_k, new_v = torch.zeros(B, nkv, hd, dtype=BF16), torch.zeros(B, nkv, hd, dtype=BF16)
+    for b, n in enumerate(lengths):
+        page, at = case.place(b, n)
+        new_k[b], new_v[b] = k[page, :, at], v[page, :, :, at]
+        k[page, :, at], v[page, :, :, at] = math.nan, math.nan
+    rows = torch.cat([case.q, new_k.flatten(1), new_v.flatten(1)], 1)
+    if planes:                                                   # of which all but one are nothing: the sum is exact
+        rows = torch.stack([rows.float() if p == planes // 2 else torch.zeros(rows.shape) for p in range(planes)])
+    i = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    k_dev, v_dev = k.to(DEV), v.to(DEV)
+    got = ops.attention_decode_fused(rows.to(DEV), k_dev, v_dev, case.table.to(DEV), i(case.slots), i(lengths), nh, nkv, hd, hd ** -0.5, window, 3, kept=kept,
+                                     pages=by_pages)
+    case.check(got.cpu())
+    bits = lambda t: t.cpu().view(torch.int16)
+    assert torch.equal(bits(k_dev), bits(case.k)) and torch.equal(bits(v_dev), bits(case.v))
+
+
+@pytest.mark.gpu
+def test_a_captured_step_cut_by_pages_replays_with_new_contents(ops):
+    starts = [500, 70, 1500, 0, 64, 900]
+    cases = [Case([(n, 1) for n in starts], 8, 2, 128, 300, 4, BF16, seed=s) for s in (8, 9)]
+    i = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    held = [t.to(DEV) for t in (cases[0].q, cases[0].k, cases[0].v, cases[0].table)] + [i(cases[0].slots), i(starts), i([1] * 6), i(cases[0].cu)]
+    args = (1, 1501, 8, 2, 128, 128 ** -0.5, 300, 4)
+    ops.attention_kept(*held, *args, by_pages=True)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            graphs.append((graph, ops.attention_kept(*held, *args, by_pages=True)))
+    for turn in range(4):
+        now = cases[turn % 2]
+        for t, new in zip(held, (now.q, now.k, now.v, now.table, torch.tensor(now.slots, dtype=torch.int32))):
+            t.copy_(new.to(DEV))
+        for graph, out in graphs:
+            graph.replay()
+            torch.cuda.synchronize()
+            now.check(out.cpu())
+        now.check(ops.attention_kept(*held, *args, by_pages=True).cpu())
+
+
 PLANS = [(False, 1, 1), (False, 2, 1), (False, 1, 3), (False, 2, 5), (False, 1, 16), (False, 2, 2), (True, 0, 1)]
 
 
@@ -278,3 +359,22 @@ def test_slices_fill_the_chip_and_leave_no_wave_without_a_page(ops):
     assert n(1, 1, 1 << 24, 32, 8, 1 << 24, 0) == 64            # 8 blocks, 512 wanted
     assert n(64, 1, 5001, 32, 8, 2048, 4) == 1
     assert n(1, 2000, 2000, 32, 8, 2048, 4) == 1
+
+
+def test_large_steps_of_single_tokens_are_cut_by_pages(ops):
+    assert not ops.kept_by_pages(1, 8, 128, 5000) and not ops.kept_by_pages(64, 8, 128, 400) and not ops.kept_by_pages(3, 2, 64, 1 << 15)
+    assert ops.kept_by_pages(48, 8, 128, 4224) and ops.kept_by_pages(64, 8, 64, 1000) and ops.kept_by_pages(1, 8, 128, 1 << 20)
+
+
+def test_a_steps_way_is_chosen_from_the_keys_that_its_sequences_see(ops, monkeypatch):
+    """Of a windowed layer with first positions: the window's and those, not the sequences' lengths."""
+    from palm_infra_amd.parts.attention import Attention
+    asked = []
+    monkeypatch.setattr(ops, "decode_pages_pays", lambda *a: asked.append(a) or True)
+    part = object.__new__(Attention)
+    part.dtype, part.hd, part.nh, part.nkv, part.window, part.kept = BF16, 128, 8, 2, 100, 30
+    assert part.decode_form([5, 400], 512)
+    assert asked == [([6, 130], 8, 2, 128, 130)]
+    part.window, part.kept = None, 0
+    part.decode_form([5, 400], 512)
+    assert asked[1] == ([6, 401], 8, 2, 128, 512)
