@@ -308,4 +308,8 @@ def call(lib: ctypes.CDLL, fn_name: str, *args) -> None:
     recorder = profile.active()
     rc = fn(*args) if recorder is None else recorder.around(fn_name, lambda: fn(*args))
     if rc != 0:
-        raise KernelError(f"{fn_name}: {lib.palm_last_error().decode(errors='replace')}")
+        failed(lib, fn_name)
+
+
+def failed(lib: ctypes.CDLL, fn_name: str) -> None:
+    raise KernelError(f"{fn_name}: {lib.palm_last_error().decode(errors='replace')}")

@@ -2962,9 +2962,9 @@ def attention_kept(q: torch.Tensor, k_cache, v_cache, block_table, seq_slot, seq
                      _p(out), kept, 1)
             return out
         n_slices = decode_slices(B, nh, nkv, keys)
-        work = torch.empty((B * nh * n_slices * (hd + 4),), dtype=F32, device=q.device) if n_slices > 1 else None
-        _call_on(q.get_device(), lib, "palm_attention_decode_kept", _p(q), _p(k_cache), _p(v_cache), _p(block_table), block_table.shape[1], _p(seq_slot),
-                 _p(seq_start), B, nh, nkv, hd, float(scale), window, n_slices, _p(work), _p(out), kept)
+        work = q.new_empty(2 * B * nh * n_slices * (hd + 4)) if n_slices > 1 else None         # (twice as many of half the size)
+        _call_on(dev, lib, "palm_attention_decode_kept", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), block_table.shape[1],
+                 seq_slot.data_ptr(), seq_start.data_ptr(), B, nh, nkv, hd, float(scale), window, n_slices, _p(work), out.data_ptr(), kept)
         return out
     wide, halves, slices = plan or kept_plan(n, B, max(max_new, max_total), nh, nkv, hd, window, kept)
     if wide:
@@ -3040,8 +3040,14 @@ def _kept_keys(max_total: int, window: int, kept: int) -> int:
 # ---- pages of the cache copied to other pages (library ``pages``) ----------------------------------------------------
 
 def _call_on(device, lib, fn_name: str, *args) -> None:
-    """``library.call`` with ``device`` (or its number) current, on torch's current stream there."""
-    if (device if device.__class__ is int else device.index) == torch._C._cuda_getDevice():
+    """``library.call`` with ``device`` (or its number) current, on torch's current stream there.  (Small calls are as long as the host takes: the
+    usual case is written out here, 0.5 us less.)"""
+    index = device if device.__class__ is int else device.index
+    if index == torch._C._cuda_getDevice():
+        if profile._active is None:
+            if getattr(lib, fn_name)(torch._C._cuda_getCurrentRawStream(index), *args) != 0:
+                library.failed(lib, fn_name)
+            return
         library.call(lib, fn_name, _stream(), *args)
         return
     with torch.cuda.device(device):
@@ -3055,22 +3061,28 @@ def _host_ints(what: str, name: str, values) -> array:
         raise KernelError(f"{what}: {name} is no list of whole numbers ({e})") from None
 
 
-def _copy(what: str, storages, layers: int, pages: int, page_tokens: int, src, dst, tokens) -> None:
-    """``storages``: (tensor, runs of a page, elements of a run, elements a position) each."""
-    s, d = _host_ints(what, "src", src), _host_ints(what, "dst", dst)
-    t = None if tokens is None else _host_ints(what, "tokens", tokens)
+_NO_STORAGE = (None, 0, 0, 0)
+
+
+def _copy(what: str, first, second, layers: int, pages: int, page_tokens: int, src, dst, tokens) -> None:
+    """``first``, ``second``: (tensor, runs of a page, bytes of a run, bytes a position), the second one None if there is one storage only."""
+    try:
+        s, d, t = array("i", src), array("i", dst), None if tokens is None else array("i", tokens)
+    except (TypeError, OverflowError):
+        s, d = _host_ints(what, "src", src), _host_ints(what, "dst", dst)
+        t = None if tokens is None else _host_ints(what, "tokens", tokens)
     if len(s) != len(d) or (t is not None and len(t) != len(s)):
         raise KernelError(f"{what}: {len(s)} sources, {len(d)} destinations" + ("" if t is None else f", {len(t)} counts of positions"))
     if len(s) == 0 or layers == 0:
         return
-    args = []
-    for tensor, runs, run, position in storages:
-        if tensor.element_size() not in (2, 4):
-            raise KernelError(f"{what}: elements of {tensor.element_size()} bytes")
-        args += [_p(tensor), runs, run * tensor.element_size(), position * tensor.element_size()]
-    args += [None, 0, 0, 0] * (2 - len(storages))
-    _call_on(storages[0][0].device, pages_lib(), "palm_copy_pages", *args, layers, pages, page_tokens, s.buffer_info()[0], d.buffer_info()[0],
-             None if t is None else t.buffer_info()[0], len(s))
+    tensor, runs, run, position = first
+    if tensor.element_size() not in (2, 4):
+        raise KernelError(f"{what}: elements of {tensor.element_size()} bytes")
+    if run >= 1 << 30 or (second and second[2] >= 1 << 30) or layers * pages >= 1 << 31:
+        raise KernelError(f"{what}: {layers} layers of {pages} pages, {run} bytes together: more than 2^30 bytes or 2^31 pages")
+    other, runs2, run2, position2 = second or _NO_STORAGE
+    _call_on(tensor.get_device(), pages_lib(), "palm_copy_pages", tensor.data_ptr(), runs, run, position, None if other is None else other.data_ptr(), runs2, run2,
+             position2, layers, pages, page_tokens, s.buffer_info()[0], d.buffer_info()[0], None if t is None else t.buffer_info()[0], len(s))
 
 
 def copy_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, src, dst, tokens=None) -> None:
@@ -3078,6 +3090,20 @@ def copy_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, src, dst, tokens=No
     pages, kv heads, head size, 64] (head counts and sizes of its own, if it has).  ``tokens[i]``: of the page's first so many positions (None: of all);
     the destination's positions behind them stay as they are.  ``src``, ``dst``, ``tokens`` are lists on the host, as a page table has them.
     A page may go to several others; one that is written twice, or both read and written, is refused."""
+    shape, v_shape, dtype = k_cache.shape, v_cache.shape, k_cache.dtype
+    # (looked at one by one only where something is wrong, see attention_kept)
+    if not (k_cache.is_cuda and k_cache.get_device() == v_cache.get_device() and k_cache.is_contiguous() and v_cache.is_contiguous() and dtype is v_cache.dtype
+            and dtype in _CODES and len(shape) == 5 and shape[3] == PAGE_TOKENS and len(v_shape) == 5 and v_shape[4] == PAGE_TOKENS and v_shape[0] == shape[0]
+            and v_shape[1] == shape[1] and k_cache.numel() > 0 and v_cache.numel() > 0):
+        _refuse_pages(k_cache, v_cache)
+    layers, pages, heads, _, hd = shape
+    size = 2 if dtype is BF16 else 4
+    _copy("copy_pages", (k_cache, heads, PAGE_TOKENS * hd * size, hd * size), (v_cache, v_shape[2] * v_shape[3], PAGE_TOKENS * size, size), layers, pages, PAGE_TOKENS,
+          src, dst, tokens)
+
+
+def _refuse_pages(k_cache, v_cache) -> None:
+    """Says what ``copy_pages`` does not take of these."""
     what = "copy_pages"
     _dev(what, k_cache, v_cache)
     for t in (k_cache, v_cache):
@@ -3088,9 +3114,6 @@ def copy_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, src, dst, tokens=No
             and v_cache.numel() > 0):
         raise KernelError(f"{what}: values {tuple(v_cache.shape)} {v_cache.dtype} are not [layers, pages, heads, size, {PAGE_TOKENS}] of the keys' "
                           f"{tuple(k_cache.shape)} {k_cache.dtype} (values are kept transposed)")
-    layers, pages, heads, _, hd = k_cache.shape
-    _copy(what, [(k_cache, heads, PAGE_TOKENS * hd, hd), (v_cache, v_cache.shape[2] * v_cache.shape[3], PAGE_TOKENS, 1)], layers, pages, PAGE_TOKENS,
-          src, dst, tokens)
 
 
 def copy_rows(data: torch.Tensor, src, dst, tokens=None) -> None:
@@ -3099,8 +3122,8 @@ def copy_rows(data: torch.Tensor, src, dst, tokens=None) -> None:
     _dev(what, data)
     if not (data.dim() >= 3 and data.shape[2] == PAGE_TOKENS and data.numel() > 0):
         raise KernelError(f"{what}: rows {tuple(data.shape)} are not [layers, pages, {PAGE_TOKENS}, ..]")
-    row = data[0, 0, 0].numel()
-    _copy(what, [(data, 1, PAGE_TOKENS * row, row)], data.shape[0], data.shape[1], PAGE_TOKENS, src, dst, tokens)
+    row = data[0, 0, 0].numel() * data.element_size()
+    _copy(what, (data, 1, PAGE_TOKENS * row, row), None, data.shape[0], data.shape[1], PAGE_TOKENS, src, dst, tokens)
 
 
 def copy_states(data: torch.Tensor, src, dst) -> None:
@@ -3109,8 +3132,8 @@ def copy_states(data: torch.Tensor, src, dst) -> None:
     _dev(what, data)
     if not (data.dim() >= 2 and data.numel() > 0):
         raise KernelError(f"{what}: states {tuple(data.shape)} are not [layers, slots, ..]")
-    size = data[0, 0].numel()
-    _copy(what, [(data, 1, size, size)], data.shape[0], data.shape[1], 1, src, dst, None)
+    size = data[0, 0].numel() * data.element_size()
+    _copy(what, (data, 1, size, size), None, data.shape[0], data.shape[1], 1, src, dst, None)
 
 
 # ---- how likely tokens are (library ``logprobs``) ----------------------------------------------------------------------
@@ -3141,13 +3164,12 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
     top = int(top)
     if not (0 <= top <= min(LOGPROBS_MOST, V)):
         raise KernelError(f"{what}: the {top} likeliest of {V} tokens ({LOGPROBS_MOST} at most)")
-    dev = logits.device
-    given = torch.empty((n,), dtype=F32, device=dev) if tokens is not None else None
-    entropy = torch.empty((n,), dtype=F32, device=dev)
-    ids = torch.empty((n, top), dtype=torch.int32, device=dev)
-    best = torch.empty((n, top), dtype=F32, device=dev)
+    given = logits.new_empty(n) if tokens is not None else None
+    entropy, best = logits.new_empty(n), logits.new_empty((n, top))
+    ids = logits.new_empty((n, top), dtype=torch.int32)
     if n:
         needed = _logprobs_work(n, V, top)
-        work = torch.empty((needed,), dtype=torch.uint8, device=dev) if needed else None
-        _call_on(dev, logprobs_lib(), "palm_token_logprobs", _p(logits), n, V, _p(tokens), top, _p(work), needed, _p(given), _p(entropy), _p(ids), _p(best))
+        work = logits.new_empty((needed + 3) // 4) if needed else None
+        _call_on(logits.get_device(), logprobs_lib(), "palm_token_logprobs", logits.data_ptr(), n, V, _p(tokens), top, _p(work), needed, _p(given),
+                 entropy.data_ptr(), ids.data_ptr(), best.data_ptr())
     return given, entropy, ids, best
