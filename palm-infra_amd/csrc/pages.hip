@@ -7,7 +7,7 @@
 // head, values, kept transposed [kv heads, head size, 64], one for each element of a head.  Positions behind those stay as they were.
 //
 // What bounds it: every byte read once and written once for each copy.  A thread takes 16 bytes of a page and writes them to
-// all copies of that page, so a page with many copies is read once.  120 pages of 36 layers (2.26 GB read and written) 370 us, 6.1 TB/s; four chunks
+// two copies of that page.  120 pages of 36 layers (2.26 GB read and written) 370 us, 6.1 TB/s; four chunks
 // a thread 417, blocks of 512 threads 388; a copy of one page's 37 positions 5 us.
 #include "common.h"
 
@@ -20,6 +20,9 @@ PALM_DEFINE_LAST_ERROR()
 constexpr int CP_THREADS = 256;
 constexpr int CP_GROUPS = 160;           // source pages of a launch, and copies: both go with its arguments
 constexpr int CP_COPIES = 256;
+// Copies that a thread writes of what it has read; a page with more is read again by others, from the caches.  us, eight to each of six pages, sixteen to each of three:
+// all of them 106 77, four at once 106 72, two 93 67, one 108 68.
+constexpr int CP_AT_ONCE = 2;
 
 struct Storage {
     char* base;
@@ -27,7 +30,7 @@ struct Storage {
     int runs, run_bytes, token_bytes;
 };
 struct CopyPlan {
-    int src[CP_GROUPS], first[CP_GROUPS + 1], tokens[CP_GROUPS];       // copies first[i] .. first[i + 1] - 1 are of page src[i]
+    int src[CP_GROUPS], first[CP_GROUPS + 1], tokens[CP_GROUPS];       // copies first[i] .. first[i + 1] - 1 are of page src[i], CP_AT_ONCE at most
     int dst[CP_COPIES];
 };
 
@@ -37,12 +40,18 @@ struct CopyPlan {
 constexpr int CP_LINE = 128;
 __host__ __device__ inline int touched_bytes(int used, int run_bytes) { return min(run_bytes, (used + CP_LINE - 1) / CP_LINE * CP_LINE); }
 
-// What is written is not read again soon: marked so, it leaves the caches to what is read (120 whole pages 374 us without, 370 with it, the six pages
-// above 122 and 117).
+// What is written is not read again soon, nor what it replaces: marked so, both leave the caches to what is read (120 whole pages 374 us without, 370 with it, the
+// six pages above 122 without, 117 with the writes marked, 106 with the reads of what they replace, 93 by two copies a thread).
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 __device__ inline void store_past(char* p, uint4 v) { __builtin_nontemporal_store(u32x4{v.x, v.y, v.z, v.w}, reinterpret_cast<u32x4*>(p)); }
 __device__ inline void store_past(char* p, uint32_t v) { __builtin_nontemporal_store(v, reinterpret_cast<uint32_t*>(p)); }
 __device__ inline void store_past(char* p, uint16_t v) { __builtin_nontemporal_store(v, reinterpret_cast<uint16_t*>(p)); }
+__device__ inline uint4 load_past(const uint4* p) {
+    const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+    return make_uint4(v.x, v.y, v.z, v.w);
+}
+__device__ inline uint32_t load_past(const uint32_t* p) { return __builtin_nontemporal_load(p); }
+__device__ inline uint16_t load_past(const uint16_t* p) { return __builtin_nontemporal_load(p); }
 
 template <int BYTES> struct Chunk;
 template <> struct Chunk<16> { using type = uint4; };
@@ -74,10 +83,10 @@ __global__ __launch_bounds__(CP_THREADS) void copy_pages_kernel(Storage first, S
     const int d0 = plan.first[group], d1 = plan.first[group + 1];
     if (__any(rest < BYTES)) {
         T old;                                                         // what the next copy's page holds there
-        if (rest < BYTES) old = *reinterpret_cast<const T*>(at + plan.dst[d0] * s.page_bytes);
+        if (rest < BYTES) old = load_past(reinterpret_cast<const T*>(at + plan.dst[d0] * s.page_bytes));
         for (int d = d0; d < d1; ++d) {
             const T now = rest < BYTES ? first_of(held, old, max(0, rest)) : held;
-            if (d + 1 < d1 && rest < BYTES) old = *reinterpret_cast<const T*>(at + plan.dst[d + 1] * s.page_bytes);
+            if (d + 1 < d1 && rest < BYTES) old = load_past(reinterpret_cast<const T*>(at + plan.dst[d + 1] * s.page_bytes));
             store_past(at + plan.dst[d] * s.page_bytes, now);
         }
     } else {
@@ -114,7 +123,7 @@ static int launch_copies(hipStream_t stream, const Storage& a, const Storage& b,
         for (; done < n && copies < CP_COPIES; ++done) {
             const int i = order[done];
             if (held(i) == 0) continue;
-            if (groups == 0 || plan.src[groups - 1] != src[i] || plan.tokens[groups - 1] != held(i)) {
+            if (groups == 0 || plan.src[groups - 1] != src[i] || plan.tokens[groups - 1] != held(i) || copies - plan.first[groups - 1] == CP_AT_ONCE) {
                 if (groups == CP_GROUPS) break;
                 plan.src[groups] = src[i];
                 plan.tokens[groups] = held(i);
