@@ -131,23 +131,33 @@ struct StepPages {
     int pos[2], slot[2], before[2], total, n_seqs, nkv, kvh, window, max_pages;
     bool writes;
     int kept;
+    const int* __restrict__ cu_new;      // with KEPT, or null: the sequences' rows, of which some have none (a sequence without a query has no page)
+    int row[2];
     __device__ static int of(const int (&v)[2], int b) {                   // b the same in every lane
         const int low = __builtin_amdgcn_readlane(v[0], b % WAVE), high = __builtin_amdgcn_readlane(v[1], b % WAVE);
         return b < WAVE ? low : high;
     }
+    __device__ int row_of(int b) const { return KEPT && cu_new ? of(row, b) : b; }
+    __device__ bool present(int b) const { return !KEPT || begin(b) < begin(b + 1); }
     __device__ int begin(int b) const { return b >= n_seqs ? total : of(before, b); }         // the total behind the last
-    __device__ void read(const int* __restrict__ seq_start, const int* __restrict__ seq_slot, int lane) {
+    __device__ void read(const int* __restrict__ seq_start, const int* __restrict__ seq_slot, const int* __restrict__ seq_new, int lane) {
+        bool here[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             pos[i] = seq_start[min(lane + WAVE * i, n_seqs - 1)];
             slot[i] = seq_slot[min(lane + WAVE * i, n_seqs - 1)];
+            here[i] = lane + WAVE * i < n_seqs;
+            if (KEPT && cu_new) {
+                here[i] = here[i] && seq_new[min(lane + WAVE * i, n_seqs - 1)] > 0;
+                row[i] = cu_new[min(lane + WAVE * i, n_seqs - 1)];
+            }
         }
-        const int n0 = lane < n_seqs ? SeenPages<KEPT>(pos[0], window, writes, kept).n : 0, sum0 = lanes_up_to(n0);
+        const int n0 = here[0] ? SeenPages<KEPT>(pos[0], window, writes, kept).n : 0, sum0 = lanes_up_to(n0);
         before[0] = sum0 - n0;
         total = __builtin_amdgcn_readlane(sum0, WAVE - 1);
         before[1] = total;
         if (n_seqs > WAVE) {
-            const int n1 = lane + WAVE < n_seqs ? SeenPages<KEPT>(pos[1], window, writes, kept).n : 0, sum1 = lanes_up_to(n1);
+            const int n1 = here[1] ? SeenPages<KEPT>(pos[1], window, writes, kept).n : 0, sum1 = lanes_up_to(n1);
             before[1] = total + sum1 - n1;
             total += __builtin_amdgcn_readlane(sum1, WAVE - 1);
         }
@@ -181,7 +191,8 @@ struct PagePlace {
     __device__ void advance(const Step& s) {                          // (there is a next one)
         if (++p < n) return;
         p = 0;
-        ++b;
+        do ++b;
+        while (!s.present(b));
         enter(s);
     }
     __device__ int page() const { return page_of_row<KEPT>(lo - front + p, lo, front); }
@@ -397,7 +408,8 @@ __global__ __launch_bounds__(DP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
     int write_cache, bf16_t* __restrict__ k_cache, bf16_t* __restrict__ v_cache,
     const int* __restrict__ block_table, int max_pages, const int* __restrict__ seq_slot,
     const int* __restrict__ seq_start, int n_seqs, int nh, int nkv, float scale_log2, int window,
-    float* work, int* arrivals, bf16_t* __restrict__ out, int kept, int row_heads) {
+    float* work, int* arrivals, bf16_t* __restrict__ out, int kept, int row_heads,
+    const int* __restrict__ seq_new, const int* __restrict__ cu_new) {
     if constexpr (PAGES_SERVE_HEAD) {
         __shared__ __attribute__((aligned(1024))) char ring[DP_WAVES][DP_RING];
         __shared__ bf16x8 queries[DP_QUERIES][DP_HEADS * CHUNKS];
@@ -414,8 +426,8 @@ __global__ __launch_bounds__(DP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
         const int G = nh / nkv, kvh = blockIdx.y;
         if (wave == DP_WAVES - 1) __builtin_amdgcn_s_setprio(3);             // it makes queries, for which all wait
 
-        StepPages<KEPT> step{block_table, {0, 0}, {0, 0}, {0, 0}, 0, n_seqs, nkv, kvh, window, max_pages, write_cache != 0, kept};
-        step.read(seq_start, seq_slot, lane0);
+        StepPages<KEPT> step{block_table, {0, 0}, {0, 0}, {0, 0}, 0, n_seqs, nkv, kvh, window, max_pages, write_cache != 0, kept, cu_new, {0, 0}};
+        step.read(seq_start, seq_slot, seq_new, lane0);
         const int runs = min((int)gridDim.x, step.total), run = blockIdx.x;
         if (run >= runs) return;
         const EvenCut over_blocks(step.total, runs);
@@ -436,7 +448,7 @@ __global__ __launch_bounds__(DP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
                 const int s = DP_WAVES - 1 - wave, b = seq0 + s, pos = StepPages<KEPT>::of(step.pos, b), lane = made_here(lane0);
                 const bool owner = write_cache && step.begin(b + 1) <= c1;                    // this block has the sequence's last page
                 SequenceQueries<TIN, PLANES> make;
-                make.ask(qkv, plane_stride, q_norm_w, k_norm_w, cos_t, sin_t, b, kvh, G, nh, KEPT ? row_heads : nh + 2 * nkv, lane);
+                make.ask(qkv, plane_stride, q_norm_w, k_norm_w, cos_t, sin_t, step.present(b) ? step.row_of(b) : 0, kvh, G, nh, KEPT ? row_heads : nh + 2 * nkv, lane);
                 const size_t new_page = owner ? step.page_bytes(b, pos / PAGE_TOKENS) / 2 : 0;
                 make.prepare(planes, plane_stride, q_norm_w != nullptr, eps, cos_t != nullptr, owner, G, scale_log2, lane, queries[s],
                              new_key[wave], new_value[s], new_score[s], k_cache + new_page + (size_t)(pos % PAGE_TOKENS) * HD,
@@ -504,7 +516,7 @@ __global__ __launch_bounds__(DP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
                 if (r >= G) return;
                 if (ends && x + 1 - at.n >= piece_from) {                  // all of the sequence: finished
                     const float inv = 1.0f / l;
-                    bf16_t* o = out + ((size_t)at.b * nh + kvh * G + r) * HD;
+                    bf16_t* o = out + ((size_t)step.row_of(at.b) * nh + kvh * G + r) * HD;
 #pragma unroll
                     for (int dt = 0; dt < DTILES; ++dt) {
                         uint2 four;
@@ -606,6 +618,7 @@ __global__ __launch_bounds__(DP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
             for (int i = wave; i < n_here * G; i += DP_WAVES) {
                 const int lane = made_here(lane0), s = i / G, h = i % G, b = seq0 + s;
                 const int from = step.begin(b), to = step.begin(b + 1);
+                if (KEPT && from == to) continue;
                 const int begins = c0 + over_waves.begin(lane % DP_WAVES);   // of the waves' runs, a wave a lane
                 const int wa = __popcll(__ballot(lane < DP_WAVES && begins <= max(from, c0))) - 1;
                 const int we = __popcll(__ballot(lane < DP_WAVES && begins < min(to, c1))) - 1;
@@ -632,7 +645,7 @@ __global__ __launch_bounds__(DP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
 #pragma unroll
                     for (int e = 0; e < PER; ++e) o[e] += wa + k <= we ? v[k][e] * wk : 0.f;
                 }
-                const size_t head = (size_t)b * nh + kvh * G + h;
+                const size_t head = (size_t)step.row_of(b) * nh + kvh * G + h;
                 if (whole) {
 #pragma unroll
                     for (int e = 0; e < PER; ++e) out[head * HD + lane * PER + e] = f32_to_bf16(o[e] / l);
@@ -659,8 +672,8 @@ __global__ __launch_bounds__(DP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
                     const int from = step.begin(b), to = step.begin(b + 1), ba = over_blocks.holder(from), n_rec = over_blocks.holder(to - 1) - ba + 1;
                     if (__builtin_amdgcn_readlane(arrived, k) != n_rec - 1) continue;
                     asm volatile("" ::: "memory");
-                    const size_t head = (size_t)b * nh + kvh * G + h;
-                    if (lane == 0) __hip_atomic_store(arrivals + head, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    const size_t head = (size_t)step.row_of(b) * nh + kvh * G + h;
+                    if (lane == 0) __hip_atomic_store(arrivals + (size_t)b * nh + kvh * G + h, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                     float big = -INFINITY, total = 0.f, sum[PER] = {};
                     for (int k0 = 0; k0 < n_rec; k0 += DP_WAVES) {
                         float rec_ml[DP_WAVES][2], rec_o[DP_WAVES][PER];

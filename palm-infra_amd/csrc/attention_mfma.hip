@@ -270,7 +270,7 @@ constexpr int WORK_O = 4, WORK_STRIDE = HD + WORK_O;
 
 // What a slice's wave leaves: with one slice the output itself, else its record in the workspace (maximum, sum, two
 // floats unused, HD floats of the unnormalised output) for the merge; an empty slice leaves nothing.
-__device__ inline void finish_slice(Columns& c, bool valid, int b, int head, int nh, int slice, int n_slices, bool empty,
+__device__ inline void finish_slice(Columns& c, bool valid, int b, int row, int head, int nh, int slice, int n_slices, bool empty,
                                     int g, float* __restrict__ work, bf16_t* __restrict__ out) {
     float l = c.l;
     l += __shfl_xor(l, 16, WAVE);
@@ -278,7 +278,7 @@ __device__ inline void finish_slice(Columns& c, bool valid, int b, int head, int
     if (!valid) return;
     if (n_slices == 1) {
         const float inv = 1.0f / l;
-        bf16_t* o = out + ((size_t)b * nh + head) * HD;
+        bf16_t* o = out + ((size_t)row * nh + head) * HD;
 #pragma unroll
         for (int dt = 0; dt < DTILES; ++dt) {
             uint2 four;
@@ -306,8 +306,10 @@ __global__ __launch_bounds__(WAVE) DECODE_WAVES_PER_SIMD void attention_decode_k
     const bf16_t* __restrict__ q, const bf16_t* __restrict__ k_cache, const bf16_t* __restrict__ v_cache,
     const int* __restrict__ block_table, int max_pages, const int* __restrict__ seq_slot,
     const int* __restrict__ seq_start, int nh, int nkv, float scale_log2, int window, int n_slices,
-    float* __restrict__ work, bf16_t* __restrict__ out, int kept) {
+    float* __restrict__ work, bf16_t* __restrict__ out, int kept, const int* __restrict__ seq_new, const int* __restrict__ cu_new) {
     const int slice = blockIdx.x, b = blockIdx.z;
+    if (KEPT && seq_new[b] <= 0) return;                // (with KEPT a sequence may have no query; its page table is not looked at)
+    const int row = KEPT ? cu_new[b] : b;
     const int G = nh / nkv, groups = (G + 15) / 16;
     const int kvh = blockIdx.y / groups, qg = blockIdx.y % groups;
     const int lane = threadIdx.x, r = lane % 16, g = lane / 16;
@@ -318,7 +320,7 @@ __global__ __launch_bounds__(WAVE) DECODE_WAVES_PER_SIMD void attention_decode_k
     const bool valid = qg * 16 + r < G;
 
     bf16x8 qv[KSTEPS];
-    load_query(q + ((size_t)b * nh + (valid ? head : 0)) * HD, valid, g, qv);
+    load_query(q + ((size_t)row * nh + (valid ? head : 0)) * HD, valid, g, qv);
     Columns c;
     c.m = -INFINITY;
     c.l = 0.f;
@@ -328,7 +330,7 @@ __global__ __launch_bounds__(WAVE) DECODE_WAVES_PER_SIMD void attention_decode_k
     const int* pages = block_table + (size_t)seq_slot[b] * max_pages;
     Ready ready;
     attend_pages<KEPT>(k_cache, v_cache, pages, nkv, kvh, p0, p1, qv, first, pos, scale_log2, c, r, g, ready, kept, cut.page_lo, cut.front);
-    finish_slice(c, valid, b, head, nh, slice, n_slices, p0 >= p1, g, work, out);
+    finish_slice(c, valid, b, row, head, nh, slice, n_slices, p0 >= p1, g, work, out);
 }
 
 // One wave per (sequence, head): merge the slices in a fixed order.  Lane s holds slice s's maximum and sum, the wave
@@ -343,7 +345,8 @@ __global__ __launch_bounds__(WAVE) DECODE_WAVES_PER_SIMD void attention_decode_k
 template <int AT_ONCE, bool KEPT>
 __global__ __launch_bounds__(WAVE) void attention_merge_kernel(const float* __restrict__ work, int n_slices, int nh,
                                                                const int* __restrict__ seq_start, int window,
-                                                               bf16_t* __restrict__ out, int kept) {
+                                                               bf16_t* __restrict__ out, int kept, const int* __restrict__ seq_new,
+                                                               const int* __restrict__ cu_new) {
     constexpr int PER = (HD + WAVE - 1) / WAVE;
     const float* w = work + (size_t)blockIdx.x * n_slices * WORK_STRIDE;
     const int lane = threadIdx.x;
@@ -359,6 +362,12 @@ __global__ __launch_bounds__(WAVE) void attention_merge_kernel(const float* __re
         }
     };
     ask(0);
+    size_t at = blockIdx.x;                                     // the (row, head) of the result
+    if (KEPT && cu_new) {
+        const int b = blockIdx.x / nh;
+        if (seq_new[b] <= 0) return;
+        at = (size_t)cu_new[b] * nh + blockIdx.x % nh;
+    }
     const int live = SliceCut<KEPT>(seq_start[blockIdx.x / nh], window, n_slices, kept).live;       // as the decode kernels cut the range
     float m = lane < live ? mine.x : -INFINITY, l = 0.f;
     for (int s = lane + WAVE; s < live; s += WAVE) m = fmaxf(m, w[(size_t)s * WORK_STRIDE]);
@@ -384,24 +393,24 @@ __global__ __launch_bounds__(WAVE) void attention_merge_kernel(const float* __re
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         const int d = lane + i * WAVE;
-        if (d < HD) out[(size_t)blockIdx.x * HD + d] = f32_to_bf16(o[i] / l);
+        if (d < HD) out[at * HD + d] = f32_to_bf16(o[i] / l);
     }
 }
 
 // slices read together by the merge: all of a step's where they are few, never more than fit in registers
 template <bool KEPT = false>
 static void launch_merge(hipStream_t stream, const float* work, int n_slices, int n_seqs, int nh, const int* seq_start,
-                         int window, bf16_t* out, int kept = 0) {
-    if (n_slices <= 4) attention_merge_kernel<4, KEPT><<<n_seqs * nh, WAVE, 0, stream>>>(work, n_slices, nh, seq_start, window, out, kept);
-    else if (n_slices <= 8) attention_merge_kernel<8, KEPT><<<n_seqs * nh, WAVE, 0, stream>>>(work, n_slices, nh, seq_start, window, out, kept);
-    else attention_merge_kernel<16, KEPT><<<n_seqs * nh, WAVE, 0, stream>>>(work, n_slices, nh, seq_start, window, out, kept);
+                         int window, bf16_t* out, int kept = 0, const int* seq_new = nullptr, const int* cu_new = nullptr) {
+    if (n_slices <= 4) attention_merge_kernel<4, KEPT><<<n_seqs * nh, WAVE, 0, stream>>>(work, n_slices, nh, seq_start, window, out, kept, seq_new, cu_new);
+    else if (n_slices <= 8) attention_merge_kernel<8, KEPT><<<n_seqs * nh, WAVE, 0, stream>>>(work, n_slices, nh, seq_start, window, out, kept, seq_new, cu_new);
+    else attention_merge_kernel<16, KEPT><<<n_seqs * nh, WAVE, 0, stream>>>(work, n_slices, nh, seq_start, window, out, kept, seq_new, cu_new);
 }
 
 template <bool KEPT = false>
 static int launch_attention_decode(hipStream_t stream, const void* q, const void* k_cache, const void* v_cache,
                                    const int* block_table, int max_pages, const int* seq_slot, const int* seq_start,
                                    int n_seqs, int nh, int nkv, int hd, float scale, int window, int n_slices,
-                                   float* work, void* out, int kept = 0) {
+                                   float* work, void* out, int kept = 0, const int* seq_new = nullptr, const int* cu_new = nullptr) {
     PALM_CHECK(hd == HD, "attention_decode: this library was built for head size %d, not %d", HD, hd);
     PALM_CHECK(n_seqs >= 0 && nh > 0 && nkv > 0 && nh % nkv == 0, "attention_decode: seqs=%d heads=%d kv=%d", n_seqs, nh, nkv);
     PALM_CHECK(n_slices >= 1 && n_slices <= 65535, "attention_decode: %d slices", n_slices);
@@ -413,10 +422,10 @@ static int launch_attention_decode(hipStream_t stream, const void* q, const void
     dim3 grid(n_slices, nkv * groups, n_seqs);
     attention_decode_kernel<KEPT><<<grid, WAVE, 0, stream>>>((const bf16_t*)q, (const bf16_t*)k_cache, (const bf16_t*)v_cache,
                                                             block_table, max_pages, seq_slot, seq_start, nh, nkv, scale * LOG2E,
-                                                            window, n_slices, work, (bf16_t*)out, kept);
+                                                            window, n_slices, work, (bf16_t*)out, kept, seq_new, cu_new);
     PALM_LAUNCHED();
     if (n_slices > 1) {
-        launch_merge<KEPT>(stream, work, n_slices, n_seqs, nh, seq_start, window, (bf16_t*)out, kept);
+        launch_merge<KEPT>(stream, work, n_slices, n_seqs, nh, seq_start, window, (bf16_t*)out, kept, seq_new, cu_new);
         PALM_LAUNCHED();
     }
     return 0;
@@ -430,14 +439,15 @@ PALM_API int palm_attention_decode(hipStream_t stream, const void* q, const void
                                    hd, scale, window, n_slices, work, out);
 }
 
-// The same with the sequence's first `kept` keys visible behind the window (> 0).
+// The same with the sequence's first `kept` keys visible behind the window (> 0).  Sequence b's query is row cu_new[b], if seq_new[b] is one; it has none if that is zero.
 PALM_API int palm_attention_decode_kept(hipStream_t stream, const void* q, const void* k_cache, const void* v_cache,
                                         const int* block_table, int max_pages, const int* seq_slot, const int* seq_start,
                                         int n_seqs, int nh, int nkv, int hd, float scale, int window, int n_slices,
-                                        float* work, void* out, int kept) {
+                                        float* work, void* out, int kept, const int* seq_new, const int* cu_new) {
+    PALM_CHECK(seq_new && cu_new, "attention_decode_kept: the sequences' rows are needed");
     PALM_CHECK(window > 0 && kept >= 0 && kept < 1 << 30, "attention_decode_kept: window=%d kept=%d", window, kept);
     return launch_attention_decode<true>(stream, q, k_cache, v_cache, block_table, max_pages, seq_slot, seq_start, n_seqs, nh, nkv,
-                                         hd, scale, window, n_slices, work, out, kept);
+                                         hd, scale, window, n_slices, work, out, kept, seq_new, cu_new);
 }
 
 // ---- decode with the q/k/v pass folded in -----------------------------------------------------------
@@ -730,7 +740,7 @@ __global__ __launch_bounds__(WAVE) DECODE_WAVES_PER_SIMD void attention_decode_f
         // with a key and value of its own making the step sees the cache up to the position before
         attend_pages<KEPT>(k_cache, v_cache, pages, nkv, kvh, p0, p1, qv, first, write_cache ? pos - 1 : pos, scale_log2, c, r, g, start, kept, cut.page_lo,
                            cut.front);
-        finish_slice(c, valid, b, head, nh, slice, n_slices, p0 >= p1, g, work, out);
+        finish_slice(c, valid, b, b, head, nh, slice, n_slices, p0 >= p1, g, work, out);
     }
 }
 
@@ -816,7 +826,7 @@ template <bool KEPT>
 static int launch_decode_pages(hipStream_t stream, const void* qkv, int qkv_is_planes, int planes, const float* q_norm_w, const float* k_norm_w, float eps,
                                const float* cos_t, const float* sin_t, int rotary_dim, int pairing, int write_cache, void* k_cache, void* v_cache,
                                const int* block_table, int max_pages, const int* seq_slot, const int* seq_start, int n_seqs, int nh, int nkv, int hd,
-                               float scale, int window, float* work, int* arrivals, void* out, int kept, int row_heads) {
+                               float scale, int window, float* work, int* arrivals, void* out, int kept, int row_heads, const int* seq_new, const int* cu_new) {
     PALM_CHECK(hd == HD, "attention_decode_pages: this library was built for head size %d, not %d", HD, hd);
     PALM_CHECK((cos_t == nullptr) == (sin_t == nullptr), "attention_decode_pages: cos and sin tables come together");
     PALM_CHECK(palm_attention_decode_fused_serves(cos_t ? rotary_dim : 0, pairing),
@@ -832,7 +842,7 @@ static int launch_decode_pages(hipStream_t stream, const void* qkv, int qkv_is_p
     const size_t plane_stride = (size_t)n_seqs * (nh + 2 * nkv) * HD;
 #define PALM_PAGES(TIN, P) attention_decode_pages_kernel<TIN, P, KEPT><<<dim3(max(1, DP_BLOCKS / nkv), nkv), DP_THREADS, 0, stream>>>( \
         (const TIN*)qkv, planes, plane_stride, q_norm_w, k_norm_w, eps, cos_t, sin_t, write_cache, (bf16_t*)k_cache, \
-        (bf16_t*)v_cache, block_table, max_pages, seq_slot, seq_start, n_seqs, nh, nkv, scale * LOG2E, window, work, arrivals, (bf16_t*)out, kept, row_heads)
+        (bf16_t*)v_cache, block_table, max_pages, seq_slot, seq_start, n_seqs, nh, nkv, scale * LOG2E, window, work, arrivals, (bf16_t*)out, kept, row_heads, seq_new, cu_new)
     if (!qkv_is_planes) PALM_PAGES(bf16_t, 1);
     else if (planes == 1) PALM_PAGES(float, 1);
     else if (planes == 2) PALM_PAGES(float, 2);
@@ -851,20 +861,21 @@ PALM_API int palm_attention_decode_pages(hipStream_t stream, const void* qkv, in
                                          const int* seq_start, int n_seqs, int nh, int nkv, int hd, float scale,
                                          int window, float* work, int* arrivals, void* out) {
     return launch_decode_pages<false>(stream, qkv, qkv_is_planes, planes, q_norm_w, k_norm_w, eps, cos_t, sin_t, rotary_dim, pairing, write_cache, k_cache, v_cache,
-                                      block_table, max_pages, seq_slot, seq_start, n_seqs, nh, nkv, hd, scale, window, work, arrivals, out, 0, nh + 2 * nkv);
+                                      block_table, max_pages, seq_slot, seq_start, n_seqs, nh, nkv, hd, scale, window, work, arrivals, out, 0, nh + 2 * nkv, nullptr, nullptr);
 }
-// The same with the sequence's first `kept` keys visible behind the window (> 0).  plain: qkv is finished queries [n_seqs, nh hd] and the cache holds
-// their own keys and values already.
+// The same with the sequence's first `kept` keys visible behind the window (> 0).  With cu_new qkv is finished queries' rows of nh hd, sequence b's row cu_new[b] if
+// seq_new[b] is one (it has none if that is zero), and the cache holds their own keys and values already.
 PALM_API int palm_attention_decode_pages_kept(hipStream_t stream, const void* qkv, int qkv_is_planes, int planes,
                                          const float* q_norm_w, const float* k_norm_w, float eps, const float* cos_t,
                                          const float* sin_t, int rotary_dim, int pairing, int write_cache, void* k_cache,
                                          void* v_cache, const int* block_table, int max_pages, const int* seq_slot,
                                          const int* seq_start, int n_seqs, int nh, int nkv, int hd, float scale,
-                                         int window, float* work, int* arrivals, void* out, int kept, int plain) {
+                                         int window, float* work, int* arrivals, void* out, int kept, const int* seq_new, const int* cu_new) {
     PALM_CHECK(window > 0 && kept >= 0 && kept < 1 << 30, "attention_decode_pages: window=%d kept=%d", window, kept);
-    PALM_CHECK(!plain || (!qkv_is_planes && !q_norm_w && !cos_t && !write_cache), "attention_decode_pages: finished queries are rows without norm or rotation");
+    PALM_CHECK((seq_new == nullptr) == (cu_new == nullptr), "attention_decode_pages: the sequences' rows and counts come together");
+    PALM_CHECK(!cu_new || (!qkv_is_planes && !q_norm_w && !cos_t && !write_cache), "attention_decode_pages: finished queries are rows without norm or rotation");
     return launch_decode_pages<true>(stream, qkv, qkv_is_planes, planes, q_norm_w, k_norm_w, eps, cos_t, sin_t, rotary_dim, pairing, write_cache, k_cache, v_cache,
-                                      block_table, max_pages, seq_slot, seq_start, n_seqs, nh, nkv, hd, scale, window, work, arrivals, out, kept, plain ? nh : nh + 2 * nkv);
+                                      block_table, max_pages, seq_slot, seq_start, n_seqs, nh, nkv, hd, scale, window, work, arrivals, out, kept, cu_new ? nh : nh + 2 * nkv, seq_new, cu_new);
 }
 
 // ---- decode without a workspace argument ------------------------------------------------------------

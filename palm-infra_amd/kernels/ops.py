@@ -829,7 +829,7 @@ _ATTENTION_SIGNATURES = {
                                     c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int,
                                     c_int, c_float, c_int, c_void_p, c_void_p, c_void_p],
     "palm_attention_decode_kept": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int,
-                                   c_int, c_int, c_float, c_int, c_int, c_void_p, c_void_p, c_int],
+                                   c_int, c_int, c_float, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p],
     "palm_attention_prefill_kept": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
                                     c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_int, c_void_p, c_int, c_int,
                                     c_int, c_void_p],
@@ -838,7 +838,7 @@ _ATTENTION_SIGNATURES = {
                                          c_int, c_int, c_float, c_int, c_int, c_void_p, c_void_p, c_int],
     "palm_attention_decode_pages_kept": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_int,
                                          c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int,
-                                         c_int, c_float, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int],
+                                         c_int, c_float, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p],
     "palm_attention_decode_pages_serves": [c_int, c_int, c_int, c_int],
     "palm_attention_decode_pages_work": [c_int, c_int],
     "palm_attention_decode_fused_serves": [c_int, c_int],
@@ -1028,7 +1028,7 @@ def attention_decode_fused(qkv, k_cache, v_cache, block_table, seq_slot, seq_sta
                      qkv.shape[0] if as_planes else 1, _p(q_norm_w), _p(k_norm_w), float(eps), _p(cos), _p(sin),
                      int(rotary_dim if cos is not None else 0), int(pairing), int(write_cache), _p(k_cache), _p(v_cache),
                      _p(block_table), block_table.shape[1], _p(seq_slot), _p(seq_start), B, nh, nkv, hd, float(scale),
-                     int(window or 0), _p(work), _p(arrivals), _p(out), *more, *(more and (0,)))
+                     int(window or 0), _p(work), _p(arrivals), _p(out), *more, *(more and (None, None)))
         return out
     work = _slices_workspace(what, work, B, nh, n_slices, hd, qkv.device)
     library.call(attention_lib(hd), "palm_attention_decode_fused_kept" if kept else "palm_attention_decode_fused", _stream(), _p(qkv), int(as_planes),
@@ -2929,7 +2929,7 @@ def attention_kept(q: torch.Tensor, k_cache, v_cache, block_table, seq_slot, seq
 
     q [n, nh hd]; sequence b has seq_new[b] queries (none, if it is zero) from row cu_new[b] on, at positions seq_start[b] and up, whose keys and values are
     in the cache; ``max_new``: the most new tokens of a sequence, or more; ``max_total``: the longest sequence with them, which sizes how the work is
-    cut and nothing else.  Pages that no query of
+    cut and nothing else.  Rows of q behind the last sequence's have no result (what the returned tensor holds there is not set).  Pages that no query of
     the step sees are not read, whatever the page table says of them; what masked places hold (an infinity, a NaN) does not show.
     ``q_prescaled``: see ``attention_prefill``.  ``plan``: (wide, halves, slices), how a prompt goes on the matrix cores (None: ``kept_plan``);
     ``by_pages``: whether a step of single tokens is cut by pages there, where ``decode_pages_serves``, or by slices of every sequence (None: ``kept_by_pages``)."""
@@ -2952,19 +2952,19 @@ def attention_kept(q: torch.Tensor, k_cache, v_cache, block_table, seq_slot, seq
     if n == 0 or B == 0 or max_new == 0:
         return out
     lib = attention_lib(hd)
-    if max_new == 1 and n == B and not q_prescaled:              # (one token each: as many as there are sequences)
+    if max_new == 1 and not q_prescaled:
         keys = _kept_keys(max(1, max_total), window, kept)
         if (kept_by_pages(B, nkv, hd, keys) if by_pages is None else by_pages) and decode_pages_serves(B, nh, nkv, hd, block_table.shape[1]):
             work = torch.empty((lib.palm_attention_decode_pages_work(nh, nkv),), dtype=F32, device=q.device)
             arrivals = torch.zeros((B * nh,), dtype=torch.int32, device=q.device)
             _call_on(dev, lib, "palm_attention_decode_pages_kept", _p(q), 0, 1, None, None, 0.0, None, None, 0, 0, 0, _p(k_cache), _p(v_cache),
                      _p(block_table), block_table.shape[1], _p(seq_slot), _p(seq_start), B, nh, nkv, hd, float(scale), window, _p(work), _p(arrivals),
-                     _p(out), kept, 1)
+                     _p(out), kept, seq_new.data_ptr(), cu_new.data_ptr())
             return out
         n_slices = decode_slices(B, nh, nkv, keys)
         work = q.new_empty(2 * B * nh * n_slices * (hd + 4)) if n_slices > 1 else None         # (twice as many of half the size)
         _call_on(dev, lib, "palm_attention_decode_kept", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), block_table.shape[1],
-                 seq_slot.data_ptr(), seq_start.data_ptr(), B, nh, nkv, hd, float(scale), window, n_slices, _p(work), out.data_ptr(), kept)
+                 seq_slot.data_ptr(), seq_start.data_ptr(), B, nh, nkv, hd, float(scale), window, n_slices, _p(work), out.data_ptr(), kept, seq_new.data_ptr(), cu_new.data_ptr())
         return out
     wide, halves, slices = plan or kept_plan(n, B, max(max_new, max_total), nh, nkv, hd, window, kept)
     if wide:

@@ -182,6 +182,28 @@ def test_single_tokens_cut_by_pages(ops, nh, nkv, hd, lengths, window, kept):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("by_pages", [True, False, None])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 64), (8, 2, 128), (4, 2, 80)])
+@pytest.mark.parametrize("counts", [[1, 0, 1, 0, 1, 1], [0, 0, 1], [1, 0, 0], [0, 0], [0, 1, 1, 1, 0], [n % 3 // 2 for n in range(128)], [int(n == 77) for n in range(128)],
+                                    [int(n % 30 < 12) for n in range(100)]])
+@pytest.mark.parametrize("rows", [0, 1, 200])
+def test_single_tokens_of_some_sequences(ops, nh, nkv, hd, counts, dtype, by_pages, rows):
+    """Sequences without a query (nothing is read of theirs) between the others, and rows behind the last, as many as make one for each sequence or more."""
+    case = Case([(130 * n % 1700 + n, c) for n, c in enumerate(counts)], nh, nkv, hd, 200, 4, dtype, seed=len(counts))
+    q = case.q
+    behind = len(counts) - sum(counts) if rows == 1 else rows
+    case.q = torch.cat([q, torch.full((behind, nh * hd), math.nan, dtype=dtype)])
+    if case.q.shape[0] == 0:
+        return
+    i = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    got = ops.attention_kept(case.q.to(DEV), case.k.to(DEV), case.v.to(DEV), case.table.to(DEV), i(case.slots), i([s for s, _ in case.seqs]), i(counts), i(case.cu), 1,
+                             max(s + n for s, n in case.seqs), nh, nkv, hd, hd ** -0.5, 200, 4, by_pages=by_pages).cpu()
+    case.q = q
+    case.check(got[:q.shape[0]])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("nh,nkv,hd", [(4, 2, 80), (24, 2, 128), (140, 1, 64)])
 def test_single_tokens_that_are_not_served_by_pages(ops, nh, nkv, hd):
     case = Case([(200, 1), (70, 1)], nh, nkv, hd, 90, 4, BF16, seed=1)
