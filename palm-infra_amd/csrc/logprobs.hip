@@ -444,7 +444,11 @@ __global__ __launch_bounds__(TOP ? LP_JOIN_WAVES * WAVE : WAVE) void logprobs_jo
     finish(of_wave(all), lists[0], one, tokens != nullptr, row, top, given, entropy, ids, best, lane);
 }
 
-constexpr int LP_ROWS_APART = 256;               // rows from which each has a block of its own
+// Whether each row has a block of its own: short rows, which a block reads as soon as many waves and their joining kernel do, and as many rows as there are
+// compute units, nearly.  us in a recorded graph / called one by one, slices and a block a row: 16 rows of 4,000, no alternatives 5.7 / 14.9 and 4.2 / 10.9, five 8.9 / 15.5
+// and 6.3 / 11.4; of 16,000, five 10.5 / 15.5 8.6 / 11.5; of 32,000, none 6.1 / 15.0 8.0 / 11.0, five 10.2 / 15.5 11.2 / 11.5; of 50,000, five 10.6 / 15.4 15.5 / 14.8.  100 rows of
+// 151,936, none 16.1 / 15.7 25.1 / 24.4, five 21.6 / 21.1 30.1 / 29.6; 250 none 29.9 / 28.3 28.3 / 27.5, five 40.7 / 39.6 33.4 / 32.6.
+static bool by_row(int rows, int V, int top) { return V <= 32768 || rows >= (top ? 176 : 240); }
 constexpr int LP_WAVES_WANTED = 4096;            // below, slices are as short as it takes for so many waves
 
 static long long tiles_of(int V) { return ((long long)V + LP_TILE - 1) / LP_TILE; }
@@ -460,7 +464,7 @@ static int slices_of(int rows, int V) { return (int)(((long long)V + slice_size(
 
 // Bytes of workspace, 0: none is needed.
 PALM_API long long palm_token_logprobs_work(int rows, int V, int top) {
-    if (rows <= 0 || V <= 0 || rows >= LP_ROWS_APART) return 0;
+    if (rows <= 0 || V <= 0 || by_row(rows, V, top)) return 0;
     return (long long)rows * (slices_of(rows, V) * (long long)sizeof(Sums) + (top ? 4ll * groups_of(V) : 0));
 }
 
@@ -472,7 +476,7 @@ PALM_API int palm_token_logprobs(hipStream_t stream, const float* logits, int ro
     if (rows == 0) return 0;
     PALM_CHECK(work_bytes >= palm_token_logprobs_work(rows, V, top) && (work || work_bytes == 0), "token_logprobs: a workspace of %lld bytes is too small", work_bytes);
     const int span = span_of(V), groups = groups_of(V);
-    if (rows >= LP_ROWS_APART) {
+    if (by_row(rows, V, top)) {
         if (top) logprobs_row_kernel<true><<<rows, LP_ROW_WAVES * WAVE, groups * sizeof(float), stream>>>(logits, V, span, tokens, top, given, entropy, ids, best);
         else logprobs_row_kernel<false><<<rows, LP_ROW_WAVES * WAVE, 0, stream>>>(logits, V, span, tokens, top, given, entropy, ids, best);
         PALM_LAUNCHED();

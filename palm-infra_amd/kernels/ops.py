@@ -1113,8 +1113,9 @@ def wide_prompt_attention(starts, counts, nh: int, nkv: int) -> bool:
 
 def slices_of_step(ctx, nh: int, nkv: int, window: int | None, kept: int = 0) -> int:
     """The slices of a decode step's key ranges: what a recorded step was cut for, else what fills the chip."""
-    keys = _kept_keys(ctx.max_total, window, kept) if kept else min(ctx.max_total, window) if window else ctx.max_total
-    return ctx.decode_slices or decode_slices(ctx.n_seqs, nh, nkv, keys)
+    if kept:
+        return ctx.decode_slices or kept_slices(ctx.n_seqs, nh, nkv, _kept_keys(ctx.max_total, window, kept), 3)
+    return ctx.decode_slices or decode_slices(ctx.n_seqs, nh, nkv, min(ctx.max_total, window) if window else ctx.max_total)
 
 
 def attention(q, k_cache, v_cache, block_table, ctx, nh: int, nkv: int, hd: int, scale: float, window: int | None,
@@ -2961,7 +2962,7 @@ def attention_kept(q: torch.Tensor, k_cache, v_cache, block_table, seq_slot, seq
                      _p(block_table), block_table.shape[1], _p(seq_slot), _p(seq_start), B, nh, nkv, hd, float(scale), window, _p(work), _p(arrivals),
                      _p(out), kept, seq_new.data_ptr(), cu_new.data_ptr())
             return out
-        n_slices = decode_slices(B, nh, nkv, keys)
+        n_slices = kept_slices(B, nh, nkv, keys, 5)
         work = q.new_empty(2 * B * nh * n_slices * (hd + 4)) if n_slices > 1 else None         # (twice as many of half the size)
         _call_on(dev, lib, "palm_attention_decode_kept", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), block_table.shape[1],
                  seq_slot.data_ptr(), seq_start.data_ptr(), B, nh, nkv, hd, float(scale), window, n_slices, _p(work), out.data_ptr(), kept, seq_new.data_ptr(), cu_new.data_ptr())
@@ -2976,6 +2977,18 @@ def attention_kept(q: torch.Tensor, k_cache, v_cache, block_table, seq_slot, seq
              _p(seq_start), _p(seq_new), _p(cu_new), B, max_new, nh, nkv, hd, float(scale), window, int(bool(q_prescaled)), max_total, int(halves),
              _p(out), kept, n, int(slices), _p(work))
     return out
+
+
+def kept_slices(n_seqs: int, nh: int, nkv: int, keys: int, whole: int) -> int:
+    """Into how many slices a step of single tokens cuts rows of up to ``keys`` keys: none up to ``whole`` pages, or ten where there are waves enough without;
+    else what fills the chip.  A page more in a wave's walk is 1.1 us, slices a second launch of 2.2 to 3 us, and 3.7 us of the host.  us in a recorded graph / called one
+    by one, by ``decode_slices`` and by one: 32 heads of 128 on 8, one sequence of 3 pages 7.0 / 13.3 and 7.0 / 9.7, of 5 7.2 / 13.5 and 9.3 / 9.7, of 6 7.2 / 13.5 10.5 / 10.0,
+    of 8 7.1 / 13.5 12.8 / 12.3; 30 of 2 pages 9.6 / 13.5 7.8 / 9.5, of 5 15.0 / 14.1 12.0 / 11.2, of 10 19.8 / 19.1 18.8 / 18.1; 64 of 3 16.7 / 15.8 12.1 / 11.4, of 10
+    32.7 / 31.8 32.0 / 31.8; 16 heads of 64 on 4, 30 of 5 7.8 / 13.4 8.3 / 9.6, 64 of 8 12.3 / 13.5 12.3 / 11.5."""
+    pages = -(-keys // PAGE_TOKENS)
+    if pages <= whole or (pages <= 10 and n_seqs * nkv * -(-nh // nkv // 16) >= 240):
+        return 1
+    return decode_slices(n_seqs, nh, nkv, keys)
 
 
 def kept_by_pages(n_seqs: int, nkv: int, hd: int, keys: int) -> bool:

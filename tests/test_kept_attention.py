@@ -400,3 +400,9 @@ def test_a_steps_way_is_chosen_from_the_keys_that_its_sequences_see(ops, monkeyp
     part.window, part.kept = None, 0
     part.decode_form([5, 400], 512)
     assert asked[1] == ([6, 401], 8, 2, 128, 512)
+
+
+def test_short_rows_of_single_tokens_are_not_cut(ops):
+    assert ops.kept_slices(1, 32, 8, 3 * 64, 3) == 1 and ops.kept_slices(1, 32, 8, 3 * 64 + 1, 3) == 4 and ops.kept_slices(1, 32, 8, 5 * 64, 5) == 1
+    assert ops.kept_slices(30, 32, 8, 640, 3) == 1 and ops.kept_slices(30, 32, 8, 641, 3) == ops.decode_slices(30, 32, 8, 641)
+    assert ops.kept_slices(1, 160, 1, 320, 3) == 5 and ops.kept_slices(24, 160, 1, 320, 3) == 1

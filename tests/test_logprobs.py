@@ -87,6 +87,31 @@ def test_against_64_bits(ops, n, V, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["random", "rounded", "equal", "masked", "lowest"])
+@pytest.mark.parametrize("n,V", [(1, 32768), (7, 20001), (1, 32769), (5, 33001), (100, 40000), (175, 32769), (176, 32769), (239, 32770), (240, 32769)])
+def test_by_slices_and_a_block_for_each_row(ops, n, V, kind):
+    """At both sides of where the one begins and the other ends."""
+    x = logits(n, V, n + V, kind)
+    tokens = torch.randint(0, V, (n,), generator=torch.Generator().manual_seed(1), dtype=torch.int32)
+    for top in (0, 5, 64):
+        check(ops, x, tokens, top)
+
+
+@pytest.mark.gpu
+def test_rows_that_are_none_by_slices(ops):
+    x = logits(6, 60000, 3, "random")
+    x[0] = -math.inf
+    x[1, 59999] = math.nan
+    x[2, 5] = math.inf
+    x[3, :1024] = -math.inf
+    x[4, 700:] = -math.inf
+    tokens = torch.tensor([0, 1, 5, 0, 1999, -1], dtype=torch.int32)
+    check(ops, x, tokens, 20)
+    given, entropy, ids, best = ops.token_logprobs(x.to(DEV), tokens.to(DEV), 3)
+    assert given[3] == -math.inf and given[4] == -math.inf and bool(given[5].isnan()) and bool(entropy[:3].isnan().all()) and bool(best[:3].isnan().all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n", [5, 300])
 def test_rows_that_are_none(ops, n):
     x = logits(n, 2000, 3, "random")
