@@ -3102,7 +3102,8 @@ def copy_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, src, dst, tokens=No
     """Keys and values of page ``src[i]`` to page ``dst[i]``, in all layers: k_cache [layers, pages, kv heads, 64, head size], v_cache [layers,
     pages, kv heads, head size, 64] (head counts and sizes of its own, if it has).  ``tokens[i]``: of the page's first so many positions (None: of all);
     the destination's positions behind them stay as they are.  ``src``, ``dst``, ``tokens`` are lists on the host, as a page table has them.
-    A page may go to several others; one that is written twice, or both read and written, is refused."""
+    A page may go to several others; one that is written twice, or both read and written, is refused.  Nothing else may write to a destination page
+    meanwhile, not behind ``tokens[i]`` either: whole lines of memory are written, with what they held."""
     shape, v_shape, dtype = k_cache.shape, v_cache.shape, k_cache.dtype
     # (looked at one by one only where something is wrong, see attention_kept)
     if not (k_cache.is_cuda and k_cache.get_device() == v_cache.get_device() and k_cache.is_contiguous() and v_cache.is_contiguous() and dtype is v_cache.dtype

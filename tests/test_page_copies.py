@@ -133,3 +133,14 @@ def test_refusals(ops, monkeypatch):
     with pytest.raises(ops.KernelError, match="elements of 8 bytes"):
         ops.copy_states(torch.zeros(2, 3, dtype=torch.float64), [0], [1])
     ops.copy_pages(k, v, [], [])
+
+
+def test_pages_and_states_too_large_are_refused(ops, monkeypatch):
+    """Sizes go to the library as 32-bit numbers."""
+    monkeypatch.setattr(ops, "_dev", lambda what, *tensors: None)
+    with pytest.raises(ops.KernelError, match="more than 2\\^30 bytes"):
+        ops.copy_states(torch.empty(1, 2, 1 << 28, device="meta"), [0], [1])
+    with pytest.raises(ops.KernelError, match="more than 2\\^30 bytes"):
+        ops.copy_rows(torch.empty(1, 2, 64, 1 << 23, dtype=BF16, device="meta"), [0], [1])
+    with pytest.raises(ops.KernelError, match="2\\^31 pages"):
+        ops.copy_states(torch.empty(1 << 16, 1 << 16, 1, device="meta"), [0], [1])
