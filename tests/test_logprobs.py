@@ -112,6 +112,23 @@ def test_rows_that_are_none_by_slices(ops):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["random", "rounded", "masked"])
+@pytest.mark.parametrize("n,V", [(1, 262143), (2, 262145), (3, 400001), (1, 1500007), (180, 151936), (180, 262144), (241, 262145), (177, 300001)])
+def test_large_vocabularies(ops, n, V, kind):
+    """Groups of more than 16 logits, and as many of them as a block holds; some of the rows are looked at."""
+    some = sorted({0, n // 2, n - 1})
+    x = torch.randn(n, V, generator=torch.Generator().manual_seed(V))
+    x[some] = logits(len(some), V, n, kind)
+    tokens = torch.randint(0, V, (n,), generator=torch.Generator().manual_seed(1), dtype=torch.int32)
+    x_dev, t_dev = x.to(DEV), tokens.to(DEV)
+    for top in (0, 20, 64):
+        given, entropy, ids, best = [t[some].cpu() for t in ops.token_logprobs(x_dev, t_dev, top)]
+        w_given, w_entropy, w_ids, w_best, _ = plain(x[some], tokens[some], top)
+        assert near(given, w_given, V) and near(entropy, w_entropy, V, 17.0) and near(best, w_best, V)
+        assert torch.equal(ids.long(), w_ids)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n", [5, 300])
 def test_rows_that_are_none(ops, n):
     x = logits(n, 2000, 3, "random")
