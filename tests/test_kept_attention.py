@@ -281,6 +281,24 @@ def test_every_way_a_prompt_goes(ops, nh, nkv, hd, window, kept, plan):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 64), (8, 2, 128), (5, 1, 128), (6, 2, 20), (4, 2, 80)])
+@pytest.mark.parametrize("seqs", [[(1500, 1), (90, 1)], [(700, 130), (0, 65), (200, 1)], [(0, 400)]])
+@pytest.mark.parametrize("max_new,max_total", [(0, 0), (0, 5000), (300, 0)])
+def test_the_longest_sequence_sizes_the_work_only(ops, nh, nkv, hd, seqs, dtype, max_new, max_total):
+    """Too small or too large a longest sequence, and more new tokens than any sequence has."""
+    case = Case(seqs, nh, nkv, hd, 333, 70, dtype, seed=hd)
+    width = 80
+    table = torch.full((case.table.shape[0], width), len(case.k) - 1, dtype=torch.int32)
+    table[:, :case.table.shape[1]] = case.table
+    i = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    most = max(n for _, n in seqs)
+    got = ops.attention_kept(case.q.to(DEV), case.k.to(DEV), case.v.to(DEV), table.to(DEV), i(case.slots), i([s for s, _ in seqs]), i([n for _, n in seqs]), i(case.cu),
+                             most + max_new, max_total, nh, nkv, hd, hd ** -0.5, 333, 70).cpu()
+    case.check(got)
+
+
+@pytest.mark.gpu
 def test_prescaled_queries(ops):
     """Queries that carry scale and log2 e already, rounded with them: as the step hands them over."""
     case = Case([(0, 60), (500, 37)], 8, 2, 128, 90, 4, BF16, seed=2)
