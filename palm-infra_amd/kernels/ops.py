@@ -2892,10 +2892,10 @@ def attention_kept_exact(q: torch.Tensor, k_cache, v_cache, block_table, seq_slo
     if n == 0 or B == 0 or max_new == 0:
         return out
     slices = _kept_slices(B, max_new, max(max_new, max_total), nh, nkv, window, kept)
-    work = torch.empty((n * nh * slices * (hd + 4),), dtype=F32, device=q.device) if slices > 1 else None
-    _call_on(q.get_device(), attention_kept_lib(), "palm_attention_kept", _p(q), _code(q, "attention_kept q"), _p(k_cache), _p(v_cache), _p(block_table),
-             block_table.shape[1], _p(seq_slot), _p(seq_start), _p(seq_new), _p(cu_new), B, n, int(max_new), nh, nkv, hd, float(scale), window, kept,
-             slices, _p(work), _p(out))
+    work = q.new_empty(n * nh * slices * (hd + 4), dtype=F32) if slices > 1 else None
+    _call_on(q.get_device(), attention_kept_lib(), "palm_attention_kept", q.data_ptr(), _code(q, "attention_kept q"), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
+             block_table.shape[1], seq_slot.data_ptr(), seq_start.data_ptr(), seq_new.data_ptr(), cu_new.data_ptr(), B, n, int(max_new), nh, nkv, hd, float(scale), window, kept,
+             slices, _p(work), out.data_ptr())
     return out
 
 
@@ -2972,10 +2972,10 @@ def attention_kept(q: torch.Tensor, k_cache, v_cache, block_table, seq_slot, seq
         _call_on(q.get_device(), lib, "palm_attention_prefill_wide_kept", _p(q), _p(k_cache), _p(v_cache), _p(block_table), block_table.shape[1], _p(seq_slot),
                  _p(seq_start), _p(seq_new), _p(cu_new), B, max_new, nh, nkv, hd, float(scale), window, int(bool(q_prescaled)), _p(out), kept)
         return out
-    work = torch.empty((n * nh * slices * (hd + 4),), dtype=F32, device=q.device) if slices > 1 else None
-    _call_on(q.get_device(), lib, "palm_attention_prefill_kept", _p(q), _p(k_cache), _p(v_cache), _p(block_table), block_table.shape[1], _p(seq_slot),
-             _p(seq_start), _p(seq_new), _p(cu_new), B, max_new, nh, nkv, hd, float(scale), window, int(bool(q_prescaled)), max_total, int(halves),
-             _p(out), kept, n, int(slices), _p(work))
+    work = q.new_empty(2 * n * nh * slices * (hd + 4)) if slices > 1 else None
+    _call_on(dev, lib, "palm_attention_prefill_kept", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), block_table.shape[1],
+             seq_slot.data_ptr(), seq_start.data_ptr(), seq_new.data_ptr(), cu_new.data_ptr(), B, max_new, nh, nkv, hd, float(scale), window, int(bool(q_prescaled)),
+             max_total, int(halves), out.data_ptr(), kept, n, int(slices), _p(work))
     return out
 
 
