@@ -266,10 +266,10 @@ __global__ __launch_bounds__(KA_WAVES * WAVE) __attribute__((amdgpu_waves_per_eu
     if (wave > 0) return;
 #pragma unroll
     for (int w = 0; w < KA_WAVES - 1; ++w) {
-        const float mw = m_lds[w][lane], top = fmaxf(m, mw);
-        if (mw == -INFINITY) continue;                          // it saw none of the column's keys
+        const float mw = m_lds[w][lane], lw = l_lds[w][lane], top = fmaxf(m, mw);
+        if (mw == -INFINITY && lw == 0.f) continue;             // it saw none of the column's keys (with scores that are all NaN its sum is one, and shows)
         const float mine = exp_weight(m - top), its = exp_weight(mw - top);
-        l = l * mine + l_lds[w][lane] * its;
+        l = l * mine + lw * its;
         m = top;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[dt] = o[dt] * mine + o_lds[w][dt][lane] * its;

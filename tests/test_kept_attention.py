@@ -424,3 +424,42 @@ def test_short_rows_of_single_tokens_are_not_cut(ops):
     assert ops.kept_slices(1, 32, 8, 3 * 64, 3) == 1 and ops.kept_slices(1, 32, 8, 3 * 64 + 1, 3) == 4 and ops.kept_slices(1, 32, 8, 5 * 64, 5) == 1
     assert ops.kept_slices(30, 32, 8, 640, 3) == 1 and ops.kept_slices(30, 32, 8, 641, 3) == ops.decode_slices(30, 32, 8, 641)
     assert ops.kept_slices(1, 160, 1, 320, 3) == 5 and ops.kept_slices(24, 160, 1, 320, 3) == 1
+
+
+def _ways(ops, dtype, hd, single):
+    """Every kernel that serves the step: named, as arguments of ``Case.run``."""
+    ways = [dict(), dict(fn=ops.attention_kept_exact)]
+    if dtype == BF16 and hd in ops.MFMA_HEAD_DIMS:
+        ways += [dict(by_pages=True), dict(by_pages=False)] if single else [dict(plan=p) for p in PLANS if hd == 128 or (hd == 64 and not p[0])]
+    return ways
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 64), (8, 2, 128), (4, 2, 80), (6, 2, 20), (4, 1, 512)])
+@pytest.mark.parametrize("page", range(5))
+def test_keys_that_are_no_numbers_show_wherever_their_page_falls(ops, nh, nkv, hd, dtype, page):
+    """A query that sees a NaN among the keys has NaN, also if all that it sees of a page are such (its own key alone on the page, or the whole page), and whichever
+    wave, slice or block walks over the page; the other kv heads' queries have their numbers."""
+    for seqs in ([(64 * page, 1), (64 * page + 63, 1), (330, 1), (3000, 1)], [(0, 330), (64 * page, 30), (3000, 3)]):
+        case = Case(seqs, nh, nkv, hd, 4096, 4, dtype, seed=page)
+        for b, (start, new) in enumerate(seqs):
+            at = page + 20 if start == 3000 else page
+            case.k[case.place(b, 64 * at)[0], 0] = math.nan
+        assert bool(case.plain()[0].isnan().any(1).all()) or seqs[0][1] > 1
+        for way in _ways(ops, dtype, hd, seqs[0][1] == 1):
+            case.check(case.run(ops, **way))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 64), (8, 2, 128), (4, 2, 80), (6, 2, 20)])
+@pytest.mark.parametrize("kept", [0, 3, 67, 130])
+@pytest.mark.parametrize("what", [math.nan, math.inf])
+def test_the_windows_first_key_alone_on_its_page_is_no_number(ops, nh, nkv, hd, dtype, kept, what):
+    """The key 63 of a page is all that the window reaches of it, behind none to three pages of first positions."""
+    start = 64 * 9 + 20
+    case = Case([(start, 1), (start - 20, 1), (40, 1)], nh, nkv, hd, start - (64 * 5 + 63) + 1, kept, dtype, seed=kept)
+    case.k[case.place(0, 64 * 5 + 63)[0], 0, 63] = what
+    for way in _ways(ops, dtype, hd, True):
+        case.check(case.run(ops, **way))
