@@ -107,6 +107,7 @@ static int launch_copies(hipStream_t stream, const Storage& a, const Storage& b,
         mark[src[i]] |= 1;
     }
     for (int i = 0; i < n; ++i) PALM_CHECK(!(mark[dst[i]] & 1), "copy_pages: page %d is both read and written", dst[i]);
+    if (a.page_bytes == 0 && (n_storages < 2 || b.page_bytes == 0)) return 0;       // (a state of no elements: nothing to copy)
     std::vector<int> order(n);
     for (int i = 0; i < n; ++i) order[i] = i;
     auto held = [&](int i) { return tokens ? tokens[i] : page_tokens; };
@@ -165,7 +166,7 @@ PALM_API int palm_copy_pages(hipStream_t stream, void* base0, int runs0, int run
     const int n_storages = base1 ? 2 : 1;
     for (const Storage* s : {&a, &b}) {
         if (s == &b && n_storages < 2) break;
-        PALM_CHECK(s->runs > 0 && s->token_bytes > 0 && (long long)s->token_bytes * page_tokens == s->run_bytes && s->run_bytes % 2 == 0,
+        PALM_CHECK(s->runs > 0 && s->token_bytes >= 0 && (long long)s->token_bytes * page_tokens == s->run_bytes && s->run_bytes % 2 == 0,
                    "copy_pages: %d runs of %d bytes, %d a position", s->runs, s->run_bytes, s->token_bytes);
     }
     if (n == 0 || layers == 0) return 0;

@@ -8,6 +8,7 @@ are memory here; the one computation that torch does on the product path is the 
 from __future__ import annotations
 
 import functools
+import math
 from array import array
 from ctypes import c_float, c_int, c_longlong, c_ulonglong, c_void_p
 from dataclasses import dataclass
@@ -3141,12 +3142,13 @@ def copy_rows(data: torch.Tensor, src, dst, tokens=None) -> None:
 
 
 def copy_states(data: torch.Tensor, src, dst) -> None:
-    """The state of slot ``src[i]`` to slot ``dst[i]``, in all layers: data [layers, slots, *shape]."""
+    """The state of slot ``src[i]`` to slot ``dst[i]``, in all layers: data [layers, slots, *shape].  A state may have no elements (what a convolution of one
+    tap keeps): there is nothing to copy then."""
     what = "copy_states"
     _dev(what, data)
-    if not (data.dim() >= 2 and data.numel() > 0):
+    if data.dim() < 2:
         raise KernelError(f"{what}: states {tuple(data.shape)} are not [layers, slots, ..]")
-    size = data[0, 0].numel() * data.element_size()
+    size = math.prod(data.shape[2:]) * data.element_size()
     _copy(what, (data, 1, size, size), None, data.shape[0], data.shape[1], 1, src, dst, None)
 
 

@@ -144,3 +144,22 @@ def test_pages_and_states_too_large_are_refused(ops, monkeypatch):
         ops.copy_rows(torch.empty(1, 2, 64, 1 << 23, dtype=BF16, device="meta"), [0], [1])
     with pytest.raises(ops.KernelError, match="2\\^31 pages"):
         ops.copy_states(torch.empty(1 << 16, 1 << 16, 1, device="meta"), [0], [1])
+
+
+def test_states_of_no_elements_are_nothing_to_copy(ops, monkeypatch):
+    monkeypatch.setattr(ops, "_dev", lambda what, *tensors: None)
+    monkeypatch.setattr(ops, "_call_on", lambda device, lib, name, *args: ops.library.call(lib, name, None, *args))
+    for shape in ((2, 5, 0, 7), (2, 5, 0), (1, 5, 3, 0)):
+        ops.copy_states(torch.zeros(shape), [0, 0, 4], [1, 2, 3])
+        with pytest.raises(ops.KernelError, match="from page 0 to 5 of 5"):
+            ops.copy_states(torch.zeros(shape), [0], [5])
+        with pytest.raises(ops.KernelError, match="written twice"):
+            ops.copy_states(torch.zeros(shape), [0, 1], [2, 2])
+    with pytest.raises(ops.KernelError, match="are not \\[layers, slots"):
+        ops.copy_states(torch.zeros(0), [0], [1])
+
+
+@pytest.mark.gpu
+def test_states_of_no_elements_on_the_device(ops):
+    ops.copy_states(torch.zeros((3, 4, 0, 6), device=DEV), [0, 0], [1, 3])
+    torch.cuda.synchronize()

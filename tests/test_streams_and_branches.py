@@ -296,3 +296,36 @@ def test_the_command_line(model_dirs):
     assert rc == 0 and out.startswith("[0] total -") and len(out.strip().splitlines()) == 4, err
     rc, out, err = chat("--prompt-ids", "1,2", "--kept", "4")
     assert rc == 1 and "stand behind a window" in err
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("preset", ["tiny-sebesun", "tiny-pazilorn", "tiny-vovalix"])
+def test_branches_of_designs_whose_convolutions_have_one_tap(preset, dtype):
+    """Such a convolution keeps no earlier inputs: its state has no elements."""
+    from palm_infra_amd.config import config_from_dict, preset_dict
+    from palm_infra_amd.engine import Engine, StepEntry
+
+    def one_tap(x):
+        if isinstance(x, dict):
+            return {k: 1 if k == "conv" and v is not None else one_tap(v) for k, v in x.items()}
+        return [one_tap(v) for v in x] if isinstance(x, list) else x
+    eng = Engine.from_config(config_from_dict(one_tap(preset_dict(preset))), seed=2, dtype=dtype, max_tokens=64 * 16)
+    assert any(g.table is None and g.data.numel() == 0 for g in eng.cache.groups)
+    ids = torch.randint(0, eng.vocab_size, (90,), generator=torch.Generator().manual_seed(5)).tolist()
+
+    def run(fork):
+        slot = eng.open()
+        eng.step([StepEntry(slot, ids[:77], [])])
+        if fork:
+            branch, = eng.fork(slot)
+            eng.step([StepEntry(slot, [7], [0])])
+            eng.close(slot)
+            slot = branch
+        out = torch.stack([eng.step([StepEntry(slot, [t], [0])])[0].clone() for t in ids[77:]])
+        eng.close(slot)
+        eng.cache.check()
+        return out
+    assert torch.equal(run(False), run(True))
+    results, _ = eng.generate([ids[:9]], answers=2, temperature=0.0, max_new_tokens=3, ignore_eos=True)
+    assert results[0].token_ids == results[1].token_ids and len(results[0].token_ids) == 3
