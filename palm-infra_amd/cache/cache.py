@@ -339,7 +339,7 @@ class ModelCache:
     def fork(self, slot: int, n: int = 1) -> list[int]:
         """``n`` new sequences that begin as the one in ``slot``, with its length: its full pages are shared, what its last page
         holds and its states are copied, on the current stream.  From then on they are sequences like any other.  Nothing is
-        taken (``CacheFull``) if not all of it fits."""
+        taken (``CacheFull``) if not all of it fits, and nothing is kept if a copy fails."""
         if not self.slots.is_held(slot):
             raise CacheMisuse(f"slot {slot} is forked but not open")
         if n < 1:
@@ -356,14 +356,19 @@ class ModelCache:
                 raise CacheFull(f"{n} branches of slot {slot} need {need} more pages of {PAGE_TOKENS} tokens; "
                                 f"{g.table.pages.free_count} of {g.n_pages} are free")
         new = self.slots.take_many(n)
-        for g in self.groups:
-            if g.table is None:
-                g.copy([slot] * n, new)
-                continue
-            copies = [c for c in (g.table.fork(slot, s, length) for s in new) if c is not None]
-            if copies:
-                g.copy([a for a, _ in copies], [b for _, b in copies], [length % PAGE_TOKENS] * len(copies))
-            g.sync()
+        try:
+            for g in self.groups:
+                if g.table is None:
+                    g.copy([slot] * n, new)
+                    continue
+                copies = [c for c in (g.table.fork(slot, s, length) for s in new) if c is not None]
+                if copies:
+                    g.copy([a for a, _ in copies], [b for _, b in copies], [length % PAGE_TOKENS] * len(copies))
+                g.sync()
+        except BaseException:                                   # a copy that is refused: what was taken goes back
+            for s in new:
+                self.close(s)
+            raise
         for s in new:
             self.lengths[s] = length
         return new

@@ -226,3 +226,46 @@ def test_refusals():
     a = c.open()
     with pytest.raises(CacheMisuse, match="cannot be forked"):
         c.fork(a)
+
+
+@pytest.mark.parametrize("which", range(4))
+@pytest.mark.parametrize("length", [64, 70])
+def test_a_fork_whose_copy_fails_keeps_nothing(which, length):
+    """Whichever storage it is that fails: pages in order, states, rows or a windowed group's pages."""
+    c = make([[KVNeed(2, 8), StateNeed("s", (3,))], [RowsNeed("r", (5,))], [KVNeed(2, 8, 60, kept=3)]])
+    a = c.open()
+    grow(c, a, length)
+    fill(c)
+    before = rows_of_held(c, a)
+    free, group = [g.table.pages.free_count for g in c.paged_groups], c.groups[which]
+
+    def fails(src, dst, tokens=None):
+        raise RuntimeError("no copy")
+    group.copy = fails
+    if group.table is None or length % 64:
+        with pytest.raises(RuntimeError, match="no copy"):
+            c.fork(a, 2)
+        c.check()
+        assert c.slots.held_count == 1 and [g.table.pages.free_count for g in c.paged_groups] == free
+    del group.copy
+    b, d = c.fork(a, 2)
+    c.check()
+    assert all(same(rows_of_held(c, s), before) for s in (a, b, d)) and c.lengths[b] == c.lengths[d] == length
+    for s in (a, b, d):
+        c.close(s)
+    c.check()
+    assert all(g.table.pages.free_count == g.n_pages for g in c.paged_groups)
+
+
+def rows_of_held(c, slot):
+    """``rows_of`` of the groups that keep every position; of the windowed one the positions that it still has."""
+    n, out = c.lengths[slot], []
+    for g in c.groups:
+        if g.table is None:
+            out.append(g.data[:, slot].clone())
+            continue
+        for p in range(n):
+            page = g.table.slot_pages[slot][p // 64]
+            if page >= 0:
+                out += [g.k[:, page, :, p % 64].clone(), g.v[:, page, :, :, p % 64].clone()] if hasattr(g, "k") else [g.data[:, page, p % 64].clone()]
+    return out
