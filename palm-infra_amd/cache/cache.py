@@ -381,9 +381,10 @@ class ModelCache:
             if not hasattr(g, "copy"):
                 raise CacheMisuse(f"pages of {type(g.need).__name__} cannot be moved")
         for g in self.paged_groups:
-            moves = g.table.compact()
+            moves = g.table.moves_to_compact()
             if moves:
                 g.copy([a for a, _ in moves], [b for _, b in moves])
+                g.table.move(moves)                             # (not before the copy: one that fails leaves everything as it was)
                 g.sync()
             moved += len(moves)
         return moved

@@ -172,13 +172,14 @@ class PageTable:
         self.dirty.add(new)
         return copy
 
-    def compact(self) -> list[tuple[int, int]]:
-        """The held pages become the pages numbered lowest, with as few moves as it takes: (page, its new number) each, whose contents
-        are to be moved.  No page is both read and written by them."""
+    def moves_to_compact(self) -> list[tuple[int, int]]:
+        """By which the held pages become the pages numbered lowest, as few as it takes: (page, its new number) each.  The contents are to be
+        moved before the books (``move``): no page is both read and written, and what is written nobody holds yet."""
         n = self.pages.held_count
-        moves = list(zip([p for p in range(n, self.pages.n) if self.pages.is_held(p)], [p for p in range(n) if not self.pages.is_held(p)]))
-        if not moves:
-            return moves
+        return list(zip([p for p in range(n, self.pages.n) if self.pages.is_held(p)], [p for p in range(n) if not self.pages.is_held(p)]))
+
+    def move(self, moves) -> None:
+        """For each (page, its new number): whoever lists the page lists the other one, which holds the same by now."""
         self.pages.exchange(moves)
         for old, new in moves:
             self.users[new], self.users[old] = self.users[old], 0
@@ -187,7 +188,6 @@ class PageTable:
             if any(p in where for p in pages):
                 self.slot_pages[slot] = [where.get(p, p) for p in pages]
                 self.dirty.add(slot)
-        return moves
 
     def check(self) -> None:
         self.pages.check()

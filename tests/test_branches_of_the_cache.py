@@ -269,3 +269,29 @@ def rows_of_held(c, slot):
             if page >= 0:
                 out += [g.k[:, page, :, p % 64].clone(), g.v[:, page, :, :, p % 64].clone()] if hasattr(g, "k") else [g.data[:, page, p % 64].clone()]
     return out
+
+
+@pytest.mark.parametrize("which", range(2))
+def test_pages_whose_copy_fails_stay_where_they_are(which):
+    c = make([[KVNeed(2, 8)], [RowsNeed("r", (5,))]], max_tokens=64 * 20, max_seqs=10)
+    slots = [c.open() for _ in range(4)]
+    for i, s in enumerate(slots):
+        grow(c, s, 60 + 50 * i)
+    fill(c)
+    left = [slots[1], slots[3]] + c.fork(slots[3])
+    for s in (slots[0], slots[2]):
+        c.close(s)
+    before = {s: rows_of(c, s) for s in left}
+    group = c.paged_groups[which]
+
+    def fails(src, dst, tokens=None):
+        raise RuntimeError("no copy")
+    group.copy = fails
+    with pytest.raises(RuntimeError, match="no copy"):
+        c.compact()
+    c.check()
+    assert all(same(rows_of(c, s), before[s]) for s in left)
+    del group.copy
+    assert c.compact() > 0
+    c.check()
+    assert all(same(rows_of(c, s), before[s]) for s in left) and c.compact() == 0
