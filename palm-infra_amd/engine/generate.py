@@ -117,11 +117,12 @@ class GenerationMetrics:
     total_ms: float = 0.0
 
 
-def compute_metrics(results, prefill_ms: float, decode_ms: float) -> GenerationMetrics:
+def compute_metrics(results, prefill_ms: float, decode_ms: float, answers: int = 1) -> GenerationMetrics:
     """The reference's definitions (examples/cli_common.cpp:418-436), summed over the requests of a run:
-    every request's first token comes from the prefill, the others from decode steps."""
+    every request's first token comes from the prefill, the others from decode steps.  Of ``answers`` results of a prompt, one
+    behind the other, the prompt's tokens count once, as they ran."""
     m = GenerationMetrics()
-    m.prompt_tokens = sum(r.prompt_tokens for r in results)
+    m.prompt_tokens = sum(r.prompt_tokens for r in results[::answers])
     m.generated_tokens = sum(len(r.token_ids) for r in results)
     m.decode_tokens = sum(max(len(r.token_ids) - 1, 0) for r in results)
     m.ttft_ms = prefill_ms
@@ -295,7 +296,7 @@ def generate(engine, sampler, prompts, max_new_tokens: int = 2048, stop_token_id
         finally:
             for slot in slots.values():      # only after a fault: every sequence that ended has left already
                 engine.close(slot)
-    return results, compute_metrics(results, total_prefill, total_decode)
+    return results, compute_metrics(results, total_prefill, total_decode, answers)
 
 
 class Conversation:

@@ -270,3 +270,27 @@ def test_slots_come_back_when_a_step_launched_ahead_fails():
     with pytest.raises(RuntimeError, match="boom"):
         generate(eng, StatelessSampler(), [[1, 2], [3]], max_new_tokens=8)
     assert not eng.seen and sorted(eng.closed) == [0, 1]
+
+
+class ForkingEngine(ScriptedEngine):
+    def fork(self, slot, n=1):
+        new = [self.open() for _ in range(n)]
+        for s in new:
+            self.seen[s] = list(self.seen[slot])
+        return new
+
+
+@pytest.mark.parametrize("answers", [1, 2, 3])
+def test_a_prompts_tokens_count_once_however_many_answers(answers):
+    """The prompts run once and take a second between them, 11 tokens in all."""
+    eng = ForkingEngine(lambda seen: 30, n_slots=12)
+    clock = iter([0.0, 1.0] + [2.0] * 20)
+    results, metrics = generate(eng, ArgmaxSampler(), [[1] * 5, [2] * 6], max_new_tokens=3, answers=answers, timer=lambda: next(clock))
+    assert sum(n for step in eng.steps for _, n in step if n > 1) == 11
+    assert metrics.prompt_tokens == 11 and metrics.prefill_tps == 11.0
+    assert metrics.generated_tokens == 6 * answers and metrics.decode_tokens == 4 * answers
+    assert [r.prompt_tokens for r in results] == [5] * answers + [6] * answers
+    # in batches of one prompt each too
+    _, metrics = generate(eng, ArgmaxSampler(), [[1] * 5, [2] * 6], max_new_tokens=3, answers=answers, max_batch=answers)
+    assert metrics.prompt_tokens == 11
+    assert not eng.seen
