@@ -152,14 +152,16 @@ class Engine:
         """Move the pages that sequences hold together; how many were moved (see ``ModelCache.compact``)."""
         return self.cache.compact()
 
-    def held_tokens(self, length: int) -> int:
+    def held_tokens(self, length: int, prompt: int | None = None) -> int:
         """Room in the cache, in tokens, that a sequence takes at most while it grows to ``length``: all of it, or where every layer has a
-        window the window, the first positions that stay, and the piece of a prompt that goes through between two steps."""
+        window the window, the first positions that stay, and the piece of a prompt that goes through between two steps.
+        ``prompt``: so many of its tokens come as a prompt, the others one by one (0: a branch's, which has its prompt behind it; None: all may)."""
         most = 0
         for g in self.cache.paged_groups:
             pages = pages_for(length)
             if g.table.window:
-                pages = min(pages, pages_for(g.table.window + self.step_tokens_least) + 1 + pages_for(g.table.kept))
+                piece = min(length if prompt is None else prompt, self.step_tokens_least)
+                pages = min(pages, pages_for(g.table.window + piece) + 1 + pages_for(g.table.kept))
             most = max(most, pages)
         return (most or pages_for(length)) * PAGE_TOKENS
 

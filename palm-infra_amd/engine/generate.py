@@ -140,8 +140,8 @@ class RequestTooLong(ValueError):
 def plan_batches(prompt_lengths, max_new_tokens: int, max_batch: int, cache_tokens: int, max_seq_tokens: int, answers: int = 1, held_tokens=None):
     """Which requests run together: in the order given, as many as ``max_batch`` allows and as the cache
     can hold when every sequence of the batch grows to its full length (pages of PAGE_TOKENS each;
-    ``held_tokens(length)``: what it takes then, if it is less).  Each request is ``answers`` sequences (that they share their
-    prompt's pages is not counted on).  Returns lists of request indices."""
+    ``held_tokens(length, prompt)``: what it takes then, if it is less, with so many tokens as a prompt).  Each request is ``answers``
+    sequences, of which one runs the prompt (that they share its pages is not counted on).  Returns lists of request indices."""
     if max_batch < 1:
         raise ValueError("max_batch must be at least 1")
     if answers < 1:
@@ -156,7 +156,10 @@ def plan_batches(prompt_lengths, max_new_tokens: int, max_batch: int, cache_toke
             raise RequestTooLong(f"request {i}: a prompt of {n} tokens exceeds the longest sequence the cache takes "
                                  f"({max_seq_tokens})")
         full = min(n + max_new_tokens, max_seq_tokens)
-        need = answers * (held_tokens(full) if held_tokens else pages_for(full) * PAGE_TOKENS)
+        if held_tokens:                      # first the prompts go through, then every sequence grows by single tokens
+            need = max(held_tokens(n, n), answers * held_tokens(full, 0))
+        else:
+            need = answers * pages_for(full) * PAGE_TOKENS
         if need > cache_tokens:
             raise RequestTooLong(f"request {i}: {full} tokens{f' in {answers} sequences' if answers > 1 else ''} do not fit a cache of {cache_tokens}")
         if current and ((len(current) + 1) * answers > max_batch or held + need > cache_tokens):
