@@ -102,37 +102,41 @@ class PagedGroup:
         self.pad_page = n_pages
         self.table_host = torch.full((n_slots + 1, max_pages_per_slot), self.pad_page, dtype=torch.int32)
         self.table_dev = self.table_host.to(device)
-        # Stale rows go to the device through pinned memory, two buffers in turn, each written again only after the
+        # Stale entries go to the device through pinned memory, two buffers in turn, each written again only after the
         # copy that last read it has run: the host never waits for the step that is still running (a step launched
-        # ahead of its predecessor's results would otherwise stop at every page border of every sequence).
+        # ahead of its predecessor's results would otherwise stop at every page border of every sequence).  Of a slot only the places
+        # that changed go: what a token costs does not grow with a stream's length.
         self._pinned = torch.device(device).type == "cuda"
-        self._staging: list = [None, None]           # int32 [rows, pages of a slot + 1]: a slot's pages, then its number
+        self._staging: list = [None, None]           # int64: places in the table, then the pages that they get
         self._staged: list = [None, None]
         self._turn = 0
 
     def sync(self) -> None:
-        """Bring the device's copy of the page lists up to date: all stale rows in one indexed copy, queued on
+        """Bring the device's copy of the page lists up to date: all stale places in one indexed copy, queued on
         the stream like the step that reads them."""
         if not self.table.dirty:
             return
-        slots = sorted(self.table.dirty)
-        k, width = len(slots), self.table_host.shape[1]
+        stale = sorted(self.table.dirty.items())
+        n, width = sum(end - begin for _, (begin, end) in stale), self.table_host.shape[1]
         turn = self._turn = self._turn ^ 1
         if self._staged[turn] is not None:
             self._staged[turn].synchronize()
         buf = self._staging[turn]
-        if buf is None or buf.shape[0] < k:
-            buf = self._staging[turn] = torch.empty((max(k, 16), width + 1), dtype=torch.int32, pin_memory=self._pinned)
-        rows = buf.numpy()[:k]
-        rows[:, :width] = self.pad_page
-        for i, slot in enumerate(slots):
-            pages = self.table.slot_pages[slot]
-            if pages:
-                rows[i, :len(pages)] = np.where(np.asarray(pages, dtype=np.int32) >= 0, pages, self.pad_page)
-            rows[i, width] = slot
-        self.table_host[slots] = buf[:k, :width]
-        up = buf[:k].to(self.table_dev.device, non_blocking=True)
-        self.table_dev.index_copy_(0, up[:, width].long(), up[:, :width])
+        if buf is None or buf.shape[0] < 2 * n:
+            buf = self._staging[turn] = torch.empty((max(4 * n, 256),), dtype=torch.int64, pin_memory=self._pinned)
+        places, pages = buf.numpy()[:n], buf.numpy()[n:2 * n]
+        done = 0
+        for slot, (begin, end) in stale:
+            listed = self.table.slot_pages[slot][begin:end]
+            to = done + end - begin
+            places[done:to] = np.arange(slot * width + begin, slot * width + end)
+            pages[done:to] = -1                                     # (behind a list that has become shorter too)
+            pages[done:done + len(listed)] = listed
+            done = to
+        pages[pages < 0] = self.pad_page
+        self.table_host.numpy().reshape(-1)[places] = pages
+        up = buf[:2 * n].to(self.table_dev.device, non_blocking=True)
+        self.table_dev.view(-1).index_copy_(0, up[:n], up[n:].to(torch.int32))
         if self._pinned:
             self._staged[turn] = torch.cuda.Event()
             self._staged[turn].record()
@@ -265,7 +269,9 @@ class ModelCache:
     def __init__(self, needs: list[list], shares: list[int | None], max_tokens: int, max_seqs: int | None,
                  max_positions: int | None, dtype: torch.dtype, device, page_slack: int = 0, stream_tokens: int | None = None):
         """``stream_tokens``: the longest sequence, also beyond ``max_tokens``, where every layer that keeps positions has a window and so
-        gives pages back as a sequence grows (else, and if None: what ``max_tokens`` and ``max_positions`` allow).
+        gives pages back as a sequence grows (else, and if None: what ``max_tokens`` and ``max_positions`` allow).  The page tables have
+        room for it, 4 bytes for every 64 tokens of every slot; what a token costs does not depend on it, nor on the sequence's length, but a fork, a
+        compaction and the end of a sequence go through its list of pages once.
 
         ``page_slack``: pages beyond those of ``max_tokens``, for a caller whose ``max_tokens`` counts the tokens that
         live sequences hold and not the part of each one's last page that stays empty: one page for each sequence that may

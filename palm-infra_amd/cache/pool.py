@@ -104,7 +104,7 @@ class PageTable:
         self.users = [0] * n_pages                              # slots that list the page
         self._trimmed = [pages_for(self.kept)] * n_slots        # pages of a slot below this one were looked at already
         self.slot_pages: list[list[int]] = [[] for _ in range(n_slots)]
-        self.dirty: set[int] = set()  # slots whose device copy of the list is stale
+        self.dirty: dict[int, tuple[int, int]] = {}   # slots whose device copy of the list is stale, and the places [from, to) of it that are
 
     def pages_needed(self, slot: int, new_length: int) -> int:
         return max(0, pages_for(new_length) - len(self.slot_pages[slot]))
@@ -121,7 +121,12 @@ class PageTable:
             for p in new:
                 self.users[p] = 1
             have.extend(new)
-            self.dirty.add(slot)
+            self._changed(slot, need - len(new), need)
+
+    def _changed(self, slot: int, begin: int, end: int) -> None:
+        if begin < end:
+            was = self.dirty.get(slot, (begin, end))
+            self.dirty[slot] = min(was[0], begin), max(was[1], end)
 
     def _let_go(self, page: int) -> None:
         self.users[page] -= 1
@@ -140,16 +145,16 @@ class PageTable:
             if have[j] >= 0:
                 self._let_go(have[j])
                 have[j] = -1
-                self.dirty.add(slot)
+                self._changed(slot, j, j + 1)
         self._trimmed[slot] = max(self._trimmed[slot], end)
 
     def release(self, slot: int) -> None:
         for p in self.slot_pages[slot]:
             if p >= 0:
                 self._let_go(p)
+        self._changed(slot, 0, len(self.slot_pages[slot]))
         self.slot_pages[slot] = []
         self._trimmed[slot] = pages_for(self.kept)
-        self.dirty.add(slot)
 
     def fork_needs(self, slot: int, length: int) -> int:
         """Pages that a branch of the slot takes of its own: one, if its last page is not full."""
@@ -169,7 +174,7 @@ class PageTable:
                 self.users[p] += 1
         self.slot_pages[new] = pages
         self._trimmed[new] = self._trimmed[slot]
-        self.dirty.add(new)
+        self._changed(new, 0, len(pages))
         return copy
 
     def moves_to_compact(self) -> list[tuple[int, int]]:
@@ -185,9 +190,10 @@ class PageTable:
             self.users[new], self.users[old] = self.users[old], 0
         where = dict(moves)
         for slot, pages in enumerate(self.slot_pages):
-            if any(p in where for p in pages):
-                self.slot_pages[slot] = [where.get(p, p) for p in pages]
-                self.dirty.add(slot)
+            for j, p in enumerate(pages):
+                if p in where:
+                    pages[j] = where[p]
+                    self._changed(slot, j, j + 1)
 
     def check(self) -> None:
         self.pages.check()

@@ -1,10 +1,11 @@
-"""Which streams and answers run together, against the pages that they really hold (the cache's books on the host, no GPU)."""
+"""Which streams and answers run together, against the pages that they really hold, and what a stream's page lists cost (the cache's books on the
+host, no GPU)."""
 import random
 
 import pytest
 import torch
 
-from palm_infra_amd.cache import KVNeed, ModelCache
+from palm_infra_amd.cache import CacheFull, KVNeed, ModelCache
 from palm_infra_amd.engine import Engine
 from palm_infra_amd.engine.generate import RequestTooLong, plan_batches
 
@@ -72,3 +73,70 @@ def test_what_is_planned_together_fits(seed):
         assert b.run([prompts[i] for i in batch], answers, new) * 64 <= need <= b.cache.max_tokens
         planned += batch
     assert planned == list(range(8))
+
+
+def test_a_page_border_costs_the_same_however_long_the_stream_is():
+    """What reaches the device's page table there are the new page and the one given back, not the whole list: the places before the window are never
+    written again."""
+    c = ModelCache([[KVNeed(1, 2, 130, kept=4)]], [None], 64 * 12, 3, None, torch.float32, "cpu", stream_tokens=1 << 22)
+    group, s = c.paged_groups[0], c.open()
+    sent = []
+    real = torch.Tensor.index_copy_
+
+    def counted(self, dim, index, source):
+        sent.append(index.numel())
+        return real(self, dim, index, source)
+    for _ in range(5000):                                       # 320,000 tokens, a page at a time
+        c.reserve([(s, 64)])
+        c.commit([(s, 64)])
+    marked = group.table_dev[s, 1000:4000].clone()
+    group.table_dev[s, 1000:4000] = 7                           # places that were given back long ago
+    torch.Tensor.index_copy_ = counted
+    try:
+        for _ in range(64 * 20):
+            c.reserve([(s, 1)])
+            c.commit([(s, 1)])
+    finally:
+        torch.Tensor.index_copy_ = real
+    assert bool((group.table_dev[s, 1000:4000] == 7).all()) and bool((marked == c.paged_groups[0].pad_page).all())
+    # 20 new pages, and 20 given back
+    assert len(sent) <= 40 and sum(sent) <= 40
+    c.close(s)
+    assert c.lengths[s] == 0
+    group.sync()
+    assert bool((group.table_dev == group.pad_page).all())
+
+
+def test_the_device_has_every_list_as_the_books_have_it():
+    """After any traffic, all of the table: the pages listed, the spare page elsewhere."""
+    rng = random.Random(11)
+    needs = [[KVNeed(1, 4)], [KVNeed(1, 4, 100)], [KVNeed(1, 4, 90, kept=70)]]
+    c = ModelCache(needs, [None] * 3, 64 * 60, 10, 2000, torch.float32, "cpu")
+    live = []
+    for turn in range(500):
+        what = rng.random()
+        try:
+            if what < 0.25:
+                live.append(c.open())
+            elif what < 0.35 and live:
+                live += c.fork(rng.choice(live), rng.randint(1, 2))
+            elif what < 0.5 and live:
+                c.close(live.pop(rng.randrange(len(live))))
+            elif what < 0.55:
+                c.compact()
+            elif live:
+                for _ in range(rng.choice([1, 1, 70])):
+                    s = rng.choice(live)
+                    c.reserve([(s, rng.choice([1, 1, 5, 64, 130]))]) if rng.random() < 0.1 else None     # (room taken and not used)
+                    n = rng.choice([1, 1, 5, 64])
+                    c.reserve([(s, n)])
+                    c.commit([(s, n)])
+        except CacheFull:
+            pass
+        for g in c.paged_groups:
+            g.sync()
+            want = torch.full_like(g.table_dev, g.pad_page)
+            for slot, pages in enumerate(g.table.slot_pages):
+                for j, p in enumerate(pages):
+                    want[slot, j] = p if p >= 0 else g.pad_page
+            assert torch.equal(g.table_dev, want) and torch.equal(g.table_host, want)
