@@ -25,7 +25,7 @@
 // sequences 39.6 and 37.9, one of 100 15.8 and 10.8.  Tried: rings of 16 KB (no change).
 //
 // With KEPT a sequence's first pages stand in front of its window's (SeenPages): 48 sequences of 300 to 9,000 tokens, the last 4,096 and the first 4 seen, 645 MB,
-// 106 us, 6.1 TB/s (by slices 121 and 5 to join them).  Its queries may also come finished (row_heads == nh), their keys in the cache.
+// 106 us, 6.1 TB/s (by slices 121 and 5 to join them).  Its queries may also come finished, their keys in the cache.
 constexpr bool PAGES_SERVE_HEAD = HD == 64 || HD == 128;
 constexpr int DP_WAVES = 8, DP_THREADS = DP_WAVES * WAVE;
 constexpr int DP_BLOCKS = 256;               // one a compute unit
@@ -79,15 +79,18 @@ __device__ __forceinline__ int read_index(const int* p) { return *(const __attri
 
 // The keys of the cache that a new position sees, first .. last, as pages: lo and the n from there on.  With a key of its own making the step sees the
 // cache up to the position before.  A sequence that sees none has one page, all of it hidden, so that it is somebody's.
-// With KEPT the pages of the sequence's first `kept` keys that lie before `lo` stand in front, and count in n.
+// With KEPT the pages of the sequence's first `kept` keys that lie before `lo` stand in front, and count in n.  (What only KEPT has is in structs that are empty
+// without: with members that it does not use the kernel without was compiled another way.)
+template <bool KEPT> struct FrontPages { int front; };
+template <> struct FrontPages<false> { static constexpr int front = 0; };
 template <bool KEPT>
-struct SeenPages {
-    int lo, n, front;
+struct SeenPages : FrontPages<KEPT> {
+    int lo, n;
     __device__ SeenPages(int pos, int window, bool writes, int kept) {
         const int first = window > 0 ? max(0, pos - window + 1) : 0;
         lo = first / PAGE_TOKENS;
-        front = pages_in_front<KEPT>(kept, lo);
-        n = max(writes ? pos - 1 : pos, first) / PAGE_TOKENS - lo + 1 + front;
+        n = max(writes ? pos - 1 : pos, first) / PAGE_TOKENS - lo + 1;
+        if constexpr (KEPT) n += this->front = pages_in_front<KEPT>(kept, lo);
     }
 };
 
@@ -125,39 +128,45 @@ __device__ __forceinline__ float max_of_8(float v) {
 }
 
 // The step's sequences, two a lane (l and l + 64): new position, slot, and the pages of the sequences before.
+template <bool KEPT> struct StepRows {
+    int kept;
+    const int* __restrict__ cu_new;      // or null: the sequences' rows, of which some have none (a sequence without a query has no page)
+    int row[2];
+};
+template <> struct StepRows<false> { static constexpr int kept = 0; };
 template <bool KEPT>
-struct StepPages {
+struct StepPages : StepRows<KEPT> {
     const int* __restrict__ block_table;
     int pos[2], slot[2], before[2], total, n_seqs, nkv, kvh, window, max_pages;
     bool writes;
-    int kept;
-    const int* __restrict__ cu_new;      // with KEPT, or null: the sequences' rows, of which some have none (a sequence without a query has no page)
-    int row[2];
     __device__ static int of(const int (&v)[2], int b) {                   // b the same in every lane
         const int low = __builtin_amdgcn_readlane(v[0], b % WAVE), high = __builtin_amdgcn_readlane(v[1], b % WAVE);
         return b < WAVE ? low : high;
     }
-    __device__ int row_of(int b) const { return KEPT && cu_new ? of(row, b) : b; }
+    __device__ int row_of(int b) const {
+        if constexpr (KEPT) return this->cu_new ? of(this->row, b) : b;
+        else return b;
+    }
     __device__ bool present(int b) const { return !KEPT || begin(b) < begin(b + 1); }
     __device__ int begin(int b) const { return b >= n_seqs ? total : of(before, b); }         // the total behind the last
     __device__ void read(const int* __restrict__ seq_start, const int* __restrict__ seq_slot, const int* __restrict__ seq_new, int lane) {
-        bool here[2];
+        bool missing[2] = {false, false};
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             pos[i] = seq_start[min(lane + WAVE * i, n_seqs - 1)];
             slot[i] = seq_slot[min(lane + WAVE * i, n_seqs - 1)];
-            here[i] = lane + WAVE * i < n_seqs;
-            if (KEPT && cu_new) {
-                here[i] = here[i] && seq_new[min(lane + WAVE * i, n_seqs - 1)] > 0;
-                row[i] = cu_new[min(lane + WAVE * i, n_seqs - 1)];
-            }
+            if constexpr (KEPT)
+                if (this->cu_new) {
+                    missing[i] = seq_new[min(lane + WAVE * i, n_seqs - 1)] <= 0;
+                    this->row[i] = this->cu_new[min(lane + WAVE * i, n_seqs - 1)];
+                }
         }
-        const int n0 = here[0] ? SeenPages<KEPT>(pos[0], window, writes, kept).n : 0, sum0 = lanes_up_to(n0);
+        const int n0 = lane < n_seqs && !missing[0] ? SeenPages<KEPT>(pos[0], window, writes, this->kept).n : 0, sum0 = lanes_up_to(n0);
         before[0] = sum0 - n0;
         total = __builtin_amdgcn_readlane(sum0, WAVE - 1);
         before[1] = total;
         if (n_seqs > WAVE) {
-            const int n1 = here[1] ? SeenPages<KEPT>(pos[1], window, writes, kept).n : 0, sum1 = lanes_up_to(n1);
+            const int n1 = lane + WAVE < n_seqs && !missing[1] ? SeenPages<KEPT>(pos[1], window, writes, this->kept).n : 0, sum1 = lanes_up_to(n1);
             before[1] = total + sum1 - n1;
             total += __builtin_amdgcn_readlane(sum1, WAVE - 1);
         }
@@ -173,9 +182,9 @@ struct StepPages {
 
 // A page of the row: its sequence, and which of the sequence's pages it is.
 template <bool KEPT>
-struct PagePlace {
+struct PagePlace : FrontPages<KEPT> {
     using Step = StepPages<KEPT>;
-    int b, p, n, lo, pos, front;
+    int b, p, n, lo, pos;
     __device__ PagePlace(const Step& s, int x, int lane) {
         b = s.sequence_of(x, lane);
         enter(s);
@@ -186,16 +195,20 @@ struct PagePlace {
         const SeenPages<KEPT> seen(pos, s.window, s.writes, s.kept);
         lo = seen.lo;
         n = seen.n;
-        front = seen.front;
+        if constexpr (KEPT) this->front = seen.front;
     }
     __device__ void advance(const Step& s) {                          // (there is a next one)
         if (++p < n) return;
         p = 0;
-        do ++b;
-        while (!s.present(b));
+        ++b;
+        if constexpr (KEPT)
+            while (!s.present(b)) ++b;
         enter(s);
     }
-    __device__ int page() const { return page_of_row<KEPT>(lo - front + p, lo, front); }
+    __device__ int page() const {
+        if constexpr (KEPT) return page_of_row<KEPT>(lo - this->front + p, lo, this->front);
+        else return lo + p;
+    }
     __device__ size_t bytes(const Step& s) const { return s.page_bytes(b, page()); }
 };
 
@@ -304,16 +317,16 @@ struct SequenceQueries {
     const TIN* row[PASSES];
 
     __device__ void ask(const TIN* __restrict__ qkv, size_t plane_stride, const float* q_norm_w, const float* k_norm_w, const float* cos_t,
-                        const float* sin_t, int b, int kvh, int G, int nh, int row_heads, int lane) {
+                        const float* sin_t, int b, int kvh, int G, int nh, int nkv, bool finished, int lane) {
         const int sub = lane / CHUNKS, ch = lane % CHUNKS;
         const size_t turn = (size_t)b * (HD / 2) + ch % (CHUNKS / 2) * 8;
         cs.read(cos_t ? cos_t + turn : k_norm_w ? k_norm_w : (const float*)qkv);       // (something that is there, where nothing is asked for)
         sn.read(cos_t ? sin_t + turn : k_norm_w ? k_norm_w : (const float*)qkv);
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
-            const int t = min(i * ROWS + sub, row_heads > nh ? G + 1 : G - 1), nkv = (row_heads - nh) / 2;
+            const int t = min(i * ROWS + sub, finished ? G - 1 : G + 1);
             const int head = t < G ? kvh * G + t : t == G ? nh + kvh : nh + nkv + kvh;
-            row[i] = qkv + ((size_t)b * row_heads + head) * HD + ch * 8;
+            row[i] = qkv + ((size_t)b * (finished ? nh : nh + 2 * nkv) + head) * HD + ch * 8;
 #pragma unroll
             for (int pl = 0; pl < HELD; ++pl) raw[i][pl].read(row[i] + pl * plane_stride);
             w[i].read(q_norm_w ? (t < G ? q_norm_w : k_norm_w) + ch * 8 : (const float*)qkv);
@@ -401,16 +414,20 @@ struct SequenceQueries {
     }
 };
 
-template <typename TIN, int PLANES, bool KEPT>
-__global__ __launch_bounds__(DP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) void attention_decode_pages_kernel(
+// (Aligned: 30 KB of code that every call reads anew, and where they lay made 0.13 us of 19.3, 8 sequences of 2,048 tokens, as the code in front of them changed.)
+// With KEPT `more` is a KeptRows.  With its cu_new the rows are finished queries, whose keys the cache has; without, sequence b's row is b.
+template <typename TIN, int PLANES, bool KEPT, typename... More>
+__global__ __launch_bounds__(DP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2), aligned(4096))) void attention_decode_pages_kernel(
     const TIN* __restrict__ qkv, int planes, size_t plane_stride, const float* __restrict__ q_norm_w,
     const float* __restrict__ k_norm_w, float eps, const float* __restrict__ cos_t, const float* __restrict__ sin_t,
     int write_cache, bf16_t* __restrict__ k_cache, bf16_t* __restrict__ v_cache,
     const int* __restrict__ block_table, int max_pages, const int* __restrict__ seq_slot,
     const int* __restrict__ seq_start, int n_seqs, int nh, int nkv, float scale_log2, int window,
-    float* work, int* arrivals, bf16_t* __restrict__ out, int kept, int row_heads,
-    const int* __restrict__ seq_new, const int* __restrict__ cu_new) {
+    float* work, int* arrivals, bf16_t* __restrict__ out, More... more) {
     if constexpr (PAGES_SERVE_HEAD) {
+        KeptRows rows_kept{};
+        if constexpr (KEPT) rows_kept = KeptRows{more...};
+        const auto [kept, seq_new, cu_new] = rows_kept;
         __shared__ __attribute__((aligned(1024))) char ring[DP_WAVES][DP_RING];
         __shared__ bf16x8 queries[DP_QUERIES][DP_HEADS * CHUNKS];
         __shared__ bf16x8 new_key[DP_WAVES][CHUNKS];
@@ -426,7 +443,9 @@ __global__ __launch_bounds__(DP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
         const int G = nh / nkv, kvh = blockIdx.y;
         if (wave == DP_WAVES - 1) __builtin_amdgcn_s_setprio(3);             // it makes queries, for which all wait
 
-        StepPages<KEPT> step{block_table, {0, 0}, {0, 0}, {0, 0}, 0, n_seqs, nkv, kvh, window, max_pages, write_cache != 0, kept, cu_new, {0, 0}};
+        StepRows<KEPT> rows;
+        if constexpr (KEPT) rows = {kept, cu_new, {0, 0}};
+        StepPages<KEPT> step{rows, block_table, {0, 0}, {0, 0}, {0, 0}, 0, n_seqs, nkv, kvh, window, max_pages, write_cache != 0};
         step.read(seq_start, seq_slot, seq_new, lane0);
         const int runs = min((int)gridDim.x, step.total), run = blockIdx.x;
         if (run >= runs) return;
@@ -448,7 +467,7 @@ __global__ __launch_bounds__(DP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
                 const int s = DP_WAVES - 1 - wave, b = seq0 + s, pos = StepPages<KEPT>::of(step.pos, b), lane = made_here(lane0);
                 const bool owner = write_cache && step.begin(b + 1) <= c1;                    // this block has the sequence's last page
                 SequenceQueries<TIN, PLANES> make;
-                make.ask(qkv, plane_stride, q_norm_w, k_norm_w, cos_t, sin_t, step.present(b) ? step.row_of(b) : 0, kvh, G, nh, KEPT ? row_heads : nh + 2 * nkv, lane);
+                make.ask(qkv, plane_stride, q_norm_w, k_norm_w, cos_t, sin_t, step.present(b) ? step.row_of(b) : 0, kvh, G, nh, nkv, KEPT && cu_new, lane);
                 const size_t new_page = owner ? step.page_bytes(b, pos / PAGE_TOKENS) / 2 : 0;
                 make.prepare(planes, plane_stride, q_norm_w != nullptr, eps, cos_t != nullptr, owner, G, scale_log2, lane, queries[s],
                              new_key[wave], new_value[s], new_score[s], k_cache + new_page + (size_t)(pos % PAGE_TOKENS) * HD,
@@ -673,7 +692,7 @@ __global__ __launch_bounds__(DP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
                     if (__builtin_amdgcn_readlane(arrived, k) != n_rec - 1) continue;
                     asm volatile("" ::: "memory");
                     const size_t head = (size_t)step.row_of(b) * nh + kvh * G + h;
-                    if (lane == 0) __hip_atomic_store(arrivals + (size_t)b * nh + kvh * G + h, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    if (lane == 0) __hip_atomic_store(arrivals + (KEPT ? (size_t)b * nh + kvh * G + h : head), 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                     float big = -INFINITY, total = 0.f, sum[PER] = {};
                     for (int k0 = 0; k0 < n_rec; k0 += DP_WAVES) {
                         float rec_ml[DP_WAVES][2], rec_o[DP_WAVES][PER];

@@ -3,7 +3,8 @@
 // (models/qwen3.py:336-341; kernels/attention.cpp:84-217, 937-962): head h reads kv head h / (nh / nkv),
 // keys j <= p of the query's own sequence (j > p - window with a window), softmax in 32-bit with the
 // running maximum, o = sum_j p_j v_j.  With KEPT a query also sees its sequence's first `kept` keys, however far back they lie: the pages
-// that hold them and lie before the window's first page stand in front of it in the row of pages that is walked over.
+// that hold them and lie before the window's first page stand in front of it in the row of pages that is walked over.  PALM_KEPT=1 makes a library
+// of those kernels alone, PALM_KEPT=0 one of the others (in one library, of three times the code, decode steps that never ran them took 0.2 % more).
 //
 // Cache layouts: K [pages, nkv, 64 keys, hd] (a key's row is contiguous); V is kept transposed,
 // [pages, nkv, hd, 64 keys], so that for both products the summed index is contiguous in memory.
@@ -29,6 +30,13 @@
 
 #include <type_traits>
 
+#ifndef PALM_KEPT
+#define PALM_WITH_KEPT 1
+#define PALM_WITHOUT_KEPT 1
+#else
+#define PALM_WITH_KEPT PALM_KEPT
+#define PALM_WITHOUT_KEPT !PALM_KEPT
+#endif
 #ifndef PALM_HEAD_DIM
 #error "compile with -DPALM_HEAD_DIM=<head size>"
 #endif
@@ -95,9 +103,7 @@ template <bool KEPT> __device__ inline int pages_in_front(int kept, int page_lo)
 // The row of pages is numbered so that the window's pages have their own numbers; those in front of page_lo are the sequence's first.
 template <bool KEPT> __device__ inline int page_of_row(int p, int page_lo, int front) { return KEPT && p < page_lo ? p - (page_lo - front) : p; }
 // Whether key `key` is seen: in-page indices of the first and the last key of the window, and of the first key that is not one of the first `kept`.
-template <bool KEPT> __device__ inline bool key_is_seen(int key, int lo, int hi, int kept) {
-    return KEPT ? key <= hi && (key >= lo || key < kept) : key >= lo && key <= hi;
-}
+__device__ inline bool key_is_seen(int key, int lo, int hi, int kept) { return key <= hi && (key >= lo || key < kept); }
 // The same for all keys of a page: bit k for key k.
 __device__ inline uint64_t keys_seen(int lo, int hi, int kept) {
     auto below = [](int n) { return n >= PAGE_TOKENS ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; };
@@ -130,7 +136,9 @@ __device__ inline float score_page(const PageOperands& ops, const bf16x8 (&qv)[K
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int key = tile_key(t, 4 * g + i);
-            const float v = key_is_seen<KEPT>(key, lo, hi, kept) ? s[t][i] * scale_log2 : -INFINITY;
+            float v;
+            if constexpr (KEPT) v = key_is_seen(key, lo, hi, kept) ? s[t][i] * scale_log2 : -INFINITY;
+            else v = (key >= lo && key <= hi) ? s[t][i] * scale_log2 : -INFINITY;
             s[t][i] = v;
             mx = fmaxf(mx, v);
         }
@@ -177,7 +185,7 @@ __device__ inline void blank_values_unseen(PageOperands& ops, int lo, int hi, in
     for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const bool seen = key_is_seen<true>(h * 32 + g * 8 + e, lo, hi, kept);
+            const bool seen = key_is_seen(h * 32 + g * 8 + e, lo, hi, kept);
 #pragma unroll
             for (int dt = 0; dt < DTILES; ++dt) ops.v[dt][h][e] = seen ? ops.v[dt][h][e] : (__bf16)0.0f;
         }
@@ -217,13 +225,15 @@ __device__ inline void attend_pages(const bf16_t* __restrict__ k_cache, const bf
         const size_t next = more ? ((size_t)pages[page_of_row<KEPT>(p + 1, page_lo, front)] * nkv + kvh) * PAGE_TOKENS * HD : base;
         bf16x8 pv[2];
         const int key0 = page_of_row<KEPT>(p, page_lo, front) * PAGE_TOKENS;
-        const float alpha = score_page<KEPT>(ops, qv, first - key0, last - key0, scale_log2, c, g, pv, kept - key0);
+        float alpha;
+        if constexpr (KEPT) alpha = score_page<KEPT>(ops, qv, first - key0, last - key0, scale_log2, c, g, pv, kept - key0);
+        else alpha = score_page(ops, qv, first - p * PAGE_TOKENS, last - p * PAGE_TOKENS, scale_log2, c, g, pv);
         if (more) load_keys(k_cache + next, r, g, ops);
         // (the same in every lane)
         if constexpr (KEPT) {
             if (last - key0 < PAGE_TOKENS - 1 || (first > key0 && kept - key0 < PAGE_TOKENS)) blank_values_unseen(ops, first - key0, last - key0, kept - key0, g);
         } else {
-            if (last - key0 < PAGE_TOKENS - 1) blank_values_after(ops, last - key0, g);
+            if (last - p * PAGE_TOKENS < PAGE_TOKENS - 1) blank_values_after(ops, last - p * PAGE_TOKENS, g);
         }
         weigh_values(ops, pv, alpha, c);
         if (more) load_values(v_cache + next, r, g, ops);
@@ -301,15 +311,25 @@ __device__ inline void finish_slice(Columns& c, bool valid, int b, int row, int 
 #else
 #define DECODE_WAVES_PER_SIMD
 #endif
-template <bool KEPT>
+// What a kernel with KEPT takes beside the others' arguments comes behind them, as `more`; without KEPT it has nothing there.  (Arguments that it does not use
+// took places among those that arrive in registers, and moved the grid's size to another line of memory: 0.2 us for 8 sequences of 2,048 tokens cut by pages.)
+struct KeptRows {
+    int kept;
+    const int *seq_new, *cu_new;
+};
+template <bool KEPT, typename... More>
 __global__ __launch_bounds__(WAVE) DECODE_WAVES_PER_SIMD void attention_decode_kernel(
     const bf16_t* __restrict__ q, const bf16_t* __restrict__ k_cache, const bf16_t* __restrict__ v_cache,
     const int* __restrict__ block_table, int max_pages, const int* __restrict__ seq_slot,
     const int* __restrict__ seq_start, int nh, int nkv, float scale_log2, int window, int n_slices,
-    float* __restrict__ work, bf16_t* __restrict__ out, int kept, const int* __restrict__ seq_new, const int* __restrict__ cu_new) {
+    float* __restrict__ work, bf16_t* __restrict__ out, More... more) {
     const int slice = blockIdx.x, b = blockIdx.z;
-    if (KEPT && seq_new[b] <= 0) return;                // (with KEPT a sequence may have no query; its page table is not looked at)
-    const int row = KEPT ? cu_new[b] : b;
+    int row = b, kept = 0;
+    if constexpr (KEPT) {                               // a sequence may have no query; its page table is not looked at
+        const KeptRows rows{more...};
+        if (rows.seq_new[b] <= 0) return;
+        row = rows.cu_new[b], kept = rows.kept;
+    }
     const int G = nh / nkv, groups = (G + 15) / 16;
     const int kvh = blockIdx.y / groups, qg = blockIdx.y % groups;
     const int lane = threadIdx.x, r = lane % 16, g = lane / 16;
@@ -342,11 +362,10 @@ __global__ __launch_bounds__(WAVE) DECODE_WAVES_PER_SIMD void attention_decode_k
 // shorter one's last records exist but hold what an earlier step left: one sequence of 2,048 tokens in a step
 // recorded for 4,096 fills 33 of 64) and counts as nothing by a select.  (8 sequences, 12 slices: a step of 36 layers
 // 4.04 ms against 4.12 with the reads where they are used.)
-template <int AT_ONCE, bool KEPT>
+template <int AT_ONCE, bool KEPT, typename... More>
 __global__ __launch_bounds__(WAVE) void attention_merge_kernel(const float* __restrict__ work, int n_slices, int nh,
                                                                const int* __restrict__ seq_start, int window,
-                                                               bf16_t* __restrict__ out, int kept, const int* __restrict__ seq_new,
-                                                               const int* __restrict__ cu_new) {
+                                                               bf16_t* __restrict__ out, More... more) {
     constexpr int PER = (HD + WAVE - 1) / WAVE;
     const float* w = work + (size_t)blockIdx.x * n_slices * WORK_STRIDE;
     const int lane = threadIdx.x;
@@ -363,10 +382,15 @@ __global__ __launch_bounds__(WAVE) void attention_merge_kernel(const float* __re
     };
     ask(0);
     size_t at = blockIdx.x;                                     // the (row, head) of the result
-    if (KEPT && cu_new) {
-        const int b = blockIdx.x / nh;
-        if (seq_new[b] <= 0) return;
-        at = (size_t)cu_new[b] * nh + blockIdx.x % nh;
+    int kept = 0;
+    if constexpr (KEPT) {
+        const KeptRows rows{more...};
+        kept = rows.kept;
+        if (rows.cu_new) {                                      // (else sequence b's result is row b)
+            const int b = blockIdx.x / nh;
+            if (rows.seq_new[b] <= 0) return;
+            at = (size_t)rows.cu_new[b] * nh + blockIdx.x % nh;
+        }
     }
     const int live = SliceCut<KEPT>(seq_start[blockIdx.x / nh], window, n_slices, kept).live;       // as the decode kernels cut the range
     float m = lane < live ? mine.x : -INFINITY, l = 0.f;
@@ -401,9 +425,13 @@ __global__ __launch_bounds__(WAVE) void attention_merge_kernel(const float* __re
 template <bool KEPT = false>
 static void launch_merge(hipStream_t stream, const float* work, int n_slices, int n_seqs, int nh, const int* seq_start,
                          int window, bf16_t* out, int kept = 0, const int* seq_new = nullptr, const int* cu_new = nullptr) {
-    if (n_slices <= 4) attention_merge_kernel<4, KEPT><<<n_seqs * nh, WAVE, 0, stream>>>(work, n_slices, nh, seq_start, window, out, kept, seq_new, cu_new);
-    else if (n_slices <= 8) attention_merge_kernel<8, KEPT><<<n_seqs * nh, WAVE, 0, stream>>>(work, n_slices, nh, seq_start, window, out, kept, seq_new, cu_new);
-    else attention_merge_kernel<16, KEPT><<<n_seqs * nh, WAVE, 0, stream>>>(work, n_slices, nh, seq_start, window, out, kept, seq_new, cu_new);
+    auto launch = [&](auto... more) {
+        if (n_slices <= 4) attention_merge_kernel<4, KEPT><<<n_seqs * nh, WAVE, 0, stream>>>(work, n_slices, nh, seq_start, window, out, more...);
+        else if (n_slices <= 8) attention_merge_kernel<8, KEPT><<<n_seqs * nh, WAVE, 0, stream>>>(work, n_slices, nh, seq_start, window, out, more...);
+        else attention_merge_kernel<16, KEPT><<<n_seqs * nh, WAVE, 0, stream>>>(work, n_slices, nh, seq_start, window, out, more...);
+    };
+    if constexpr (KEPT) launch(kept, seq_new, cu_new);
+    else launch();
 }
 
 template <bool KEPT = false>
@@ -420,9 +448,13 @@ static int launch_attention_decode(hipStream_t stream, const void* q, const void
     const int groups = (nh / nkv + 15) / 16;
     PALM_CHECK(nkv * groups <= 65535 && n_seqs <= 65535, "attention_decode: grid too large");
     dim3 grid(n_slices, nkv * groups, n_seqs);
-    attention_decode_kernel<KEPT><<<grid, WAVE, 0, stream>>>((const bf16_t*)q, (const bf16_t*)k_cache, (const bf16_t*)v_cache,
-                                                            block_table, max_pages, seq_slot, seq_start, nh, nkv, scale * LOG2E,
-                                                            window, n_slices, work, (bf16_t*)out, kept, seq_new, cu_new);
+    auto launch = [&](auto... more) {
+        attention_decode_kernel<KEPT><<<grid, WAVE, 0, stream>>>((const bf16_t*)q, (const bf16_t*)k_cache, (const bf16_t*)v_cache,
+                                                                block_table, max_pages, seq_slot, seq_start, nh, nkv, scale * LOG2E,
+                                                                window, n_slices, work, (bf16_t*)out, more...);
+    };
+    if constexpr (KEPT) launch(kept, seq_new, cu_new);
+    else launch();
     PALM_LAUNCHED();
     if (n_slices > 1) {
         launch_merge<KEPT>(stream, work, n_slices, n_seqs, nh, seq_start, window, (bf16_t*)out, kept, seq_new, cu_new);
@@ -431,6 +463,7 @@ static int launch_attention_decode(hipStream_t stream, const void* q, const void
     return 0;
 }
 
+#if PALM_WITHOUT_KEPT
 PALM_API int palm_attention_decode(hipStream_t stream, const void* q, const void* k_cache, const void* v_cache,
                                    const int* block_table, int max_pages, const int* seq_slot, const int* seq_start,
                                    int n_seqs, int nh, int nkv, int hd, float scale, int window, int n_slices,
@@ -438,7 +471,8 @@ PALM_API int palm_attention_decode(hipStream_t stream, const void* q, const void
     return launch_attention_decode(stream, q, k_cache, v_cache, block_table, max_pages, seq_slot, seq_start, n_seqs, nh, nkv,
                                    hd, scale, window, n_slices, work, out);
 }
-
+#endif
+#if PALM_WITH_KEPT
 // The same with the sequence's first `kept` keys visible behind the window (> 0).  Sequence b's query is row cu_new[b], if seq_new[b] is one; it has none if that is zero.
 PALM_API int palm_attention_decode_kept(hipStream_t stream, const void* q, const void* k_cache, const void* v_cache,
                                         const int* block_table, int max_pages, const int* seq_slot, const int* seq_start,
@@ -449,6 +483,7 @@ PALM_API int palm_attention_decode_kept(hipStream_t stream, const void* q, const
     return launch_attention_decode<true>(stream, q, k_cache, v_cache, block_table, max_pages, seq_slot, seq_start, n_seqs, nh, nkv,
                                          hd, scale, window, n_slices, work, out, kept, seq_new, cu_new);
 }
+#endif
 
 // ---- decode with the q/k/v pass folded in -----------------------------------------------------------
 // The same grid and the same slices, but the kernel starts from the joined projection's output (whole rows, or
@@ -680,15 +715,16 @@ struct FromProjection {
     }
 };
 
-template <typename TIN, int PLANES, bool KEPT>
+template <typename TIN, int PLANES, bool KEPT, typename... More>
 __global__ __launch_bounds__(WAVE) DECODE_WAVES_PER_SIMD void attention_decode_fused_kernel(
     const TIN* __restrict__ qkv, int planes, size_t plane_stride, const float* __restrict__ q_norm_w,
     const float* __restrict__ k_norm_w, float eps, const float* __restrict__ cos_t, const float* __restrict__ sin_t,
     int write_cache, bf16_t* __restrict__ k_cache, bf16_t* __restrict__ v_cache,
     const int* __restrict__ block_table, int max_pages, const int* __restrict__ seq_slot,
     const int* __restrict__ seq_start, int nh, int nkv, float scale_log2, int window, int n_slices,
-    float* __restrict__ work, bf16_t* __restrict__ out, int kept) {
+    float* __restrict__ work, bf16_t* __restrict__ out, More... more) {
     if constexpr (FUSED_SERVES_HEAD) {
+        const int kept = (0 + ... + more);
         __shared__ float new_key[HD], new_value[HD];
         const int slice = blockIdx.x, b = blockIdx.z;
         const int G = nh / nkv, groups = (G + 15) / 16;
@@ -774,14 +810,18 @@ static int launch_decode_fused(hipStream_t stream, const void* qkv, int qkv_is_p
     PALM_CHECK(nkv * groups <= 65535 && n_seqs <= 65535, "attention_decode_fused: grid too large");
     dim3 grid(n_slices, nkv * groups, n_seqs);
     const size_t plane_stride = (size_t)n_seqs * (nh + 2 * nkv) * HD;
+    auto launch = [&](auto... more) {
 #define PALM_FUSED(TIN, P) attention_decode_fused_kernel<TIN, P, KEPT><<<grid, WAVE, 0, stream>>>( \
         (const TIN*)qkv, planes, plane_stride, q_norm_w, k_norm_w, eps, cos_t, sin_t, write_cache, (bf16_t*)k_cache, \
-        (bf16_t*)v_cache, block_table, max_pages, seq_slot, seq_start, nh, nkv, scale * LOG2E, window, n_slices, work, (bf16_t*)out, kept)
-    if (!qkv_is_planes) PALM_FUSED(bf16_t, 1);
-    else if (planes == 1) PALM_FUSED(float, 1);
-    else if (planes == 2) PALM_FUSED(float, 2);
-    else PALM_FUSED(float, 0);
+        (bf16_t*)v_cache, block_table, max_pages, seq_slot, seq_start, nh, nkv, scale * LOG2E, window, n_slices, work, (bf16_t*)out, more...)
+        if (!qkv_is_planes) PALM_FUSED(bf16_t, 1);
+        else if (planes == 1) PALM_FUSED(float, 1);
+        else if (planes == 2) PALM_FUSED(float, 2);
+        else PALM_FUSED(float, 0);
 #undef PALM_FUSED
+    };
+    if constexpr (KEPT) launch(kept);
+    else launch();
     PALM_LAUNCHED();
     if (n_slices > 1) {
         launch_merge<KEPT>(stream, work, n_slices, n_seqs, nh, seq_start, window, (bf16_t*)out, kept);
@@ -790,6 +830,7 @@ static int launch_decode_fused(hipStream_t stream, const void* qkv, int qkv_is_p
     return 0;
 }
 
+#if PALM_WITHOUT_KEPT
 PALM_API int palm_attention_decode_fused(hipStream_t stream, const void* qkv, int qkv_is_planes, int planes,
                                          const float* q_norm_w, const float* k_norm_w, float eps, const float* cos_t,
                                          const float* sin_t, int rotary_dim, int pairing, int write_cache, void* k_cache,
@@ -799,6 +840,8 @@ PALM_API int palm_attention_decode_fused(hipStream_t stream, const void* qkv, in
     return launch_decode_fused<false>(stream, qkv, qkv_is_planes, planes, q_norm_w, k_norm_w, eps, cos_t, sin_t, rotary_dim, pairing, write_cache, k_cache, v_cache,
                                       block_table, max_pages, seq_slot, seq_start, n_seqs, nh, nkv, hd, scale, window, n_slices, work, out, 0);
 }
+#endif
+#if PALM_WITH_KEPT
 // The same with the sequence's first `kept` keys visible behind the window (> 0).
 PALM_API int palm_attention_decode_fused_kept(hipStream_t stream, const void* qkv, int qkv_is_planes, int planes,
                                          const float* q_norm_w, const float* k_norm_w, float eps, const float* cos_t,
@@ -810,6 +853,7 @@ PALM_API int palm_attention_decode_fused_kept(hipStream_t stream, const void* qk
     return launch_decode_fused<true>(stream, qkv, qkv_is_planes, planes, q_norm_w, k_norm_w, eps, cos_t, sin_t, rotary_dim, pairing, write_cache, k_cache, v_cache,
                                       block_table, max_pages, seq_slot, seq_start, n_seqs, nh, nkv, hd, scale, window, n_slices, work, out, kept);
 }
+#endif
 
 // ---- decode cut by pages ------------------------------------------------------------------------------
 #include "attention_decode_pages.h"
@@ -826,7 +870,7 @@ template <bool KEPT>
 static int launch_decode_pages(hipStream_t stream, const void* qkv, int qkv_is_planes, int planes, const float* q_norm_w, const float* k_norm_w, float eps,
                                const float* cos_t, const float* sin_t, int rotary_dim, int pairing, int write_cache, void* k_cache, void* v_cache,
                                const int* block_table, int max_pages, const int* seq_slot, const int* seq_start, int n_seqs, int nh, int nkv, int hd,
-                               float scale, int window, float* work, int* arrivals, void* out, int kept, int row_heads, const int* seq_new, const int* cu_new) {
+                               float scale, int window, float* work, int* arrivals, void* out, int kept, const int* seq_new, const int* cu_new) {
     PALM_CHECK(hd == HD, "attention_decode_pages: this library was built for head size %d, not %d", HD, hd);
     PALM_CHECK((cos_t == nullptr) == (sin_t == nullptr), "attention_decode_pages: cos and sin tables come together");
     PALM_CHECK(palm_attention_decode_fused_serves(cos_t ? rotary_dim : 0, pairing),
@@ -840,18 +884,23 @@ static int launch_decode_pages(hipStream_t stream, const void* qkv, int qkv_is_p
     if (n_seqs == 0) return 0;
     PALM_CHECK(work && arrivals, "attention_decode_pages: a workspace and counters are needed");
     const size_t plane_stride = (size_t)n_seqs * (nh + 2 * nkv) * HD;
+    auto launch = [&](auto... more) {
 #define PALM_PAGES(TIN, P) attention_decode_pages_kernel<TIN, P, KEPT><<<dim3(max(1, DP_BLOCKS / nkv), nkv), DP_THREADS, 0, stream>>>( \
         (const TIN*)qkv, planes, plane_stride, q_norm_w, k_norm_w, eps, cos_t, sin_t, write_cache, (bf16_t*)k_cache, \
-        (bf16_t*)v_cache, block_table, max_pages, seq_slot, seq_start, n_seqs, nh, nkv, scale * LOG2E, window, work, arrivals, (bf16_t*)out, kept, row_heads, seq_new, cu_new)
-    if (!qkv_is_planes) PALM_PAGES(bf16_t, 1);
-    else if (planes == 1) PALM_PAGES(float, 1);
-    else if (planes == 2) PALM_PAGES(float, 2);
-    else PALM_PAGES(float, 0);
+        (bf16_t*)v_cache, block_table, max_pages, seq_slot, seq_start, n_seqs, nh, nkv, scale * LOG2E, window, work, arrivals, (bf16_t*)out, more...)
+        if (!qkv_is_planes) PALM_PAGES(bf16_t, 1);
+        else if (planes == 1) PALM_PAGES(float, 1);
+        else if (planes == 2) PALM_PAGES(float, 2);
+        else PALM_PAGES(float, 0);
 #undef PALM_PAGES
+    };
+    if constexpr (KEPT) launch(kept, seq_new, cu_new);
+    else launch();
     PALM_LAUNCHED();
     return 0;
 }
 
+#if PALM_WITHOUT_KEPT
 // palm_attention_decode_fused by the kernel that is cut by pages.  arrivals: n_seqs * nh counters, zero before the call and after it; calls
 // that overlap in time need counters and a workspace of their own.
 PALM_API int palm_attention_decode_pages(hipStream_t stream, const void* qkv, int qkv_is_planes, int planes,
@@ -861,8 +910,10 @@ PALM_API int palm_attention_decode_pages(hipStream_t stream, const void* qkv, in
                                          const int* seq_start, int n_seqs, int nh, int nkv, int hd, float scale,
                                          int window, float* work, int* arrivals, void* out) {
     return launch_decode_pages<false>(stream, qkv, qkv_is_planes, planes, q_norm_w, k_norm_w, eps, cos_t, sin_t, rotary_dim, pairing, write_cache, k_cache, v_cache,
-                                      block_table, max_pages, seq_slot, seq_start, n_seqs, nh, nkv, hd, scale, window, work, arrivals, out, 0, nh + 2 * nkv, nullptr, nullptr);
+                                      block_table, max_pages, seq_slot, seq_start, n_seqs, nh, nkv, hd, scale, window, work, arrivals, out, 0, nullptr, nullptr);
 }
+#endif
+#if PALM_WITH_KEPT
 // The same with the sequence's first `kept` keys visible behind the window (> 0).  With cu_new qkv is finished queries' rows of nh hd, sequence b's row cu_new[b] if
 // seq_new[b] is one (it has none if that is zero), and the cache holds their own keys and values already.
 PALM_API int palm_attention_decode_pages_kept(hipStream_t stream, const void* qkv, int qkv_is_planes, int planes,
@@ -875,9 +926,11 @@ PALM_API int palm_attention_decode_pages_kept(hipStream_t stream, const void* qk
     PALM_CHECK((seq_new == nullptr) == (cu_new == nullptr), "attention_decode_pages: the sequences' rows and counts come together");
     PALM_CHECK(!cu_new || (!qkv_is_planes && !q_norm_w && !cos_t && !write_cache), "attention_decode_pages: finished queries are rows without norm or rotation");
     return launch_decode_pages<true>(stream, qkv, qkv_is_planes, planes, q_norm_w, k_norm_w, eps, cos_t, sin_t, rotary_dim, pairing, write_cache, k_cache, v_cache,
-                                      block_table, max_pages, seq_slot, seq_start, n_seqs, nh, nkv, hd, scale, window, work, arrivals, out, kept, cu_new ? nh : nh + 2 * nkv, seq_new, cu_new);
+                                      block_table, max_pages, seq_slot, seq_start, n_seqs, nh, nkv, hd, scale, window, work, arrivals, out, kept, seq_new, cu_new);
 }
+#endif
 
+#if PALM_WITHOUT_KEPT
 // ---- decode without a workspace argument ------------------------------------------------------------
 // The slices' partial results go through this array instead of a buffer of the caller's.  Each GPU has a copy of
 // its own at an address of its own; in host code the array's name is only a handle for hipGetSymbolAddress, never
@@ -930,6 +983,7 @@ PALM_API int palm_attention_decode_static(hipStream_t stream, const void* q, con
     return launch_attention_decode(stream, q, k_cache, v_cache, block_table, max_pages, seq_slot, seq_start, n_seqs, nh, nkv,
                                    hd, scale, window, n_slices, work, out);
 }
+#endif
 
 // ---- prefill --------------------------------------------------------------------------------------
 // A block of four waves serves one kv head, up to eight query heads of its group (more heads: more blocks)
@@ -1167,7 +1221,9 @@ __device__ inline void unit_scores(const bf16_t* k_lds, Unit (&u)[PF_UNITS], int
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int key = tile_key(t, 4 * g + i);
-                    const float v = key_is_seen<KEPT>(key, lo, hi, kept - page_first_key) ? s[x][t][i] : -INFINITY;
+                    float v;
+                    if constexpr (KEPT) v = key_is_seen(key, lo, hi, kept - page_first_key) ? s[x][t][i] : -INFINITY;
+                    else v = (key >= lo && key <= hi) ? s[x][t][i] : -INFINITY;
                     s[x][t][i] = v;
                     mx = fmaxf(mx, v);
                 }
@@ -1244,12 +1300,13 @@ __device__ inline void unit_values(const bf16_t* v_lds, Unit (&u)[PF_UNITS], int
 #else
 #define PF_WAVES_PER_SIMD
 #endif
-template <bool KEPT>
+template <bool KEPT, typename... More>
 __global__ __launch_bounds__(PF_THREADS) PF_WAVES_PER_SIMD void attention_prefill_kernel(
     const bf16_t* __restrict__ q, const bf16_t* __restrict__ k_cache, const bf16_t* __restrict__ v_cache,
     const int* __restrict__ block_table, int max_pages, const int* __restrict__ seq_slot,
     const int* __restrict__ seq_start, const int* __restrict__ seq_new, const int* __restrict__ cu_new, int nh,
-    int nkv, float scale_log2, int window, int qb, int hg, bf16_t* __restrict__ out, int kept) {
+    int nkv, float scale_log2, int window, int qb, int hg, bf16_t* __restrict__ out, More... more) {
+    const int kept = (0 + ... + more);
     constexpr int K_TILE = PAGE_TOKENS * K_STRIDE, V_TILE = HD * V_STRIDE;
     // Head sizes whose pages fit twice keep two pages of K and of V^T in LDS: while one is used the next is laid
     // down beside it, and one barrier a page is enough.  Larger heads share one buffer between K and V^T.
@@ -1432,7 +1489,7 @@ __global__ __launch_bounds__(PF_THREADS) PF_WAVES_PER_SIMD void attention_prefil
             if (!at_an_edge(key0)) continue;
 #pragma unroll
             for (int x = 0; x < PF_UNITS; ++x)
-                add_wild_values(v_cache + offset_of(p), u[x].c.o, g, [&](int key) { return key_is_seen<true>(key, u[x].first - key0, u[x].pos - key0, kept - key0); });
+                add_wild_values(v_cache + offset_of(p), u[x].c.o, g, [&](int key) { return key_is_seen(key, u[x].first - key0, u[x].pos - key0, kept - key0); });
         }
     }
 #pragma unroll
@@ -1550,7 +1607,7 @@ __device__ __forceinline__ void paired_page(const bf16_t* k_lds, const bf16_t* v
                 for (int i = 0; i < 4; ++i) {
                     const int key = tile_key(t, 4 * g + i);
                     if constexpr (KEPT) s[x][t][i] = if_bit((uint32_t)(seen >> t / 2 * 32), t % 2 * 4 + i, s[x][t][i]);
-                    else s[x][t][i] = key_is_seen<KEPT>(key, lo, hi, kept - page_first_key) ? s[x][t][i] : -INFINITY;
+                    else s[x][t][i] = (key >= lo && key <= hi) ? s[x][t][i] : -INFINITY;
                 }
         }
         float top = s[x][0][0];
@@ -1653,14 +1710,21 @@ struct NthTile {
     }
 };
 
-template <int HALVES, bool PRESCALED, bool KEPT>
+struct KeptPrompt {
+    int kept, slices;
+    float* work;
+    int n_seqs, tiles_most;
+};
+template <int HALVES, bool PRESCALED, bool KEPT, typename... More>
 __global__ __launch_bounds__(HALVES * PF_THREADS) PF_WAVES_PER_SIMD void attention_prefill_paired_kernel(
     const bf16_t* __restrict__ q, const bf16_t* __restrict__ k_cache, const bf16_t* __restrict__ v_cache,
     const int* __restrict__ block_table, int max_pages, const int* __restrict__ seq_slot,
     const int* __restrict__ seq_start, const int* __restrict__ seq_new, const int* __restrict__ cu_new, int nh,
-    int nkv, float scale_log2, int window, int qb, int hg, int partners_follow, bf16_t* __restrict__ out, int kept, int slices,
-    float* __restrict__ work, int n_seqs, int tiles_most) {
+    int nkv, float scale_log2, int window, int qb, int hg, int partners_follow, bf16_t* __restrict__ out, More... more) {
     if constexpr (PF_DMA) {
+        KeptPrompt prompt{};
+        if constexpr (KEPT) prompt = KeptPrompt{more...};
+        const auto [kept, slices, work, n_seqs, tiles_most] = prompt;
         constexpr int K_TILE = PAGE_TOKENS * K_STRIDE, V_TILE = HD * V_STRIDE;
         __shared__ __attribute__((aligned(16))) bf16_t k_lds[HALVES * 2 * K_TILE];
         __shared__ __attribute__((aligned(16))) bf16_t v_lds[HALVES * 2 * V_TILE];
@@ -1695,19 +1759,28 @@ __global__ __launch_bounds__(HALVES * PF_THREADS) PF_WAVES_PER_SIMD void attenti
 
         {
             const int tile_first = tile * qb;                         // the tile's first query, within the step
+            int tile_last, page_lo, front, p_lo, p_hi;
+            bf16_t *k_half, *v_half;
             // the pages any query of the tile sees (the same for all waves)
-            const int tile_last = min(tile_first + qb - 1, n_new - 1);
-            const int row_hi = (start + tile_last) / PAGE_TOKENS;
-            const int page_lo = window > 0 ? max(0, start + tile_first - window + 1) / PAGE_TOKENS : 0;
-            const int front = pages_in_front<KEPT>(kept, page_lo), row_lo = page_lo - front;        // the row of pages, see page_of_row
-            const int per = KEPT ? (row_hi - row_lo + slices) / slices : 0;                         // pages of a slice of it
-            const int p_lo = KEPT ? row_lo + slice * per : row_lo, p_hi = KEPT ? min(row_hi, p_lo + per - 1) : row_hi;
-            // of every HALVES pages in turn each half takes one, into two places of its own
-            bf16_t *k_half = k_lds + half * 2 * K_TILE, *v_half = v_lds + half * 2 * V_TILE;
+            auto cut_pages = [&] {
+                tile_last = min(tile_first + qb - 1, n_new - 1);
+                p_hi = (start + tile_last) / PAGE_TOKENS;
+                page_lo = window > 0 ? max(0, start + tile_first - window + 1) / PAGE_TOKENS : 0;
+                front = 0, p_lo = page_lo;
+                if constexpr (KEPT) {                                 // the row of pages, see page_of_row, and a slice of it
+                    front = pages_in_front<KEPT>(kept, page_lo);
+                    const int row_lo = page_lo - front, per = (p_hi - row_lo + slices) / slices;
+                    p_lo = row_lo + slice * per;
+                    p_hi = min(p_hi, p_lo + per - 1);
+                }
+                // of every HALVES pages in turn each half takes one, into two places of its own
+                k_half = k_lds + half * 2 * K_TILE, v_half = v_lds + half * 2 * V_TILE;
+            };
             auto load_page = [&](int p, int step) {
                 const size_t at = ((size_t)pages[page_of_row<KEPT>(p, page_lo, front)] * nkv + kvh) * PAGE_TOKENS * HD;
                 page_into_lds(k_cache + at, v_cache + at, sources, k_half + step % 2 * K_TILE, v_half + step % 2 * V_TILE);
             };
+            if constexpr (KEPT) cut_pages();
             // (with KEPT the first page is on its way before the queries are asked for)
             if (KEPT && p_lo + half <= p_hi) load_page(p_lo + half, 0);
             PairedUnit u[PF_UNITS];
@@ -1740,6 +1813,7 @@ __global__ __launch_bounds__(HALVES * PF_THREADS) PF_WAVES_PER_SIMD void attenti
 #pragma unroll
                 for (int dt = 0; dt < DTILES; ++dt) u[x].o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
             }
+            if constexpr (!KEPT) cut_pages();
             // is every key of page p visible to every column of this wave?
             auto interior = [&](int key0) -> bool {
                 bool inside = true;
@@ -1779,7 +1853,7 @@ __global__ __launch_bounds__(HALVES * PF_THREADS) PF_WAVES_PER_SIMD void attenti
                 wait_for_all_but_the_youngest_loads<0>();             // the half's next page has landed
                 page_barrier();
             }
-            if (HALVES > 1 && p_lo >= p_hi) {                         // one page: the first half had it
+            if (HALVES > 1 && (KEPT ? p_lo >= p_hi : p_lo == p_hi)) {     // one page: the first half had it
                 if (half == 1) return;
             } else if constexpr (HALVES > 1) {
                 // the second half's sums go through LDS (nobody reads pages any more, none is on its way) to the same lanes of the first
@@ -1819,7 +1893,7 @@ __global__ __launch_bounds__(HALVES * PF_THREADS) PF_WAVES_PER_SIMD void attenti
 #pragma unroll
                     for (int x = 0; x < PF_UNITS; ++x)
                         add_wild_values(v_cache + ((size_t)pages[page] * nkv + kvh) * PAGE_TOKENS * HD, u[x].o, g,
-                                        [&](int key) { return key_is_seen<true>(key, u[x].first - key0, u[x].pos - key0, kept - key0); });
+                                        [&](int key) { return key_is_seen(key, u[x].first - key0, u[x].pos - key0, kept - key0); });
                 }
             }
             if (KEPT && slices > 1) {
@@ -1856,6 +1930,7 @@ __global__ __launch_bounds__(HALVES * PF_THREADS) PF_WAVES_PER_SIMD void attenti
 
 // A wave for each (row, head) of a prompt whose rows of pages were cut: the slices' records in their order.
 constexpr int JOIN_WAVES = 4;
+template <bool KEPT>
 __global__ __launch_bounds__(JOIN_WAVES * WAVE) void attention_prefill_join_kernel(const float* __restrict__ work, int slices, long long heads, bf16_t* __restrict__ out) {
     constexpr int PER = (HD + WAVE - 1) / WAVE;
     const long long head = (long long)blockIdx.x * JOIN_WAVES + threadIdx.x / WAVE;
@@ -1924,13 +1999,14 @@ __device__ __forceinline__ float wide_max(float a, float b, float c) {         /
     return most;
 }
 
-template <bool PRESCALED, bool KEPT>
+template <bool PRESCALED, bool KEPT, typename... More>
 __global__ __launch_bounds__(PF_THREADS) __attribute__((amdgpu_waves_per_eu(1, 1))) void attention_prefill_wide_kernel(
     const bf16_t* __restrict__ q, const bf16_t* __restrict__ k_cache, const bf16_t* __restrict__ v_cache,
     const int* __restrict__ block_table, int max_pages, const int* __restrict__ seq_slot,
     const int* __restrict__ seq_start, const int* __restrict__ seq_new, const int* __restrict__ cu_new, int nh,
-    int nkv, float scale_log2, int window, int qb, int hg, bf16_t* __restrict__ out, int kept) {
+    int nkv, float scale_log2, int window, int qb, int hg, bf16_t* __restrict__ out, More... more) {
     if constexpr (PF_WIDE) {
+        const int kept = (0 + ... + more);
         constexpr int K_TILE = PAGE_TOKENS * K_STRIDE, V_TILE = HD * V_STRIDE, PAGE_LOADS = 2 * PF_LOADS;
         constexpr int QK = 8 * KSTEPS, PV = 4 * DTILES + 4;         // products of a pair of units
         static_assert(QK == 32 && PV == 36 && PAGE_LOADS == 8, "what goes between which products below is laid out for heads of 128");
@@ -2057,7 +2133,8 @@ __global__ __launch_bounds__(PF_THREADS) __attribute__((amdgpu_waves_per_eu(1, 1
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const int key = tile_key(t, 0) + quad / 4 * 8 + i;
-                            s[pair][x][t][i] = key_is_seen<KEPT>(key, lo, hi, kept - page_first_key) ? s[pair][x][t][i] : -INFINITY;
+                            if constexpr (KEPT) s[pair][x][t][i] = key_is_seen(key, lo, hi, kept - page_first_key) ? s[pair][x][t][i] : -INFINITY;
+                            else s[pair][x][t][i] = (key >= lo && key <= hi) ? s[pair][x][t][i] : -INFINITY;
                             top[x] = fmaxf(top[x], s[pair][x][t][i]);
                         }
                 }
@@ -2240,7 +2317,7 @@ __global__ __launch_bounds__(PF_THREADS) __attribute__((amdgpu_waves_per_eu(1, 1
                 for (int x = 0; x < WIDE_UNITS; ++x) {
                     const int pos = start + min(first_query(x) + r, n_new - 1);
                     add_wild_values(v_cache + ((size_t)pages[page] * nkv + kvh) * PAGE_TOKENS * HD, o[x], g,
-                                    [&](int key) { return key_is_seen<true>(key, first_key(pos) - key0, pos - key0, kept - key0); });
+                                    [&](int key) { return key_is_seen(key, first_key(pos) - key0, pos - key0, kept - key0); });
                 }
             }
         }
@@ -2333,16 +2410,20 @@ static int launch_attention_prefill(hipStream_t stream, const void* q, const voi
         const long long blocks = (long long)grid.x * grid.y * grid.z;
         const bool few = halves ? halves == 2 : prefill_takes_halves(n_seqs, max_new, max_keys, nh, nkv, KEPT ? window + kept : window);
         const int partners_follow = !few && blocks <= 512 && n_seqs == 1;     // all blocks run at once, two a unit
+        auto launch = [&](auto... more) {
 #define PALM_PAIRED(HALVES, PRE) attention_prefill_paired_kernel<HALVES, PRE, KEPT><<<grid, HALVES * PF_THREADS, 0, stream>>>( \
         (const bf16_t*)q, (const bf16_t*)k_cache, (const bf16_t*)v_cache, block_table, max_pages, seq_slot, seq_start, seq_new, \
-        cu_new, nh, nkv, scale_log2, window, qb, hg, partners_follow, (bf16_t*)out, kept, slices, work, n_seqs, n_q)
-        if (few) { if (q_prescaled) PALM_PAIRED(2, true); else PALM_PAIRED(2, false); }
-        else { if (q_prescaled) PALM_PAIRED(1, true); else PALM_PAIRED(1, false); }
+        cu_new, nh, nkv, scale_log2, window, qb, hg, partners_follow, (bf16_t*)out, more...)
+            if (few) { if (q_prescaled) PALM_PAIRED(2, true); else PALM_PAIRED(2, false); }
+            else { if (q_prescaled) PALM_PAIRED(1, true); else PALM_PAIRED(1, false); }
 #undef PALM_PAIRED
+        };
+        if constexpr (KEPT) launch(kept, slices, work, n_seqs, n_q);
+        else launch();
         PALM_LAUNCHED();
-        if (slices > 1) {
+        if constexpr (KEPT) if (slices > 1) {
             const long long heads = (long long)rows * nh;
-            attention_prefill_join_kernel<<<(unsigned)((heads + JOIN_WAVES - 1) / JOIN_WAVES), JOIN_WAVES * WAVE, 0, stream>>>(work, slices, heads, (bf16_t*)out);
+            attention_prefill_join_kernel<KEPT><<<(unsigned)((heads + JOIN_WAVES - 1) / JOIN_WAVES), JOIN_WAVES * WAVE, 0, stream>>>(work, slices, heads, (bf16_t*)out);
             PALM_LAUNCHED();
         }
         return 0;
@@ -2352,13 +2433,18 @@ static int launch_attention_prefill(hipStream_t stream, const void* q, const voi
     const int n_tiles = subs > 1 ? ((n16 + 1) / 2 + subs / 2 - 1) / (subs / 2) : n16;
     PALM_CHECK(n_tiles <= 65535, "attention_prefill: %d new tokens are more than one launch takes", max_new);
     dim3 grid(nkv * n_hg, n_tiles, n_seqs);
-    attention_prefill_kernel<KEPT><<<grid, PF_THREADS, 0, stream>>>((const bf16_t*)q, (const bf16_t*)k_cache, (const bf16_t*)v_cache,
-                                                             block_table, max_pages, seq_slot, seq_start, seq_new, cu_new, nh,
-                                                             nkv, scale_log2, window, qb, hg, (bf16_t*)out, kept);
+    auto launch = [&](auto... more) {
+        attention_prefill_kernel<KEPT><<<grid, PF_THREADS, 0, stream>>>((const bf16_t*)q, (const bf16_t*)k_cache, (const bf16_t*)v_cache,
+                                                                 block_table, max_pages, seq_slot, seq_start, seq_new, cu_new, nh,
+                                                                 nkv, scale_log2, window, qb, hg, (bf16_t*)out, more...);
+    };
+    if constexpr (KEPT) launch(kept);
+    else launch();
     PALM_LAUNCHED();
     return 0;
 }
 
+#if PALM_WITHOUT_KEPT
 PALM_API int palm_attention_prefill_in(hipStream_t stream, const void* q, const void* k_cache, const void* v_cache,
                                        const int* block_table, int max_pages, const int* seq_slot, const int* seq_start,
                                        const int* seq_new, const int* cu_new, int n_seqs, int max_new, int nh, int nkv,
@@ -2366,6 +2452,15 @@ PALM_API int palm_attention_prefill_in(hipStream_t stream, const void* q, const 
     return launch_attention_prefill<false>(stream, q, k_cache, v_cache, block_table, max_pages, seq_slot, seq_start, seq_new, cu_new, n_seqs, max_new, nh, nkv, hd, scale,
                                            window, q_prescaled, max_keys, halves, out, 0, 0, 1, nullptr);
 }
+PALM_API int palm_attention_prefill(hipStream_t stream, const void* q, const void* k_cache, const void* v_cache,
+                                    const int* block_table, int max_pages, const int* seq_slot, const int* seq_start,
+                                    const int* seq_new, const int* cu_new, int n_seqs, int max_new, int nh, int nkv,
+                                    int hd, float scale, int window, int q_prescaled, void* out) {
+    return palm_attention_prefill_in(stream, q, k_cache, v_cache, block_table, max_pages, seq_slot, seq_start, seq_new, cu_new, n_seqs, max_new,
+                                     nh, nkv, hd, scale, window, q_prescaled, 0, 0, out);
+}
+#endif
+#if PALM_WITH_KEPT
 // The same with the sequences' first `kept` keys visible behind the window (> 0).  Each sequence's pages may be cut into slices whose
 // results meet in `work`: rows (of q) * nh * slices * (hd + 4) floats.
 PALM_API int palm_attention_prefill_kept(hipStream_t stream, const void* q, const void* k_cache, const void* v_cache,
@@ -2376,15 +2471,7 @@ PALM_API int palm_attention_prefill_kept(hipStream_t stream, const void* q, cons
     return launch_attention_prefill<true>(stream, q, k_cache, v_cache, block_table, max_pages, seq_slot, seq_start, seq_new, cu_new, n_seqs, max_new, nh, nkv, hd, scale,
                                            window, q_prescaled, max_keys, halves, out, kept, rows, slices, work);
 }
-
-PALM_API int palm_attention_prefill(hipStream_t stream, const void* q, const void* k_cache, const void* v_cache,
-                                    const int* block_table, int max_pages, const int* seq_slot, const int* seq_start,
-                                    const int* seq_new, const int* cu_new, int n_seqs, int max_new, int nh, int nkv,
-                                    int hd, float scale, int window, int q_prescaled, void* out) {
-    return palm_attention_prefill_in(stream, q, k_cache, v_cache, block_table, max_pages, seq_slot, seq_start, seq_new, cu_new, n_seqs, max_new,
-                                     nh, nkv, hd, scale, window, q_prescaled, 0, 0, out);
-}
-
+#endif
 PALM_API int palm_attention_prefill_takes_prescaled() { return PF_DMA ? 1 : 0; }
 
 // The same by the kernel for long prompts, where palm_attention_prefill_wide_serves() says so.
@@ -2403,14 +2490,19 @@ static int launch_attention_wide(hipStream_t stream, const void* q, const void* 
     PALM_CHECK(nkv * n_hg <= 65535 && n_seqs <= 65535 && (max_new + qb - 1) / qb <= 65535, "attention_prefill_wide: grid too large");
     const dim3 grid(nkv * n_hg, (max_new + qb - 1) / qb, n_seqs);       // (the kv head fastest: see palm_attention_prefill)
     const float scale_log2 = q_prescaled ? 1.0f : scale * LOG2E;
+    auto launch = [&](auto... more) {
 #define PALM_WIDE(PRE) attention_prefill_wide_kernel<PRE, KEPT><<<grid, PF_THREADS, 0, stream>>>( \
         (const bf16_t*)q, (const bf16_t*)k_cache, (const bf16_t*)v_cache, block_table, max_pages, seq_slot, seq_start, seq_new, \
-        cu_new, nh, nkv, scale_log2, window, qb, hg, (bf16_t*)out, kept)
-    if (q_prescaled) PALM_WIDE(true); else PALM_WIDE(false);
+        cu_new, nh, nkv, scale_log2, window, qb, hg, (bf16_t*)out, more...)
+        if (q_prescaled) PALM_WIDE(true); else PALM_WIDE(false);
 #undef PALM_WIDE
+    };
+    if constexpr (KEPT) launch(kept);
+    else launch();
     PALM_LAUNCHED();
     return 0;
 }
+#if PALM_WITHOUT_KEPT
 PALM_API int palm_attention_prefill_wide(hipStream_t stream, const void* q, const void* k_cache, const void* v_cache,
                                          const int* block_table, int max_pages, const int* seq_slot, const int* seq_start,
                                          const int* seq_new, const int* cu_new, int n_seqs, int max_new, int nh, int nkv,
@@ -2418,6 +2510,8 @@ PALM_API int palm_attention_prefill_wide(hipStream_t stream, const void* q, cons
     return launch_attention_wide<false>(stream, q, k_cache, v_cache, block_table, max_pages, seq_slot, seq_start, seq_new, cu_new, n_seqs, max_new, nh, nkv, hd, scale,
                                         window, q_prescaled, out, 0);
 }
+#endif
+#if PALM_WITH_KEPT
 // The same with the sequences' first `kept` keys visible behind the window (> 0).
 PALM_API int palm_attention_prefill_wide_kept(hipStream_t stream, const void* q, const void* k_cache, const void* v_cache,
                                          const int* block_table, int max_pages, const int* seq_slot, const int* seq_start,
@@ -2427,5 +2521,6 @@ PALM_API int palm_attention_prefill_wide_kept(hipStream_t stream, const void* q,
     return launch_attention_wide<true>(stream, q, k_cache, v_cache, block_table, max_pages, seq_slot, seq_start, seq_new, cu_new, n_seqs, max_new, nh, nkv, hd, scale,
                                         window, q_prescaled, out, kept);
 }
+#endif
 PALM_API int palm_attention_prefill_wide_serves() { return PF_WIDE ? 1 : 0; }
 

@@ -25,6 +25,7 @@ Libraries:
   ``delta_head_d<N>``   the delta rule with one decay a head behind short convolutions, compiled for key sizes up to N
   ``streams``           a residual stream in several copies with learned weights between them, and its norms
   ``attention_kept``    attention with a window and first positions that stay visible, in 32-bit, any head size
+  ``attention_kept_hd<N>``  the same on the matrix cores, compiled for one head size
   ``pages``             pages of the cache copied to other pages, in all layers at once
   ``logprobs``          log probabilities of given tokens, entropies and the likeliest tokens
   ``mlstm``             a matrix memory with input and forget gates per head and token
@@ -265,9 +266,11 @@ def _spec(name: str):
     if name.startswith("latent_attention_k"):
         kk, vt = name[len("latent_attention_k"):].split("_v")
         return LATENT_ATTENTION_SOURCES, (f"PALM_LAT_KK={int(kk)}", f"PALM_LAT_VT={int(vt)}")
+    if name.startswith("attention_kept_hd"):
+        return ATTENTION_SOURCES, (f"PALM_HEAD_DIM={int(name[len('attention_kept_hd'):])}", "PALM_KEPT=1")
     if name.startswith("attention_hd"):
         hd = int(name[len("attention_hd"):])
-        return ATTENTION_SOURCES, (f"PALM_HEAD_DIM={hd}",)
+        return ATTENTION_SOURCES, (f"PALM_HEAD_DIM={hd}", "PALM_KEPT=0")
     raise KeyError(name)
 
 

@@ -821,14 +821,19 @@ _ATTENTION_SIGNATURES = {
     "palm_attention_prefill_wide": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
                                     c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p],
     "palm_attention_prefill_wide_serves": [],
-    "palm_attention_prefill_wide_kept": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
-                                         c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p, c_int],
     "palm_attention_decode_fused": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_int,
                                     c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int,
                                     c_int, c_int, c_float, c_int, c_int, c_void_p, c_void_p],
     "palm_attention_decode_pages": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_int,
                                     c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int,
                                     c_int, c_float, c_int, c_void_p, c_void_p, c_void_p],
+    "palm_attention_decode_pages_serves": [c_int, c_int, c_int, c_int],
+    "palm_attention_decode_pages_work": [c_int, c_int],
+    "palm_attention_decode_fused_serves": [c_int, c_int],
+}
+_ATTENTION_KEPT_HD_SIGNATURES = {
+    "palm_attention_prefill_wide_kept": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
+                                         c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p, c_int],
     "palm_attention_decode_kept": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int,
                                    c_int, c_int, c_float, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p],
     "palm_attention_prefill_kept": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
@@ -840,30 +845,40 @@ _ATTENTION_SIGNATURES = {
     "palm_attention_decode_pages_kept": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_int,
                                          c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int,
                                          c_int, c_float, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p],
-    "palm_attention_decode_pages_serves": [c_int, c_int, c_int, c_int],
     "palm_attention_decode_pages_work": [c_int, c_int],
-    "palm_attention_decode_fused_serves": [c_int, c_int],
 }
 _attention_libs: dict = {}
+_attention_kept_libs: dict = {}
 MFMA_HEAD_DIMS = tuple(range(16, 257, 16))
 DECODE_WAVES_WANTED = 768         # slices of the key range are made until about this many waves run (measured best)
 
 
+def _attention_lib(name: str, hd: int, signatures: dict):
+    if hd not in MFMA_HEAD_DIMS:
+        raise KernelError(f"the matrix-core attention kernels take head sizes in steps of 16 up to 256, not {hd}")
+    lib = library.load(name)
+    for fn_name, argtypes in signatures.items():
+        fn = getattr(lib, fn_name)
+        fn.argtypes, fn.restype = argtypes, c_int
+    if lib.palm_attention_head_dim() != hd:
+        raise KernelError(f"library {name} was built for head size {lib.palm_attention_head_dim()}")
+    if lib.palm_attention_page_tokens() != PAGE_TOKENS:
+        raise KernelError(f"library {name} was built for pages of {lib.palm_attention_page_tokens()} tokens, "
+                          f"the cache has pages of {PAGE_TOKENS}")
+    return lib
+
+
 def attention_lib(hd: int):
     if hd not in _attention_libs:
-        if hd not in MFMA_HEAD_DIMS:
-            raise KernelError(f"the matrix-core attention kernels take head sizes in steps of 16 up to 256, not {hd}")
-        lib = library.load(f"attention_hd{hd}")
-        for name, argtypes in _ATTENTION_SIGNATURES.items():
-            fn = getattr(lib, name)
-            fn.argtypes, fn.restype = argtypes, c_int
-        if lib.palm_attention_head_dim() != hd:
-            raise KernelError(f"library attention_hd{hd} was built for head size {lib.palm_attention_head_dim()}")
-        if lib.palm_attention_page_tokens() != PAGE_TOKENS:
-            raise KernelError(f"library attention_hd{hd} was built for pages of {lib.palm_attention_page_tokens()} tokens, "
-                              f"the cache has pages of {PAGE_TOKENS}")
-        _attention_libs[hd] = lib
+        _attention_libs[hd] = _attention_lib(f"attention_hd{hd}", hd, _ATTENTION_SIGNATURES)
     return _attention_libs[hd]
+
+
+def attention_kept_hd_lib(hd: int):
+    """The same kernels with first positions that stay visible behind the window."""
+    if hd not in _attention_kept_libs:
+        _attention_kept_libs[hd] = _attention_lib(f"attention_kept_hd{hd}", hd, _ATTENTION_KEPT_HD_SIGNATURES)
+    return _attention_kept_libs[hd]
 
 
 def mfma_attention_serves(q: torch.Tensor, hd: int) -> bool:
@@ -1023,7 +1038,7 @@ def attention_decode_fused(qkv, k_cache, v_cache, block_table, seq_slot, seq_sta
         _i32(what, arrivals)
         if not (arrivals.is_contiguous() and arrivals.numel() >= B * nh):
             raise KernelError(f"{what}: {arrivals.numel()} counters for {B} sequences x {nh} heads")
-        lib = attention_lib(hd)
+        lib = attention_kept_hd_lib(hd) if kept else attention_lib(hd)
         work = torch.empty((lib.palm_attention_decode_pages_work(nh, nkv),), dtype=F32, device=qkv.device)
         library.call(lib, "palm_attention_decode_pages_kept" if kept else "palm_attention_decode_pages", _stream(), _p(qkv), int(as_planes),
                      qkv.shape[0] if as_planes else 1, _p(q_norm_w), _p(k_norm_w), float(eps), _p(cos), _p(sin),
@@ -1032,7 +1047,8 @@ def attention_decode_fused(qkv, k_cache, v_cache, block_table, seq_slot, seq_sta
                      int(window or 0), _p(work), _p(arrivals), _p(out), *more, *(more and (None, None)))
         return out
     work = _slices_workspace(what, work, B, nh, n_slices, hd, qkv.device)
-    library.call(attention_lib(hd), "palm_attention_decode_fused_kept" if kept else "palm_attention_decode_fused", _stream(), _p(qkv), int(as_planes),
+    library.call(attention_kept_hd_lib(hd) if kept else attention_lib(hd), "palm_attention_decode_fused_kept" if kept else "palm_attention_decode_fused",
+                 _stream(), _p(qkv), int(as_planes),
                  qkv.shape[0] if as_planes else 1, _p(q_norm_w), _p(k_norm_w), float(eps), _p(cos), _p(sin),
                  int(rotary_dim if cos is not None else 0), int(pairing), int(write_cache), _p(k_cache), _p(v_cache),
                  _p(block_table), block_table.shape[1], _p(seq_slot), _p(seq_start), B, nh, nkv, hd, float(scale),
@@ -2953,7 +2969,7 @@ def attention_kept(q: torch.Tensor, k_cache, v_cache, block_table, seq_slot, seq
     out = torch.empty_like(q)
     if n == 0 or B == 0 or max_new == 0:
         return out
-    lib = attention_lib(hd)
+    lib = attention_kept_hd_lib(hd)
     if max_new == 1 and not q_prescaled:
         keys = _kept_keys(max(1, max_total), window, kept)
         if (kept_by_pages(B, nkv, hd, keys) if by_pages is None else by_pages) and decode_pages_serves(B, nh, nkv, hd, block_table.shape[1]):

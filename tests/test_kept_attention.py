@@ -463,3 +463,15 @@ def test_the_windows_first_key_alone_on_its_page_is_no_number(ops, nh, nkv, hd, 
     case.k[case.place(0, 64 * 5 + 63)[0], 0, 63] = what
     for way in _ways(ops, dtype, hd, True):
         case.check(case.run(ops, **way))
+
+
+@pytest.mark.parametrize("hd", [64, 128, 80])
+def test_the_kernels_without_first_positions_are_a_library_of_their_own(ops, hd):
+    """The code of those with them would lie between, and decode steps that never run it took longer."""
+    plain, kept = ops.attention_lib(hd), ops.attention_kept_hd_lib(hd)
+    for name in ("decode", "decode_fused", "decode_pages", "prefill_wide"):
+        assert hasattr(plain, f"palm_attention_{name}") and not hasattr(plain, f"palm_attention_{name}_kept")
+        assert hasattr(kept, f"palm_attention_{name}_kept") and not hasattr(kept, f"palm_attention_{name}")
+    assert plain.palm_attention_decode_pages_work(32, 8) == kept.palm_attention_decode_pages_work(32, 8)
+    with pytest.raises(ops.KernelError, match="steps of 16"):
+        ops.attention_kept_hd_lib(72)
