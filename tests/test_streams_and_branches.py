@@ -329,3 +329,42 @@ def test_branches_of_designs_whose_convolutions_have_one_tap(preset, dtype):
     assert torch.equal(run(False), run(True))
     results, _ = eng.generate([ids[:9]], answers=2, temperature=0.0, max_new_tokens=3, ignore_eos=True)
     assert results[0].token_ids == results[1].token_ids and len(results[0].token_ids) == 3
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_the_totals_that_choose_among_answers_are_the_answers_own(model_dirs, dtype):
+    """Each answer's log probabilities against 64 bits of the logits of the very steps that drew it, made again: the prompt once, the same forks, the four tokens together.
+
+    Bounds.  The same steps give the same logits, so a log probability is off by the operator's own rounding, (V / 512 + 160 + 4 |log p|) 2^-24 (tests of
+    ``token_logprobs``), a total by the sum of those.  Scoring the whole answer in pieces is another pass: logits of two passes are each within the gate's 5 % of
+    their mean square of the exact ones (bfloat16; 1e-4 in float32), a log probability is a logit less a mean of logits, so a total of 60 is off by 60 x 2 x 2 of that
+    if every error had one sign."""
+    from palm_infra_amd.engine import StepEntry
+    eng = engine_for(model_dirs, "D", dtype, 40, 4, max_tokens=64 * 120, stream_tokens=64 * 150)
+    prompt = tiny.prompts("D", [150], seed=8)[0]
+    got, _ = eng.generate([prompt], answers=4, max_new_tokens=60, ignore_eos=True, temperature=0.9, seed=7, logprobs=0)
+    slot = eng.open()
+    logits = eng.step([StepEntry(slot, prompt, [len(prompt) - 1])])
+    slots = [slot] + eng.fork(slot, 3)
+    rows = [logits.repeat_interleave(4, dim=0)]
+    for t in range(59):
+        rows.append(eng.step([StepEntry(s, [r.token_ids[t]], [0]) for s, r in zip(slots, got)]).clone())
+    for s in slots:
+        eng.close(s)
+    rows = torch.stack(rows).double().cpu()                                     # [tokens, answers, vocabulary]
+    tokens = torch.tensor([r.token_ids for r in got]).T
+    exact = torch.log_softmax(rows, -1).gather(2, tokens[..., None])[..., 0]
+    told = torch.tensor([r.scores.logprobs for r in got], dtype=torch.float64).T
+    off = (rows.shape[2] / 512 + 160 + 4 * exact.abs()) * 2.0 ** -24
+    assert bool(((told - exact).abs() <= off).all())
+    totals, room = exact.sum(0), float(off.sum(0).max())
+    best = max(range(4), key=lambda i: got[i].scores.total)
+    assert float(totals[best]) >= float(totals.max()) - 2 * room
+    # (another answer's total is not within it: the comparison tells them apart)
+    assert float((totals.sort().values[1:] - totals.sort().values[:-1]).min()) > 4 * room
+    logit_off = 1e-4 if dtype == "float32" else tiny.BFLOAT16_RMS_REL * float(rows.pow(2).mean().sqrt())
+    rescored = [sum(s.logprobs[len(prompt) - 1:]) for s in eng.score([prompt + r.token_ids for r in got])]
+    bound = 60 * 2 * 2 * logit_off
+    assert all(abs(r.scores.total - s) <= bound for r, s in zip(got, rescored))
+    assert rescored[best] >= max(rescored) - 2 * bound
