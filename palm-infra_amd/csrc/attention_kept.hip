@@ -92,10 +92,12 @@ struct SeenRow {
 //
 // Up to 128 elements a head (AHEAD) a page's keys are asked for together, and its values as the keys' registers come free: a wave has few pages, and
 // what it waits for memory is what a short prompt takes.  A page is 256 products of 32 clocks for heads of 128, 3.4 us of a wave.  A prompt of
-// 157 tokens, 32 heads of 128 over 8, a window of 64 takes 13.7 us (20.6 with reads behind branches, waited for one by one; 32 with two pages' reads in flight
-// and half the waves), 8.0 with heads of 64; 600 tokens with a window of 512: 76 us, 38 TFLOP/s, bounded by the products' own rate and the
-// causal half of each page that is computed and masked.  Longer heads have no registers for it and read as they go: heads of 256 take 53 us for the
-// 157 tokens.
+// 157 tokens, 32 heads of 128 over 8, a window of 64 takes 13.3 us (20.6 with reads behind branches, waited for one by one; 32 with two pages' reads in flight
+// and half the waves), 7.7 with heads of 64, 19.5 with heads of 90; 600 tokens with a window of 512: 76 us, 38 TFLOP/s of what is seen.  There the matrix cores
+// are at work a quarter of the time (an eighth of it for keys of whole pages that are masked): a SIMD has 1.1 waves in the mean of the two it has places
+// for, and a compute unit none for a third of the time, because rows of one to ten pages are dealt to four waves, 1,200 blocks come in 2.3 rounds, and a wave's
+// first page is waited for.  Longer heads have no registers for a page ahead and read as they go: heads of 256 take 52 us for the 157 tokens.  One token behind 5,000 in
+// a window of 2,048 takes 22 us, 48 of 300 to 9,000 tokens 166.
 template <typename T, int DT, Rows ROWS>
 __global__ __launch_bounds__(KA_WAVES * WAVE) __attribute__((amdgpu_waves_per_eu(DT <= 8 ? 2 : 1))) void attention_kept_kernel(
     const T* __restrict__ q, const T* __restrict__ k_cache, const T* __restrict__ v_cache, const int* __restrict__ block_table, int max_pages,

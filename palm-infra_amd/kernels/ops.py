@@ -3025,13 +3025,16 @@ def kept_plan(rows: int, n_seqs: int, max_total: int, nh: int, nkv: int, hd: int
 
     A block holds 128 columns, (position, head) pairs of a kv head, and walks its row of pages.  With one half two blocks share a compute unit; with
     two, which take every other page, it has it to itself.  Slices are blocks of their own whose results a second kernel joins: it starts in some 5 us
-    and passes every slice's output through memory.  us, (halves, slices): 64 tokens behind 6,000, window 4,096, 32 heads of 128 on 8 (16 blocks of 66 pages) (1, 1) 121,
-    (2, 1) 89, (2, 4) 34, (2, 12) 26, (2, 16) 28; 517 behind 6,000, window 1,000 (136 blocks of 19) 42, 36, 49, (1, 3) 35; 16 heads of 64 on 4 (68 blocks) 30, 26,
-    (2, 3) 20; 7 behind 8,000 in a window of 8,000 (8 blocks of 126) 185, 137, (2, 16) 25; three times 700 behind 5,000 to 9,000, window 2,048 (528 of 34) 151, 151,
-    (1, 2) 130; 1,000 from the start, window 128 (256 of 4) 19, 17, (2, 2) 36; 8,192, window 2,048 (2,048 of 34) 291, 351.
+    and passes every slice's output through memory.  us, (halves, slices), 32 heads of 128 on 8 if nothing is said: 64 tokens behind 6,000, window 4,096 (16 blocks of
+    66 pages) (1, 1) 115, (2, 1) 86, (2, 4) 32, (2, 12) 24, (2, 16) 25; 517 behind 6,000, window 1,000 (136 blocks of 19) (1, 1) 37, (2, 1) 32, (1, 2) 35, (2, 2) 42,
+    (1, 3) 32; with 16 heads of 64 (68 blocks) (1, 1) 28, (2, 1) 23, (2, 2) 19, (2, 3) 19, (2, 4) 25; 7 behind 8,000 in a window of 8,000 (8 blocks of 126) (1, 1) 178,
+    (2, 1) 132, (2, 8) 28, (2, 16) 23; three times 700 behind 5,000 to 9,000, window 2,048 (528 of 34) (1, 1) 139, (2, 1) 144, (1, 2) 138; 1,000 from the start, window
+    128 (256 of 4) (1, 1) 16, (2, 1) 16, (1, 2) 26; 8,192, window 2,048 (2,048 of 34) (1, 1) 262, (2, 1) 325, (1, 2) 366.
 
-    The other kernel is sooner where rows are long, blocks many and its sixteen units all used (16 heads of 128 on 2, 16,000 tokens, window 8,192: 670 and 768; 32 on
-    8, 5,000, window 4,000: 198 and 213; 8,192, window 4,096 428 and 432, 2,048 328 and 291)."""
+    The other kernel is sooner where rows are long, blocks many and its sixteen units all used.  us, (1, 1) and the other: 16 heads of 128 on 2, 16,000 tokens, window 8,192
+    776 and 733; 32 on 8, 16,000 in 8,192 1,533 and 1,438, in 4,096 961 and 983; 8,192 in 4,096 426 and 423, in 2,048 262 and 266; twice 4,096 280 and 262; 5,000 in
+    4,000 206 and 208; 64 on 8, 8,192 in 8,192 1,046 and 935.  Its blocks are half as many, which the rule does not look at: 2,048 behind 8,000 151 and 153, 8 heads
+    on 8, 8,192 in 4,096 (256 of them) 130 and 169, and it is taken."""
     if hd not in (64, 128):
         return False, 0, 1
     group = nh // nkv
@@ -3042,7 +3045,8 @@ def kept_plan(rows: int, n_seqs: int, max_total: int, nh: int, nkv: int, hd: int
     pages = -(-keys // PAGE_TOKENS)
     if hd == 128 and pages >= 64 and 16 % group == 0 and blocks >= 512 and attention_lib(hd).palm_attention_prefill_wide_serves():
         return True, 0, 1
-    # Fitted to 62 such steps: the way taken is 2 % slower than the best of them in the mean.  A page takes 1.6 us where one half has the unit to itself, 1.75
+    # Fitted to 62 such steps, when a page of edges took longer than it does now; of the 17 steps timed since, the way taken is the best of those tried in ten, up to 4 % slower in six,
+    # and 30 % in the one told above.  A page takes 1.6 us where one half has the unit to itself, 1.75
     # beside another block, 0.97 by two halves, and 0.8 of it more for up to four pages with masks.  Blocks beyond those that run at once come in further
     # rounds, which prompts from their start, whose first tiles are short, do not fill.
     page = 0.3 + 0.7 * hd / 128
